@@ -8,6 +8,11 @@ from .api import sparse_attention_warmup_varlen as flash_msa_warmup_varlen_func
 from .api import sparse_attention_warmup as flash_msa_func_warmup
 from .api import sparse_attention_warmup as flash_msa_warmup_func
 from .api import check_pending_status, last_kl_value
+from .serving import cache_append as flash_msa_cache_append
+from .serving import cache_attention as flash_msa_cache_func
+from .serving import cache_empty as flash_msa_cache_empty
+from .serving import cache_evict as flash_msa_cache_evict
+from .serving import cache_unpack as flash_msa_cache_unpack
 
 __all__ = [
     "flash_msa_func",
@@ -18,4 +23,9 @@ __all__ = [
     "sparse_attention_warmup",
     "last_kl_value",
     "check_pending_status",
+    "flash_msa_cache_append",
+    "flash_msa_cache_empty",
+    "flash_msa_cache_evict",
+    "flash_msa_cache_func",
+    "flash_msa_cache_unpack",
 ]

@@ -347,3 +347,24 @@ extern "C" int fmsa_doc_start(const int32_t* boundaries, int32_t n, int32_t per_
         D, doc_start, S);
     return check_launch();
 }
+
+// The boundaries themselves to device memory, for kernels that read them there.
+namespace fmsa {
+namespace {
+__global__ void __launch_bounds__(256) boundaries_kernel(const __grid_constant__ DocBounds D, int32_t* __restrict__ dst) {
+    for (int i = threadIdx.x; i < D.n; i += 256) dst[i] = D.at[i];
+}
+}  // namespace
+}  // namespace fmsa
+
+extern "C" int fmsa_boundaries(const int32_t* boundaries, int32_t n, int32_t* dst, void* stream) {
+    using namespace fmsa;
+    FMSA_REQUIRE(boundaries && dst && n > 0);
+    if (n > FMSA_MAX_HOST_BOUNDARIES) return FMSA_ERR_UNSUPPORTED;
+    DocBounds D;
+    D.n = n;
+    D.per_batch = 0;
+    for (int32_t i = 0; i < n; ++i) D.at[i] = boundaries[i];
+    boundaries_kernel<<<1, 256, 0, static_cast<cudaStream_t>(stream)>>>(D, dst);
+    return check_launch();
+}

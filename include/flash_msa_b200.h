@@ -340,6 +340,49 @@ int fmsa_backward(const fmsa_backward_args* args, fmsa_marks* marks, int32_t* la
 #define FMSA_MAX_HOST_BOUNDARIES 896
 int fmsa_doc_start(const int32_t* boundaries, int32_t n, int32_t per_batch, int32_t B, int32_t S, int32_t* doc_start, void* stream);
 
+/* ---- Serving: a key/value cache held in 4 bits (no counterpart in the reference, which trains) ----
+ *
+ * The cache is a pool of pages of FMSA_CACHE_PAGE tokens, records[pages][heads][FMSA_CACHE_RECORD_BYTES]: per KV head K codes
+ * [128][64 bytes], K scales bf16 [128][4], V codes [128][64 bytes], V scales bf16 [128][4]; a value is (nibble - 8) * the scale of its
+ * token and group of 32 channels (order of the nibbles inside a row: csrc/cache4.cuh).  Sequence i holds lengths[i] tokens, token j in page
+ * block_table[i][j / 128] at slot j % 128.  Table and lengths are device memory: nothing waits for the device.  Lengths beyond
+ * width * 128 count as that; a page outside 0 .. pages-1 is not touched and status becomes 2. */
+#define FMSA_CACHE_PAGE 128
+#define FMSA_CACHE_RECORD_BYTES 18432
+typedef struct {
+    void* records;
+    const int32_t *block_table, *lengths; /* [seqs][width], rows table_stride apart; [seqs] */
+    int64_t table_stride;
+    int32_t pages, heads, seqs, width;
+} fmsa_cache4;
+
+/* Stores new keys and values (B,heads,n,128).  `lengths` count them already.  cu_seqlens NULL: the n rows of batch element i are the last
+ * n tokens of sequence i (B = seqs); rows for which a sequence has no place (lengths[i] < n) are left out.  cu_seqlens [seqs+1] (B = 1):
+ * rows cu_seqlens[i] .. cu_seqlens[i+1]-1 are the last tokens of sequence i; rows in no sequence are left out.
+ * weights fp32 [pages][heads][128] or NULL: set to zero for the stored tokens.  k_values, v_values: NULL, or (B,heads,n,128) views that
+ * receive the values the cache now holds (zero for rows left out). */
+int fmsa_cache_append(const fmsa_cache4* cache, const fmsa_tensor* k, const fmsa_tensor* v, int32_t B, int32_t n, int32_t dtype,
+                      const int32_t* cu_seqlens, float* weights, const fmsa_tensor* k_values, const fmsa_tensor* v_values, int32_t* status,
+                      void* stream);
+
+/* Attention of the last n tokens of every sequence over the cache: query j of q (seqs,Hq,n,128) sees the first lengths[i] - n + 1 + j
+ * tokens; a row that sees none is zero.  out [seqs][n][Hq*128] contiguous.  sinks fp32 [Hq] or NULL, as in fmsa_forward_args.
+ * weights fp32 [pages][heads][128] or NULL: for every token below lengths[i] the probability it got, summed over the rows of its KV
+ * head, is added (accumulate = 1) or written (0).  Two launches, three with weights.  workspace 256-byte aligned. */
+int64_t fmsa_cache_attend_workspace_bytes(int32_t seqs, int32_t Hq, int32_t heads, int32_t n);
+int fmsa_cache_attend(const fmsa_cache4* cache, const fmsa_tensor* q, int32_t Hq, int32_t n, float scale, int32_t dtype, const float* sinks,
+                      float* weights, int32_t accumulate, void* out, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+
+/* Eviction by accumulated attention weight: of every sequence and KV head min(lengths[i], keep) tokens stay, the last `recent` ones and
+ * the others of largest weight (of equal ones the first, NaN above everything), in their order; they are copied, weights with them, to
+ * new_table [seqs][new_width] (pages that no row of block_table names; new_width * 128 >= keep).  new_lengths [seqs];
+ * kept int32 [seqs][heads][keep]: where they were, -1 behind the last.  Two launches. */
+int fmsa_cache_evict(const fmsa_cache4* cache, float* weights, const int32_t* new_table, int64_t new_table_stride, int32_t new_width,
+                     int32_t keep, int32_t recent, int32_t* new_lengths, int32_t* kept, int32_t* status, void* stream);
+
+/* Boundaries in HOST memory to the device, as a kernel parameter (at most FMSA_MAX_HOST_BOUNDARIES). */
+int fmsa_boundaries(const int32_t* boundaries, int32_t n, int32_t* dst, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

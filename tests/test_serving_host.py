@@ -1,0 +1,113 @@
+"""Host side of the serving operators, without a GPU: refusals, boundaries, the layout of the cache."""
+import ctypes
+
+import pytest
+import torch
+
+import flash_msa_b200 as fm
+from flash_msa_b200 import _lib, serving
+from tests import serving_ref as R
+
+F = torch.float32
+BF = torch.bfloat16
+
+
+def test_constants_of_the_header():
+    import re
+    with open(_lib.HEADER_PATH) as f:
+        text = f.read()
+    for name, value in (("FMSA_CACHE_PAGE", serving.PAGE), ("FMSA_CACHE_RECORD_BYTES", serving.RECORD_BYTES)):
+        assert int(re.search(rf"#define {name}\s+(\d+)", text).group(1)) == value
+
+
+def test_unpack_reads_what_the_layout_says():
+    g = torch.Generator().manual_seed(1)
+    cache = torch.randint(0, 256, (2, 3, serving.RECORD_BYTES), generator=g, dtype=torch.uint8)
+    for lo, hi in ((8192, 9216), (17408, 18432)):
+        cache[..., lo:hi] = (torch.rand(2, 3, 512, generator=g) + 0.1).to(BF).view(torch.uint8)
+    k, v = fm.flash_msa_cache_unpack(cache)
+    assert k.shape == v.shape == (2, 3, 128, 128)
+    assert torch.equal(k.double(), R.unpack(cache, "k")) and torch.equal(v.double(), R.unpack(cache, "v"))
+    row = torch.randn(128, generator=g).to(BF)
+    rec = torch.zeros(serving.RECORD_BYTES, dtype=torch.uint8)
+    for slot in (0, 5, 127):
+        R.pack_into(rec, slot, "k", row)
+        R.pack_into(rec, slot, "v", row)
+        q, s = R.quantize(row)
+        want = (q.unflatten(-1, (4, 32)) * s.unsqueeze(-1)).flatten()
+        got = fm.flash_msa_cache_unpack(rec)
+        assert torch.equal(got[0][slot].double(), want) and torch.equal(got[1][slot].double(), want)
+        assert ((want - row.double()).abs().view(4, 32) <= s.view(4, 1) / 2 + 2.0 ** -8 * row.double().abs().view(4, 32)).all()
+
+
+def _call(what, **change):
+    """A call of the operator on CPU tensors that is right but for the device, with arguments replaced."""
+    a = dict(cache=torch.zeros(4, 2, serving.RECORD_BYTES, dtype=torch.uint8), k=torch.zeros(3, 2, 1, 128, dtype=BF),
+             v=torch.zeros(3, 2, 1, 128, dtype=BF), q=torch.zeros(3, 4, 1, 128, dtype=BF), table=torch.zeros(3, 2, dtype=torch.int32),
+             lengths=torch.ones(3, dtype=torch.int32), weights=torch.zeros(4, 2, 128), new=torch.zeros(3, 1, dtype=torch.int32), keep=100,
+             recent=10, cu=None, sinks=None)
+    a.update(change)
+    if what == "append":
+        return fm.flash_msa_cache_append(a["cache"], a["k"], a["v"], a["table"], a["lengths"], cu_seqlens=a["cu"], weights=a["weights"])
+    if what == "attend":
+        return fm.flash_msa_cache_func(a["q"], a["cache"], a["table"], a["lengths"], 0.1, sinks=a["sinks"], weights=a["weights"])
+    return fm.flash_msa_cache_evict(a["cache"], a["weights"], a["table"], a["lengths"], a["new"], a["keep"], a["recent"])
+
+
+def z(*shape, dtype=BF):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+COMMON = [
+    (dict(cache=z(4, 2, 100, dtype=torch.uint8)), ValueError), (dict(cache=z(4, 2, 18432)), ValueError),
+    (dict(cache=z(4, 4, 18432, dtype=torch.uint8)[:, ::2]), ValueError), (dict(cache=z(0, 2, 18432, dtype=torch.uint8), weights=z(0, 2, 128, dtype=F)), ValueError),
+    (dict(table=z(3, 2, dtype=torch.int64)), TypeError), (dict(table=z(3, dtype=torch.int32)), TypeError),
+    (dict(table=z(2, 3, dtype=torch.int32).T), ValueError), (dict(table=z(3, 0, dtype=torch.int32)), ValueError),
+    (dict(lengths=z(3, dtype=torch.int64)), TypeError), (dict(lengths=z(2, dtype=torch.int32)), ValueError),
+    (dict(lengths=z(6, dtype=torch.int32)[::2]), ValueError), (dict(weights=z(4, 2, 128)), ValueError),
+    (dict(weights=z(4, 2, 127, dtype=F)), ValueError), (dict(weights=z(4, 2, 256, dtype=F)[..., ::2]), ValueError), (dict(), RuntimeError)]
+APPEND = [
+    (dict(k=z(3, 2, 1, 64)), NotImplementedError), (dict(k=z(3, 2, 128)), ValueError), (dict(k=z(3, 2, 1, 128, dtype=F)), TypeError),
+    (dict(v=z(3, 2, 1, 128, dtype=torch.float16)), TypeError), (dict(v=z(3, 2, 2, 128)), ValueError),
+    (dict(k=z(3, 1, 1, 128), v=z(3, 1, 1, 128)), ValueError), (dict(k=z(2, 2, 1, 128), v=z(2, 2, 1, 128)), ValueError),
+    (dict(cu=[0, 1, 1, 1]), ValueError), (dict(cu=[0, 1, 1], k=z(1, 2, 5, 128), v=z(1, 2, 5, 128)), ValueError),
+    (dict(k=z(3, 2, 1, 128).requires_grad_()), RuntimeError)]
+ATTEND = [
+    (dict(q=z(3, 5, 1, 128)), ValueError), (dict(q=z(3, 0, 1, 128)), ValueError), (dict(q=z(2, 4, 1, 128)), ValueError), (dict(q=z(3, 4, 1, 64)), NotImplementedError),
+    (dict(q=z(3, 4, 1, 128, dtype=F)), TypeError), (dict(sinks=z(3, dtype=F)), ValueError), (dict(q=z(3, 4, 1, 128).requires_grad_()), RuntimeError)]
+EVICT = [
+    (dict(keep=0), ValueError), (dict(recent=101), ValueError), (dict(recent=-1), ValueError), (dict(keep=129, recent=0), ValueError),
+    (dict(new=z(2, 1, dtype=torch.int32)), ValueError), (dict(new=z(3, 1, dtype=torch.int64)), TypeError), (dict(weights=None), ValueError)]
+
+
+@pytest.mark.parametrize("what,change,error", [(w, c, e) for w, more in (("append", APPEND), ("attend", ATTEND), ("evict", EVICT))
+                                               for c, e in COMMON + more])
+def test_refusals(what, change, error):
+    with pytest.raises(error):
+        _call(what, **change)
+
+
+@pytest.mark.parametrize("cu", [[0, 3, 2], [1, 3], [0, 9], [0], [[[0, 1]]]])
+def test_boundaries_that_are_refused(cu):
+    with pytest.raises(ValueError):
+        serving._boundaries(cu, 8, torch.device("cpu"))
+
+
+def test_c_entries_refuse_before_they_touch_anything():
+    lib = _lib.load()
+    c = _lib.FmsaCache4(0x10, 0x10, 0x10, 2, 4, 2, 3, 2)     # (never dereferenced)
+    t = _lib.FmsaTensor(0x10, 256, 128, 128)
+    r = ctypes.byref
+    assert lib.fmsa_cache_append(r(c), r(t), r(t), 2, 1, 0, None, None, None, None, 0x10, None) == -1        # B is not seqs
+    assert lib.fmsa_cache_append(r(c), r(t), r(t), 3, 1, 7, None, None, None, None, 0x10, None) == -1        # type
+    assert lib.fmsa_cache_append(r(c), r(t), r(t), 3, 1, 0, None, None, r(t), None, 0x10, None) == -1        # one of two outputs
+    odd = _lib.FmsaTensor(0x12, 256, 128, 128)
+    assert lib.fmsa_cache_append(r(c), r(odd), r(t), 3, 1, 0, None, None, None, None, 0x10, None) == -1      # off the 16-byte grid
+    assert lib.fmsa_cache_append(r(c), r(t), r(t), 3, 1 << 30, 0, None, None, None, None, 0x10, None) == -2
+    assert lib.fmsa_cache_evict(r(c), 0x10, 0x10, 1, 1, 129, 0, 0x10, 0x10, 0x10, None) == -1                # no room for keep
+    assert lib.fmsa_cache_evict(r(c), 0x10, 0x10, 1, 1, 100, 101, 0x10, 0x10, 0x10, None) == -1
+    assert lib.fmsa_cache_attend(r(c), r(t), 5, 1, 1.0, 0, None, None, 0, 0x10, 0x100, 1 << 30, 0x10, None) == -1
+    bad = _lib.FmsaCache4(0x10, 0x10, 0x10, 2, 0, 2, 3, 2)
+    assert lib.fmsa_cache_evict(r(bad), 0x10, 0x10, 1, 1, 100, 0, 0x10, 0x10, 0x10, None) == -1
+    assert lib.fmsa_boundaries(None, 3, None, None) == -1
+    assert lib.fmsa_boundaries((ctypes.c_int32 * 4)(), 897, 0x10, None) == -2
