@@ -13,6 +13,7 @@ from .serving import cache_attention as flash_msa_cache_func
 from .serving import cache_empty as flash_msa_cache_empty
 from .serving import cache_evict as flash_msa_cache_evict
 from .serving import cache_unpack as flash_msa_cache_unpack
+from .serving import prompt_attention as flash_msa_prompt_func
 
 __all__ = [
     "flash_msa_func",
@@ -28,4 +29,5 @@ __all__ = [
     "flash_msa_cache_evict",
     "flash_msa_cache_func",
     "flash_msa_cache_unpack",
+    "flash_msa_prompt_func",
 ]

@@ -126,6 +126,10 @@ def _declare(lib):
     lib.fmsa_cache_attend.argtypes = [CA, T, c_int32, c_int32, c_float, c_int32, P, P, c_int32, P, P, c_int64, P, P]
     lib.fmsa_cache_evict.restype = c_int
     lib.fmsa_cache_evict.argtypes = [CA, P, P, c_int64, c_int32, c_int32, c_int32, P, P, P, P]
+    lib.fmsa_prompt_workspace_bytes.restype = c_int64
+    lib.fmsa_prompt_workspace_bytes.argtypes = [c_int32, c_int32, c_int32, c_int32, c_int32]
+    lib.fmsa_prompt_fwd.restype = c_int
+    lib.fmsa_prompt_fwd.argtypes = [T, T, T, c_int32, c_int32, c_int32, c_int32, P, c_int32, c_int32, c_float, c_int32, P, P, P, c_int64, P, P]
     lib.fmsa_boundaries.restype = c_int
     lib.fmsa_boundaries.argtypes = [P, c_int32, P, P]
     lib.fmsa_copy2d_async.restype = c_int

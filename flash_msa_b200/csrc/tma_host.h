@@ -55,6 +55,22 @@ inline bool make_tmap_bhsd(CUtensorMap* map, const void* base, uint64_t B, uint6
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// The same activation for boxes of `box_heads` neighbouring heads times `box_rows` positions: a map {128, H, S, B}, so that the heads of a
+// position are neighbouring rows of the tile.
+inline bool make_tmap_heads(CUtensorMap* map, const void* base, uint64_t B, uint64_t H, uint64_t S, int64_t stride_b, int64_t stride_h,
+                            int64_t stride_s, uint32_t box_heads, uint32_t box_rows) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[4] = {128, H, S, B};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(stride_h) * 2, static_cast<cuuint64_t>(stride_s) * 2,
+                                   static_cast<cuuint64_t>(stride_b) * 2};
+    const cuuint32_t box[4] = {64, box_heads, box_rows, 1};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Row-gather view of a (B, H, S, 128) bf16 activation whose strides are all multiples of 128 elements: a
 // 2-D matrix of 256-byte rows in which element row (b, h, s) has index (b*stride_b + h*stride_h +
 // s*stride_s) / 128.  Box = 64 columns x 1 row, 128-byte swizzle: the form tile::gather4 loads take.

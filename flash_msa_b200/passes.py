@@ -287,7 +287,7 @@ class StatusBoard:
     kinds of call, shared by all threads, streams and devices: it says what kind of call met trouble, not whose it was, and the
     RuntimeError is raised by whichever call of the library comes next, or by `drain`."""
     KINDS = ("flash_msa_func forward", "flash_msa_func backward", "flash_msa_warmup_func forward", "flash_msa_warmup_func backward",
-             "flash_msa_cache_append", "flash_msa_cache_func", "flash_msa_cache_evict")
+             "flash_msa_cache_append", "flash_msa_cache_func", "flash_msa_cache_evict", "flash_msa_prompt_func")
 
     def __init__(self):
         self._words = None

@@ -1,5 +1,5 @@
-"""Serving: a key/value cache held in 4 bits, and the operators that write, read and shrink it.  The reference has no counterpart (it
-trains; its forward takes whole sequences of multiples of 128).
+"""Serving: attention over whole prompts, a key/value cache held in 4 bits, and the operators that write, read and shrink it.  The
+reference has no counterpart (it trains; its forward takes whole sequences of multiples of 128).
 
 The cache is a pool of pages of 128 tokens (the block of the training path), a uint8 tensor [pages, KV heads, RECORD_BYTES] that the caller
 owns (`cache_empty`), with a block table int32 [sequences, pages of a sequence] and lengths int32 [sequences] in device memory: no call
@@ -18,7 +18,7 @@ PAGE = 128              # FMSA_CACHE_PAGE: tokens of a page
 RECORD_BYTES = 18432    # FMSA_CACHE_RECORD_BYTES: a page of one KV head
 HEAD_DIM = 128
 
-_KIND_APPEND, _KIND_ATTEND, _KIND_EVICT = 4, 5, 6   # passes.StatusBoard.KINDS
+_KIND_APPEND, _KIND_ATTEND, _KIND_EVICT, _KIND_PROMPT = 4, 5, 6, 7   # passes.StatusBoard.KINDS
 
 
 def _on(device):
@@ -244,3 +244,64 @@ def cache_evict(cache, weights, block_table, lengths, new_block_table, keep: int
             new_block_table.shape[1], keep, recent, new_lengths.data_ptr(), kept.data_ptr(), status.ptr, ops._stream(dev)), dev)
         status.check()
     return new_lengths, kept
+
+
+def _tma_readable(t):
+    """`t` as tile loads read it, copied once if it has to be."""
+    t = t.detach()
+    st = t.stride()
+    if st[3] == 1 and all(s > 0 and s % 8 == 0 for s in st[:3]) and st[2] >= HEAD_DIM and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def prompt_attention(q, k, v, cu_seqlens, scale: float, sinks=None):
+    """Dense causal attention over whole prompts of any length, heads grouped: q (B,Hq,S,128), k and v (B,Hkv,S,128), Hq/Hkv at most 128.
+    Returns [B, S, Hq*128].  `cu_seqlens` None: every batch element is one sequence.  Otherwise [n+1], or [B,n+1] for a packing per batch
+    element: the rows cu_seqlens[i] .. cu_seqlens[i+1]-1 are sequence i, a row sees the rows of its own sequence up to itself; it starts
+    at 0 and may end before S (rows behind the last sequence come back zero, whatever they hold).  Boundaries in host memory are checked;
+    those in device memory are not waited for, and have to rise from 0 to at most S.  `sinks` as in `flash_msa_func`; scale > 0.
+    For serving: it keeps nothing for a backward (training: `flash_msa_func`, `flash_msa_warmup_func`)."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _activation(name, t)
+    _no_gradients("flash_msa_prompt_func", q, k, v, sinks)
+    b, hq, s, _ = q.shape
+    hkv = k.shape[1]
+    if k.shape != v.shape or k.shape[0] != b or k.shape[2] != s:
+        raise ValueError("q, k, and v must agree on batch, sequence, head dimension, and KV head count")
+    if hkv == 0 or hq == 0 or hq % hkv:
+        raise ValueError("n_heads must be divisible by n_kv_heads")
+    if hq // hkv > 128:
+        raise NotImplementedError("at most 128 heads may share a KV head")
+    if not q.dtype == k.dtype == v.dtype:
+        raise TypeError("q, k, and v must have one dtype")
+    dev = q.device
+    if k.device != dev or v.device != dev:
+        raise ValueError("q, k, and v must be on one CUDA device")
+    if not scale > 0:
+        raise ValueError("scale must be positive")
+    sinks = api._check_sinks(sinks, q)
+    if cu_seqlens is not None:
+        shape = tuple(torch.as_tensor(cu_seqlens).shape)
+        if len(shape) not in (1, 2) or shape[-1] < 2 or (len(shape) == 2 and shape[0] != b):
+            raise ValueError("cu_seqlens must have shape [n+1] or [B, n+1]")
+    api._require_cuda(q)
+    out = torch.empty(b, s, hq * HEAD_DIM, dtype=q.dtype, device=dev)
+    if not out.numel():
+        return out
+    with _on(dev):
+        lib = _lib.load()
+        n_seqs, per_batch = 1, 0
+        if cu_seqlens is not None:
+            cu_seqlens = _boundaries(cu_seqlens, s, dev)
+            n_seqs, per_batch = cu_seqlens.shape[-1] - 1, int(cu_seqlens.ndim == 2)
+        qr, kr, vr, logits = _tma_readable(q), _tma_readable(k), _tma_readable(v), api._sink_logits(sinks)
+        nbytes = lib.fmsa_prompt_workspace_bytes(b, s, hq, hkv, n_seqs)
+        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+        status = api._Status(_KIND_PROMPT, dev)
+        ops._launch("fmsa_prompt_fwd", 2, lib.fmsa_prompt_fwd(
+            ops._tensor_arg(qr), ops._tensor_arg(kr), ops._tensor_arg(vr), b, s, hq, hkv,
+            None if cu_seqlens is None else cu_seqlens.data_ptr(), n_seqs, per_batch, float(scale), ops._dtype_code(q.dtype),
+            None if logits is None else logits.data_ptr(), out.data_ptr(), ws.data_ptr(), nbytes, status.ptr, ops._stream(dev)), dev)
+        status.check()
+    return out

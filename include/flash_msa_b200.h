@@ -340,7 +340,7 @@ int fmsa_backward(const fmsa_backward_args* args, fmsa_marks* marks, int32_t* la
 #define FMSA_MAX_HOST_BOUNDARIES 896
 int fmsa_doc_start(const int32_t* boundaries, int32_t n, int32_t per_batch, int32_t B, int32_t S, int32_t* doc_start, void* stream);
 
-/* ---- Serving: a key/value cache held in 4 bits (no counterpart in the reference, which trains) ----
+/* ---- Serving: a key/value cache held in 4 bits, and attention over whole prompts (no counterpart in the reference, which trains) ----
  *
  * The cache is a pool of pages of FMSA_CACHE_PAGE tokens, records[pages][heads][FMSA_CACHE_RECORD_BYTES]: per KV head K codes
  * [128][64 bytes], K scales bf16 [128][4], V codes [128][64 bytes], V scales bf16 [128][4]; a value is (nibble - 8) * the scale of its
@@ -379,6 +379,14 @@ int fmsa_cache_attend(const fmsa_cache4* cache, const fmsa_tensor* q, int32_t Hq
  * kept int32 [seqs][heads][keep]: where they were, -1 behind the last.  Two launches. */
 int fmsa_cache_evict(const fmsa_cache4* cache, float* weights, const int32_t* new_table, int64_t new_table_stride, int32_t new_width,
                      int32_t keep, int32_t recent, int32_t* new_lengths, int32_t* kept, int32_t* status, void* stream);
+
+/* Causal attention over whole prompts of any length, grouped heads: q (B,Hq,S,128), k, v (B,Hkv,S,128); out [B][S][Hq*128] contiguous.
+ * cu_seqlens NULL: every batch element is one sequence; else int32 [n_seqs+1] on the device (per_batch = 1: [B][n_seqs+1]), rising from
+ * 0: rows cu[i] .. cu[i+1]-1 are sequence i, rows behind the last one are set to zero.  Hq/Hkv <= 128.  Two launches. */
+int64_t fmsa_prompt_workspace_bytes(int32_t B, int32_t S, int32_t Hq, int32_t Hkv, int32_t n_seqs);
+int fmsa_prompt_fwd(const fmsa_tensor* q, const fmsa_tensor* k, const fmsa_tensor* v, int32_t B, int32_t S, int32_t Hq, int32_t Hkv,
+                    const int32_t* cu_seqlens, int32_t n_seqs, int32_t per_batch, float scale, int32_t dtype, const float* sinks, void* out,
+                    void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
 
 /* Boundaries in HOST memory to the device, as a kernel parameter (at most FMSA_MAX_HOST_BOUNDARIES). */
 int fmsa_boundaries(const int32_t* boundaries, int32_t n, int32_t* dst, void* stream);

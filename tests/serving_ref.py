@@ -118,3 +118,28 @@ def evict(weights, table, lengths, keep, recent):
             order = sorted(range(len(x)), key=lambda t: (-(math.inf if x[t] != x[t] else x[t]), x[t] == x[t], t))
             kept[i, h] = sorted(order[:keep - recent]) + list(range(length - recent, length))
     return kept
+
+
+def prompt(q, k, v, cu, scale, sinks=None):
+    """(out [B,S,Hq,128], tolerance), fp64; `cu`: a list of boundaries per batch element.
+
+    What the tolerance counts: the rounding of the result and that of every probability (half a step of the type each), a logit's sum of 128
+    products in fp32 and the scaling (2^-20 of the sum of the terms' magnitudes), the exponential and the division (2^-20), and in fp16
+    what is lost below its normal numbers: at most 2^-25 of a probability that is lifted by 2^7, relative to the row's maximum."""
+    b, hq, s, _ = q.shape
+    g = hq // k.shape[1]
+    out = torch.zeros(b, s, hq, D, dtype=torch.float64, device=q.device)
+    tol = torch.zeros_like(out)
+    half = torch.finfo(q.dtype).eps / 2
+    for i in range(b):
+        for lo, hi in zip(cu[i][:-1], cu[i][1:]):
+            if lo == hi:
+                continue
+            hidden = torch.ones(hi - lo, hi - lo, dtype=torch.bool, device=q.device).triu(1)
+            for h in range(hq):
+                x, y, z = (t[i, hh, lo:hi].double() for t, hh in ((q, h), (k, h // g), (v, h // g)))
+                p = softmax((x @ y.T * scale).masked_fill(hidden, -math.inf), None if sinks is None else sinks[h].double().expand(hi - lo))
+                err = (2.0 ** -20 * (x.abs() @ y.abs().T * scale).masked_fill(hidden, 0).amax(-1, keepdim=True) + 2.0 ** -20).clamp(max=1)
+                out[i, lo:hi, h] = p @ z
+                tol[i, lo:hi, h] = out[i, lo:hi, h].abs() * half + (p @ z.abs()) * (half + 2 * err) + (hi - lo) * 2.0 ** -32 * z.abs().amax()
+    return out, tol + torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps

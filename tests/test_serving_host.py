@@ -45,8 +45,11 @@ def _call(what, **change):
     a = dict(cache=torch.zeros(4, 2, serving.RECORD_BYTES, dtype=torch.uint8), k=torch.zeros(3, 2, 1, 128, dtype=BF),
              v=torch.zeros(3, 2, 1, 128, dtype=BF), q=torch.zeros(3, 4, 1, 128, dtype=BF), table=torch.zeros(3, 2, dtype=torch.int32),
              lengths=torch.ones(3, dtype=torch.int32), weights=torch.zeros(4, 2, 128), new=torch.zeros(3, 1, dtype=torch.int32), keep=100,
-             recent=10, cu=None, sinks=None)
+             recent=10, cu=None, sinks=None, pq=torch.zeros(2, 4, 7, 128, dtype=BF), pk=torch.zeros(2, 2, 7, 128, dtype=BF),
+             pv=torch.zeros(2, 2, 7, 128, dtype=BF), scale=0.1)
     a.update(change)
+    if what == "prompt":
+        return fm.flash_msa_prompt_func(a["pq"], a["pk"], a["pv"], a["cu"], a["scale"], sinks=a["sinks"])
     if what == "append":
         return fm.flash_msa_cache_append(a["cache"], a["k"], a["v"], a["table"], a["lengths"], cu_seqlens=a["cu"], weights=a["weights"])
     if what == "attend":
@@ -79,9 +82,16 @@ EVICT = [
     (dict(keep=0), ValueError), (dict(recent=101), ValueError), (dict(recent=-1), ValueError), (dict(keep=129, recent=0), ValueError),
     (dict(new=z(2, 1, dtype=torch.int32)), ValueError), (dict(new=z(3, 1, dtype=torch.int64)), TypeError), (dict(weights=None), ValueError)]
 
+PROMPT = [
+    (dict(), RuntimeError), (dict(pq=z(2, 4, 128)), ValueError), (dict(pq=z(2, 5, 7, 128)), ValueError), (dict(pq=z(2, 0, 7, 128)), ValueError),
+    (dict(pq=z(2, 258, 7, 128)), NotImplementedError), (dict(pq=z(2, 4, 6, 128)), ValueError), (dict(pq=z(1, 4, 7, 128)), ValueError),
+    (dict(pv=z(2, 1, 7, 128)), ValueError), (dict(pk=z(2, 2, 7, 128, dtype=torch.float16)), TypeError), (dict(pv=z(2, 2, 7, 64)), NotImplementedError),
+    (dict(scale=0.0), ValueError), (dict(scale=-1.0), ValueError), (dict(scale=float("nan")), ValueError), (dict(sinks=z(5, dtype=F)), ValueError),
+    (dict(cu=[0]), ValueError), (dict(cu=[[0, 7]]), ValueError), (dict(pk=z(2, 2, 7, 128).requires_grad_()), RuntimeError)]
 
-@pytest.mark.parametrize("what,change,error", [(w, c, e) for w, more in (("append", APPEND), ("attend", ATTEND), ("evict", EVICT))
-                                               for c, e in COMMON + more])
+
+@pytest.mark.parametrize("what,change,error", [(w, c, e) for w, more in (("append", COMMON + APPEND), ("attend", COMMON + ATTEND),
+                                                                         ("evict", COMMON + EVICT), ("prompt", PROMPT)) for c, e in more])
 def test_refusals(what, change, error):
     with pytest.raises(error):
         _call(what, **change)
@@ -109,5 +119,9 @@ def test_c_entries_refuse_before_they_touch_anything():
     assert lib.fmsa_cache_attend(r(c), r(t), 5, 1, 1.0, 0, None, None, 0, 0x10, 0x100, 1 << 30, 0x10, None) == -1
     bad = _lib.FmsaCache4(0x10, 0x10, 0x10, 2, 0, 2, 3, 2)
     assert lib.fmsa_cache_evict(r(bad), 0x10, 0x10, 1, 1, 100, 0, 0x10, 0x10, 0x10, None) == -1
+    prompt = lambda s, scale, ws, k=t: lib.fmsa_prompt_fwd(r(t), r(k), r(t), 1, s, 1, 1, None, 1, 0, scale, 0, None, 0x100, 0x100, ws, 0x10, None)
+    assert prompt(100, 0.0, 1 << 20) == -1 and prompt(100, 0.1, 100) == -3 and prompt(100, 0.1, 1 << 20, odd) == -1
+    assert prompt((1 << 30) + 1, 0.1, 1 << 40) == -2
+    assert lib.fmsa_prompt_workspace_bytes(1, 100, 3, 2, 1) == -1
     assert lib.fmsa_boundaries(None, 3, None, None) == -1
     assert lib.fmsa_boundaries((ctypes.c_int32 * 4)(), 897, 0x10, None) == -2
