@@ -117,29 +117,18 @@ def _declare(lib):
     lib.fmsa_backward.argtypes = [P, P, P, P]
     lib.fmsa_doc_start.restype = c_int
     lib.fmsa_doc_start.argtypes = [P, c_int32, c_int32, c_int32, c_int32, P, P]
-    CA = ctypes.POINTER(FmsaCache4)
-    lib.fmsa_cache_append.restype = c_int
-    lib.fmsa_cache_append.argtypes = [CA, T, T, c_int32, c_int32, c_int32, P, P, T, T, P, P]
+    # (argument blocks, packed by serving.py)
+    for name in ("fmsa_cache_append", "fmsa_cache_attend", "fmsa_cache_evict", "fmsa_prompt_fwd"):
+        getattr(lib, name).restype = c_int
+        getattr(lib, name).argtypes = [P, P]
     lib.fmsa_cache_attend_workspace_bytes.restype = c_int64
     lib.fmsa_cache_attend_workspace_bytes.argtypes = [c_int32, c_int32, c_int32, c_int32]
-    lib.fmsa_cache_attend.restype = c_int
-    lib.fmsa_cache_attend.argtypes = [CA, T, c_int32, c_int32, c_float, c_int32, P, P, c_int32, P, P, c_int64, P, P]
-    lib.fmsa_cache_evict.restype = c_int
-    lib.fmsa_cache_evict.argtypes = [CA, P, P, c_int64, c_int32, c_int32, c_int32, P, P, P, P]
     lib.fmsa_prompt_workspace_bytes.restype = c_int64
     lib.fmsa_prompt_workspace_bytes.argtypes = [c_int32, c_int32, c_int32, c_int32, c_int32]
-    lib.fmsa_prompt_fwd.restype = c_int
-    lib.fmsa_prompt_fwd.argtypes = [T, T, T, c_int32, c_int32, c_int32, c_int32, P, c_int32, c_int32, c_float, c_int32, P, P, P, c_int64, P, P]
     lib.fmsa_boundaries.restype = c_int
     lib.fmsa_boundaries.argtypes = [P, c_int32, P, P]
     lib.fmsa_copy2d_async.restype = c_int
     lib.fmsa_copy2d_async.argtypes = [P, ctypes.c_size_t, P, ctypes.c_size_t, ctypes.c_size_t, ctypes.c_size_t, P]
-
-
-class FmsaCache4(ctypes.Structure):
-    """Mirror of ``fmsa_cache4``."""
-    _fields_ = [("records", c_void_p), ("block_table", c_void_p), ("lengths", c_void_p), ("table_stride", c_int64), ("pages", c_int32),
-                ("heads", c_int32), ("seqs", c_int32), ("width", c_int32)]
 
 
 class FmsaProblem(ctypes.Structure):

@@ -10,10 +10,10 @@
 //     from shared memory: the 16-bit copy of every nibble would be written and read there, four times the bytes that come in.)  A word of
 //     eight nibbles gives four operand registers with a mask each:
 //       K   S^T = K Q^T: nibbles 0, 2, 4, 6 (0x000f000f) are fp16 denormals q * 2^-24 as they stand, nibbles 1, 3, 5, 7 (0x00f000f0)
-//           q * 2^-20, which queries divided by 16 make up for; the 8 of (q - 8) is a start value of the sum, -8 * sum(Q) per group.  So a
-//           K nibble costs 5/8 instruction.  The start value costs no accuracy: a group's sum has two steps.
-//       V   O^T = V^T P^T sums over the whole sequence, where such a start value would cost accuracy: the nibbles become q - 8 (fp16) by
-//           one more fma per pair (1024 + q and 1024 + 16 q are what a mask with 0x6400 gives).
+//           q * 2^-20, which queries divided by 16 make up for.  The 8 of (code = q - 8): sum over the groups of scale * -8 sum(Q), a product
+//           of its own with the scales as they stand and sum(Q) in three bf16 parts, where the sum of the groups' products begins.
+//       V   O^T = V^T P^T the same way; one product per group with a matrix of ones keeps sum(P) beside it, of which 8 times is taken from O
+//           before it has grown large beside what it is the offset of (kFlush).
 //   * scales are per token and group, so they are applied to sums (K) and to probabilities (V), not to values.
 // Queries are scaled by a power of two per row to [2^13, 2^14), so that fp16 holds bf16 ones exactly.  Probabilities times V scales are
 // fp16 relative to the running maximum of (logit + log2 scale): neither large nor tiny values of V leave fp16's range.
@@ -32,33 +32,61 @@ struct AttendParams {
     uint16_t* out;              // [seqs][n][Hq*128]
     float* weights;             // [pages][heads][128] or null
     int32_t* prefix;            // [seqs + 1]: pages of the sequences before
-    float* o_part;              // [2 * grid][rows of a block][128]
-    float2* ml_part;            // [2 * grid][rows of a block]: (reference, sum), log2 domain
+    int2* parts;                // [seqs][heads][blocks]: first slot of a pair that is cut and the number of its parts; 0 parts: not cut
+    float* o_part;              // [2 * ranges][rows of a block][128]
+    float2* ml_part;            // [2 * ranges][rows of a block]: (reference, sum), log2 domain
     float* lse;                 // [seqs][heads][blocks * rows of a block], log2 domain
     int32_t Hq, n, group, rows, blocks, fp16, accumulate, grid;   // group: heads per KV head; rows = group * n; blocks of 8 * NT rows
     float scale_log2e;
+    uint32_t magic;             // 1024, 1024 in fp16
 };
 
-constexpr int kStages = 8;
-constexpr int kMergeStride = 132;   // floats of a row in the merge area: rows 2t of four lanes start 8 banks apart
-template <int NT> constexpr int kWarps = NT == 1 ? 16 : 8;       // consumer warps; 16 of them take pages in turn, eight each
-template <int NT> constexpr int kAttendThreads = (kWarps<NT> + 4) * 32;   // and a warpgroup of which one warp loads
+// Nibbles as fp16: bits 3..6 of a half are q * 2^-21 (a denormal), bits 7..10 q * 2^-17 (from 8 on a normal number, which goes on where
+// the denormals end).  Not lower in the half: the tensor core aligns its sums by the operands' exponent fields, so every leading zero of a
+// denormal costs a bit of the sum (at bits 0..3 the probabilities of 64K tokens came out 3 times further from 64 bits' than here).
+constexpr uint32_t kLow = 0x00780078u, kHigh = 0x07800780u;
+constexpr float kUnitLow = 1.f / (1 << 21), kUnitHigh = 1.f / (1 << 17);
+
+template <bool V> struct Bool { static constexpr bool value = V; };
+
+// Teams of four warps, each with a range of pages, a ring of records and a fifth warp that loads pages and prepares queries; a warp takes 32
+// tokens of a page.  (One range and one ring for all warps of an SM, which then wait for one another at the end of every pair: B=32 Hq=32
+// Hkv=8, lengths to 8192, TEAMS_BEFORE.)
+template <int NT> constexpr int kTeams = NT == 1 ? 4 : 3;
+constexpr int kStages = 2;          // records of a team
+template <int NT> constexpr int kAttendThreads = (kTeams<NT> + 1) * 128;
 // Registers per thread after the warpgroups re-divide the register file.
-template <int NT> constexpr int kRegsLaunch = (65536 / kAttendThreads<NT>) / 8 * 8;
-template <int NT> constexpr int kRegsMath = NT == 1 ? 112 : 216;
-template <int NT> constexpr int kRegsLoad = NT == 1 ? 32 : 72;
-static_assert(4 * kRegsMath<1> + kRegsLoad<1> <= 5 * kRegsLaunch<1> && 2 * kRegsMath<2> + kRegsLoad<2> <= 3 * kRegsLaunch<2>,
-              "register re-division must balance");
+template <int NT> constexpr int kRegsLaunch = NT == 1 ? 96 : 128;
+template <int NT> constexpr int kRegsMath = NT == 1 ? 104 : 152;
+template <int NT> constexpr int kRegsLoad = NT == 1 ? 64 : 56;
+template <int NT> constexpr bool kRegsBalance = kTeams<NT> * kRegsMath<NT> + kRegsLoad<NT> <= kAttendThreads<NT> / 128 * kRegsLaunch<NT>;
+static_assert(kRegsBalance<1> && kRegsBalance<2>, "register re-division must balance");
 
-struct AttendCtrl {
-    uint64_t full[kStages], empty[kStages];
-    unsigned long long total;
-    long long rest;
-    int32_t first, sums[32];
-    float2 ml[16][16];          // [warp][row]
+// Query rows of one block as the second operand of the products, and what belongs to the columns of a product (a lane's: rows
+// 8 nt + 2 (lane % 4), + 1).  Every warp's lanes hold the same, so one warp prepares it and the others read it.
+template <int NT>
+struct Queries {
+    uint4 b[NT][4][32];      // [group of 32 channels][lane]: registers of two steps
+    uint2 corr[NT][32];      // -8 units * sum of a group's queries in three bf16 parts, the operand beside K's scales
+    float2 factor[NT][32];   // product -> logit in the log2 domain
+    int2 limit[NT][32];      // tokens the row sees, less the sequence's length
 };
-template <int NT> constexpr size_t kMergeBytes = static_cast<size_t>(kWarps<NT>) * 8 * NT * kMergeStride * 4;
-template <int NT> constexpr size_t kAttendSmem = static_cast<size_t>(kStages) * kRecordBytes + kMergeBytes<NT> + sizeof(AttendCtrl) + 128;
+
+template <int NT>
+struct AttendTeam {
+    Queries<NT> q[2];
+    float4 part[4][3][NT][2][32];    // [channels of a group, warp number][other warp][][row 2t, 2t + 1][lane]: what they have of these channels
+    float2 ml[4][8 * NT];            // [warp][row]: (reference, sum)
+    uint64_t full[kStages], empty[kStages], q_full[2], q_empty[2];
+    long long rest;
+    int32_t first;
+};
+template <int NT>
+struct AttendCtrl {
+    AttendTeam<NT> team[kTeams<NT>];
+    int32_t sums[32];
+};
+template <int NT> constexpr size_t kAttendSmem = static_cast<size_t>(kStages) * kTeams<NT> * kRecordBytes + sizeof(AttendCtrl<NT>) + 128;
 static_assert(kAttendSmem<1> <= 232448 && kAttendSmem<2> <= 232448, "shared memory budget of one CTA");
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0,
@@ -66,6 +94,11 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+__device__ __forceinline__ void mma16816_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
@@ -82,7 +115,6 @@ __device__ __forceinline__ uint2 ld_shared_v2(uint32_t addr) {
     return v;
 }
 __device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-__device__ __forceinline__ __half2 half2_from(uint32_t w) { return *reinterpret_cast<__half2*>(&w); }
 __device__ __forceinline__ void scales_of(uint2 w, float (&s)[4]) {   // four bf16
     s[0] = __uint_as_float(w.x << 16);
     s[1] = __uint_as_float(w.x & 0xffff0000u);
@@ -93,144 +125,150 @@ __device__ __forceinline__ void scales_of(uint2 w, float (&s)[4]) {   // four bf
 // need to be free of bank conflicts.
 __device__ __forceinline__ int token_of_row(int r) { return r ^ ((r >> 1) & 1); }
 
-// Query rows of one block as the second operand, and what belongs to the columns of a product (this thread's: rows 8 nt + 2t, + 1).
+// Prepares 8 query rows (number nt of a block); all lanes of a warp.
 template <int NT>
-struct Queries {
-    uint32_t b[NT][4][4];   // [group of 32 channels][registers of two steps]
-    float corr[NT][4][2];   // -8 * 2^-24 * sum of the group's queries
-    float factor[NT][2];    // product -> logit in the log2 domain
-    int limit[NT][2];       // tokens the row sees, less the sequence's length
+__device__ __forceinline__ void prepare_queries(Queries<NT>& to, const AttendParams& P, int seq, int kv, int block, int nt, int lane) {
+    const int g = lane >> 2, t = lane & 3, row = (block * NT + nt) * 8 + g;
+    float f[4][8];
+    uint32_t top = 0;
+    const bool real = row < P.rows;
+    const int hh = real ? row / P.n : 0, j = real ? row - hh * P.n : 0;
+    const uint16_t* from = P.q + seq * P.qs[0] + (static_cast<int64_t>(kv) * P.group + hh) * P.qs[1] + j * P.qs[2] + 8 * t;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint4 x = real ? __ldg(reinterpret_cast<const uint4*>(from + 32 * i)) : make_uint4(0, 0, 0, 0);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            f[i][2 * e] = P.fp16 ? act_lo<true>(w[e]) : act_lo<false>(w[e]);
+            f[i][2 * e + 1] = P.fp16 ? act_hi<true>(w[e]) : act_hi<false>(w[e]);
+            top = max(top, max(__float_as_uint(f[i][2 * e]) & 0x7fffffffu, __float_as_uint(f[i][2 * e + 1]) & 0x7fffffffu));
+        }
+    }
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // largest magnitude to [2^13, 2^14)
+    const int up = min(max(13 + 127 - static_cast<int>(top >> 23), -90), 126);
+    const float mul = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
+    float part[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[i][e] *= e & 1 ? mul * 0.0625f : mul;
+        const __half2 a0 = __floats2half2_rn(f[i][0], f[i][4]), a1 = __floats2half2_rn(f[i][2], f[i][6]);
+        const __half2 a2 = __floats2half2_rn(f[i][1], f[i][5]), a3 = __floats2half2_rn(f[i][3], f[i][7]);
+        to.b[nt][i][lane] = make_uint4(half2_bits(a0), half2_bits(a1), half2_bits(a2), half2_bits(a3));
+        const float lo = (__low2float(a0) + __high2float(a0)) + (__low2float(a1) + __high2float(a1));
+        const float hi = (__low2float(a2) + __high2float(a2)) + (__low2float(a3) + __high2float(a3));
+        float sum = lo + 16.f * hi;
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        part[i] = sum * (-8.f * kUnitLow);
+    }
+    // as an operand: steps 2t, 2t + 1 of row g are groups 2 (t % 2), + 1; first parts (t < 2) and second ones, then third ones and nothing
+    const float c0 = t & 1 ? part[2] : part[0], c1 = t & 1 ? part[3] : part[1];
+    const float h0 = __bfloat162float(__float2bfloat16_rn(c0)), h1 = __bfloat162float(__float2bfloat16_rn(c1));
+    const float m0 = __bfloat162float(__float2bfloat16_rn(c0 - h0)), m1 = __bfloat162float(__float2bfloat16_rn(c1 - h1));
+    to.corr[nt][lane] = make_uint2(t < 2 ? pack_bf16(h0, h1) : pack_bf16(m0, m1), t < 2 ? pack_bf16(c0 - h0 - m0, c1 - h1 - m1) : 0u);
+    const float fac = __uint_as_float(static_cast<uint32_t>(127 + 21 - up) << 23) * P.scale_log2e;
+    const int lim = real ? 1 - P.n + j : -0x40000000;
+    to.factor[nt][lane] = make_float2(__shfl_sync(0xffffffffu, fac, 8 * t), __shfl_sync(0xffffffffu, fac, 8 * t + 4));
+    to.limit[nt][lane] = make_int2(__shfl_sync(0xffffffffu, lim, 8 * t), __shfl_sync(0xffffffffu, lim, 8 * t + 4));
+}
 
-    __device__ __forceinline__ void load(const AttendParams& P, int seq, int kv, int block, int lane) {
-        const int g = lane >> 2, t = lane & 3;
+// s[j][nt] = {token A x row 2t, A x 2t + 1, B x 2t, B x 2t + 1} in units of 1 / factor, for the tokens of J tiles whose codes (k[j][0], [1])
+// and scales (w[j][0], [1]) are given; words: the scales' word t % 2.
+template <int NT, int J>
+__device__ __forceinline__ void logits(float (&s)[J][NT][4], const uint4 (&k)[J][2], const uint2 (&w)[J][2], const Queries<NT>& Q, int lane) {
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const uint32_t a = lane & 1 ? w[j][0].y : w[j][0].x, b = lane & 1 ? w[j][1].y : w[j][1].x;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const int row = (block * NT + nt) * 8 + g;
-            float f[4][8];
-            uint32_t top = 0;
-            const bool real = row < P.rows;
-            const int hh = real ? row / P.n : 0, j = real ? row - hh * P.n : 0;
-            const uint16_t* from = P.q + seq * P.qs[0] + (static_cast<int64_t>(kv) * P.group + hh) * P.qs[1] + j * P.qs[2] + 8 * t;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint4 x = real ? __ldg(reinterpret_cast<const uint4*>(from + 32 * i)) : make_uint4(0, 0, 0, 0);
-                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    f[i][2 * e] = P.fp16 ? act_lo<true>(w[e]) : act_lo<false>(w[e]);
-                    f[i][2 * e + 1] = P.fp16 ? act_hi<true>(w[e]) : act_hi<false>(w[e]);
-                    top = max(top, max(__float_as_uint(f[i][2 * e]) & 0x7fffffffu, __float_as_uint(f[i][2 * e + 1]) & 0x7fffffffu));
-                }
-            }
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // largest magnitude to [2^13, 2^14)
-            const int up = min(max(13 + 127 - static_cast<int>(top >> 23), -90), 126);
-            const float mul = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
-            float sum[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) f[i][e] *= e & 1 ? mul * 0.0625f : mul;
-                const __half2 a0 = __floats2half2_rn(f[i][0], f[i][4]), a1 = __floats2half2_rn(f[i][2], f[i][6]);
-                const __half2 a2 = __floats2half2_rn(f[i][1], f[i][5]), a3 = __floats2half2_rn(f[i][3], f[i][7]);
-                b[nt][i][0] = half2_bits(a0);
-                b[nt][i][1] = half2_bits(a1);
-                b[nt][i][2] = half2_bits(a2);
-                b[nt][i][3] = half2_bits(a3);
-                const float lo = (__low2float(a0) + __high2float(a0)) + (__low2float(a1) + __high2float(a1));
-                const float hi = (__low2float(a2) + __high2float(a2)) + (__low2float(a3) + __high2float(a3));
-                sum[i] = lo + 16.f * hi;
-                sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
-                sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
-            }
-            const float fac = __uint_as_float(static_cast<uint32_t>(127 + 24 - up) << 23) * P.scale_log2e;
-            const int lim = real ? 1 - P.n + j : -0x40000000;
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int from_lane = (2 * t + c) * 4;
-                factor[nt][c] = __shfl_sync(0xffffffffu, fac, from_lane);
-                limit[nt][c] = __shfl_sync(0xffffffffu, lim, from_lane);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) corr[nt][i][c] = __shfl_sync(0xffffffffu, sum[i], from_lane) * (-8.f / 16777216.f);
-            }
+            const uint2 c = Q.corr[nt][lane];
+            mma16816_bf16(s[j][nt], a, b, a, b, c.x, c.y);
         }
     }
-    // s[nt] = {token A x row 2t, A x 2t + 1, B x 2t, B x 2t + 1} in units of 1 / factor, for the tokens whose codes and scales are given.
-    __device__ __forceinline__ void logits(float (&s)[NT][4], uint4 ka, uint4 kb, uint2 sa, uint2 sb) const {
-        const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
-        float fa[4], fb[4];
-        scales_of(sa, fa);
-        scales_of(sb, fb);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t a = wa[i], c = wb[i], a8 = a >> 8, c8 = c >> 8;
+    for (int i = 0; i < 4; ++i) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
+        for (int nt = 0; nt < NT; ++nt) {
+            const uint4 q = Q.b[nt][i][lane];
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const uint32_t a = i == 0 ? k[j][0].x : i == 1 ? k[j][0].y : i == 2 ? k[j][0].z : k[j][0].w;
+                const uint32_t c = i == 0 ? k[j][1].x : i == 1 ? k[j][1].y : i == 2 ? k[j][1].z : k[j][1].w;
+                const uint32_t a0 = a << 3, c0 = c << 3, a1 = a >> 5, c1 = c >> 5;
+                const uint32_t wa = i < 2 ? w[j][0].x : w[j][0].y, wb = i < 2 ? w[j][1].x : w[j][1].y;
+                const float fa = __uint_as_float(i & 1 ? wa & 0xffff0000u : wa << 16), fb = __uint_as_float(i & 1 ? wb & 0xffff0000u : wb << 16);
                 float d[4];
-                mma16816(d, a & 0x000f000fu, c & 0x000f000fu, a8 & 0x000f000fu, c8 & 0x000f000fu, b[nt][i][0], b[nt][i][1], corr[nt][i][0],
-                         corr[nt][i][1], corr[nt][i][0], corr[nt][i][1]);
-                mma16816(d, a & 0x00f000f0u, c & 0x00f000f0u, a8 & 0x00f000f0u, c8 & 0x00f000f0u, b[nt][i][2], b[nt][i][3], d[0], d[1], d[2], d[3]);
-                if (i == 0) {
-                    s[nt][0] = fa[0] * d[0];
-                    s[nt][1] = fa[0] * d[1];
-                    s[nt][2] = fb[0] * d[2];
-                    s[nt][3] = fb[0] * d[3];
-                } else {
-                    s[nt][0] = fmaf(fa[i], d[0], s[nt][0]);
-                    s[nt][1] = fmaf(fa[i], d[1], s[nt][1]);
-                    s[nt][2] = fmaf(fb[i], d[2], s[nt][2]);
-                    s[nt][3] = fmaf(fb[i], d[3], s[nt][3]);
-                }
+                mma16816(d, a0 & kLow, c0 & kLow, a1 & kLow, c1 & kLow, q.x, q.y, 0.f, 0.f, 0.f, 0.f);
+                mma16816(d, a0 & kHigh, c0 & kHigh, a1 & kHigh, c1 & kHigh, q.z, q.w, d[0], d[1], d[2], d[3]);
+                s[j][nt][0] = fmaf(fa, d[0], s[j][nt][0]);
+                s[j][nt][1] = fmaf(fa, d[1], s[j][nt][1]);
+                s[j][nt][2] = fmaf(fb, d[2], s[j][nt][2]);
+                s[j][nt][3] = fmaf(fb, d[3], s[j][nt][3]);
             }
         }
     }
-};
+}
 
 __device__ __forceinline__ int pages_of(const Cache4& c, int seq) { return (c.length(seq) + kPage - 1) / kPage; }
 
 // Logits (log2 domain) that a tile keeps below 2^kSlack times the reference before the reference is raised, and how far below the largest
 // (logit + log2 scale) the reference is set: fp16 holds p * s up to 2^(kSlack + kLift) and, at full precision, down to 2^-14.
 constexpr float kSlack = 8.f, kLift = 6.f;
+// Code q - 8 of nibbles 0 and 4 (bits 0..3 of each half) as fp16, and of nibbles 1 and 5 (bits 4..7): 1024 + q and 1024 + 16 q are what the
+// nibble gives under the exponent bits of `magic` (0x64006400: not a constant here, so that it stays in a register and both logical
+// operations are one instruction).
+__device__ __forceinline__ uint32_t masked_or(uint32_t x, uint32_t mask, uint32_t or_with) {
+    uint32_t y;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(or_with));
+    return y;
+}
+__device__ __forceinline__ uint32_t less_eight(uint32_t x, uint32_t magic) {
+    const uint32_t y = masked_or(x, 0x000f000fu, magic);
+    return half2_bits(__hadd2(*reinterpret_cast<const __half2*>(&y), __float2half2_rn(-1032.f)));
+}
+__device__ __forceinline__ uint32_t less_eight_high(uint32_t x, uint32_t magic) {
+    const uint32_t y = masked_or(x, 0x00f000f0u, magic);
+    return half2_bits(__hfma2(*reinterpret_cast<const __half2*>(&y), __float2half2_rn(0.0625f), __float2half2_rn(-72.f)));
+}
 
 template <int NT>
 __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(const AttendParams P) {
     extern __shared__ uint8_t smem_raw[];
+    constexpr int kRows = 8 * NT, kT = kTeams<NT>, kThreads = kAttendThreads<NT>;
     const uint32_t base = (smem_u32(smem_raw) + 127u) & ~127u;
-    uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
-    float* merge = reinterpret_cast<float*>(smem + kStages * kRecordBytes);
-    AttendCtrl* sm = reinterpret_cast<AttendCtrl*>(smem + kStages * kRecordBytes + kMergeBytes<NT>);
-    constexpr int kRows = 8 * NT, kNW = kWarps<NT>, kThreads = kAttendThreads<NT>, kTeams = kNW / 8;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    AttendCtrl<NT>* sm = reinterpret_cast<AttendCtrl<NT>*>(smem_raw + (base - smem_u32(smem_raw)) + kStages * kT * kRecordBytes);
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     auto BAR = [&](uint64_t& b) { return smem_u32(&b); };
 
-    if (tid == 0) {
-        for (int i = 0; i < kStages; ++i) {
-            mbar_init(BAR(sm->full[i]), 1);
-            mbar_init(BAR(sm->empty[i]), 8);
+    if (tid < kT) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(BAR(sm->team[tid].full[i]), 1);
+            mbar_init(BAR(sm->team[tid].empty[i]), 4);
+            mbar_init(BAR(sm->team[tid].q_full[i]), 1);
+            mbar_init(BAR(sm->team[tid].q_empty[i]), 4);
         }
-        sm->total = 0;
         fence_mbar_init();
     }
-    __syncthreads();
     wait_for_previous_kernel();
 
-    // ---- the line of pages, and this CTA's range of it (a unit is a page of a (sequence, KV head, block of rows))
-    const int seqs = P.cache.seqs, per = P.cache.heads * P.blocks;
-    {
-        unsigned long long mine = 0;
-        for (int b = tid; b < seqs; b += kThreads) mine += pages_of(P.cache, b);
-        for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-        if (lane == 0 && mine) atomicAdd(&sm->total, mine);
-    }
-    __syncthreads();
-    const long long units = static_cast<long long>(sm->total) * per;
-    const long long grid = min(static_cast<long long>(P.grid), units);
-    const int cta = blockIdx.x;
-    if (cta > 0 && cta >= grid) return;
-    const long long u0 = grid ? units * cta / grid : 0, u1 = grid ? units * (cta + 1) / grid : 0;
-    long long before = 0;
-    for (int c0 = 0; c0 < seqs; c0 += kThreads) {
+    // ---- the line of pages, and the teams' ranges of it (a unit is a page of a (sequence, KV head, block of rows)); ranges are numbered
+    // team by team, so that few units go to as many SMs
+    const int seqs = P.cache.seqs, per = P.cache.heads * P.blocks, cta = blockIdx.x;
+    long long units = 0, ranges = 0;
+    auto begin_of = [&](int team) {   // of the range; the end is the next one's begin
+        const long long r = static_cast<long long>(team) * P.grid + cta;
+        return r < ranges ? units * r / ranges : units;
+    };
+    auto end_of = [&](int team) {
+        const long long r = static_cast<long long>(team) * P.grid + cta;
+        return r < ranges ? units * (r + 1) / ranges : units;
+    };
+    // Pages of up to kThreads sequences, from c0 on: what(sequence, its first page, its pages, sum so far) for the thread's own; returns the sum.
+    auto scan = [&](int c0, long long before, auto&& what) {
         const int b = c0 + tid, p = b < seqs ? pages_of(P.cache, b) : 0;
         int sum = p;
         for (int o = 1; o < 32; o <<= 1) {
@@ -239,52 +277,83 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
         }
         if (lane == 31) sm->sums[warp] = sum;
         __syncthreads();
-        long long at = before + sum - p;
-        int chunk = 0;
-        for (int w = 0; w < kThreads / 32; ++w) {
-            const int v = sm->sums[w];
-            if (w < warp) at += v;
-            chunk += v;
-        }
-        if (b < seqs && cta == 0) P.prefix[b] = static_cast<int32_t>(at);
-        if (p && at * per <= u0 && u0 < (at + p) * per) {
-            sm->first = b;
-            sm->rest = u0 - at * per;
-        }
-        before += chunk;
+        const int w = lane < kThreads / 32 ? sm->sums[lane] : 0;
+        const int ahead = __reduce_add_sync(0xffffffffu, lane < warp ? w : 0), all = __reduce_add_sync(0xffffffffu, w);
+        what(b, before + ahead + sum - p, p, before + all);
         __syncthreads();
+        return before + all;
+    };
+    auto divide = [&](long long pages) {
+        units = pages * per;
+        ranges = min(static_cast<long long>(P.grid) * kT, units);
+    };
+    auto claim = [&](int b, long long at, int p) {
+        if (b < seqs && cta == 0) P.prefix[b] = static_cast<int32_t>(at);
+#pragma unroll
+        for (int i = 0; i < kT; ++i) {
+            const long long u = begin_of(i);
+            if (at * per <= u && u < (at + p) * per) {
+                sm->team[i].first = b;
+                sm->team[i].rest = u - at * per;
+            }
+        }
+    };
+    long long pages_all = 0;
+    if (seqs <= kThreads) {
+        pages_all = scan(0, 0, [&](int b, long long at, int p, long long all) { divide(all); claim(b, at, p); });
+    } else {
+        for (int c0 = 0; c0 < seqs; c0 += kThreads) pages_all = scan(c0, pages_all, [](int, long long, int, long long) {});
+        divide(pages_all);
+        long long before = 0;
+        for (int c0 = 0; c0 < seqs; c0 += kThreads) before = scan(c0, before, [&](int b, long long at, int p, long long) { claim(b, at, p); });
     }
-    if (cta == 0 && tid == 0) P.prefix[seqs] = static_cast<int32_t>(before);
-    if (u0 == u1) return;
+    if (cta == 0 && tid == 0) P.prefix[seqs] = static_cast<int32_t>(pages_all);
+    if (begin_of(0) == units) return;   // (nothing for any team)
 
-    int seq = sm->first, pages = pages_of(P.cache, seq);
-    int item = static_cast<int>(sm->rest / pages), page = static_cast<int>(sm->rest % pages);   // item: KV head * blocks + block of rows
-    long long left = u1 - u0;
-    uint32_t k = 0;   // pages so far
+    const bool loads = warp >= 4 * kT;
+    const int team = loads ? warp - 4 * kT : warp >> 2;
+    AttendTeam<NT>* tm = &sm->team[min(team, kT - 1)];
+    const uint32_t ring = base + team * kStages * kRecordBytes;
+    int left = team < kT ? static_cast<int>(end_of(team) - begin_of(team)) : 0;
+    int seq = 0, pages = 1, item = 0, page = 0;   // item: KV head * blocks + block of rows
+    if (left > 0) {
+        seq = tm->first;
+        pages = pages_of(P.cache, seq);
+        item = static_cast<int>(tm->rest / pages);
+        page = static_cast<int>(tm->rest % pages);
+    }
+    uint32_t stage = 0, phase = 0, pieces = 0;   // ring position; pieces so far
     bool bad = false;
     auto next = [&](int took) {
         left -= took;
         page = 0;
+        ++pieces;
         if (left > 0 && ++item == per) {
             item = 0;
             do ++seq; while ((pages = pages_of(P.cache, seq)) == 0);
         }
     };
+    auto step = [&]() {
+        stage ^= 1;
+        phase ^= stage ^ 1;
+    };
+    auto wait = [&](uint32_t bar, uint32_t parity) {   // every lane of the warp calls it; after one that ran out nothing is waited for
+        if (!bad) bad = __any_sync(0xffffffffu, !mbar_wait_role(bar, parity));
+    };
 
-    if (warp >= kNW) {
-        // =========================== loads ===========================
+    if (loads) {
+        // =========================== pages and queries ===========================
         reg_dec<kRegsLoad<NT>>();
-        while (warp == kNW && left > 0) {
-            const int take = static_cast<int>(min(left, static_cast<long long>(pages - page))), head = item / P.blocks, length = P.cache.length(seq);
+        while (left > 0) {
+            const int take = min(left, pages - page), head = item / P.blocks, length = P.cache.length(seq);
             int id = -1;
-            for (int i = 0; i < take; ++i, ++k) {
-                if ((i & 31) == 0 && i + lane < take) id = P.cache.page(seq, page + i + lane);
+            for (int i = 0; i < take; ++i) {
+                if ((i & 31) == 0) id = i + lane < take ? P.cache.page(seq, page + i + lane) : -1;
                 const int pg = __shfl_sync(0xffffffffu, id, i & 31);
-                const uint32_t stage = k % kStages, bar = BAR(sm->full[stage]);
-                if (k >= kStages && !bad) bad = __any_sync(0xffffffffu, !mbar_wait_role(BAR(sm->empty[stage]), (k / kStages - 1) & 1));
-                if (bad) continue;   // (nothing is asked for any more; the others give up in the same way)
-                if (lane == 0) {
-                    const uint32_t to = base + stage * kRecordBytes;
+                const uint32_t bar = BAR(tm->full[stage]);
+                wait(BAR(tm->empty[stage]), phase ^ 1);   // (the first round finds both records free)
+                if (!bad && lane == 0) {                  // (after a wait that ran out nothing is asked for; the others give up in the same way)
+                    const uint32_t to = ring + stage * kRecordBytes;
                     const uint32_t tokens = min(kPage, (length - (page + i) * kPage + 15) & ~15);
                     if (pg < 0) {
                         mbar_arrive(bar);
@@ -301,25 +370,35 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
                     }
                 }
                 __syncwarp();
+                step();
+                if (i == min(take, kStages) - 1) {
+                    const uint32_t slot = pieces & 1;
+                    if (pieces >= 2) wait(BAR(tm->q_empty[slot]), (pieces / 2 - 1) & 1);
+#pragma unroll 1
+                    for (int nt = 0; nt < NT; ++nt) prepare_queries<NT>(tm->q[slot], P, seq, head, item % P.blocks, nt, lane);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(BAR(tm->q_full[slot]));
+                }
             }
             next(take);
         }
     } else {
         // =========================== products ===========================
         reg_inc<kRegsMath<NT>>();
-        const int g = lane >> 2, t = lane & 3, team = warp >> 3, tile = (warp & 7) * 16;
+        const int g = lane >> 2, t = lane & 3, mine = warp & 3, tile = mine * 32;
         const int tok_a = tile + token_of_row(g), tok_v0 = tile + token_of_row(2 * t), tok_v1 = tile + token_of_row(2 * t + 1);
-        const uint32_t k_at = kKCodes + tok_a * 64 + t * 16, ks_at = kKScales + tok_a * 8, vs_at = kVScales + tok_a * 8;
+        const uint32_t k_at = kKCodes + tok_a * 64 + t * 16, s_at = tok_a * 8;
         const uint32_t v0_at = kVCodes + tok_v0 * 64 + (g ^ (tok_v0 & 4)) * 8, v1_at = kVCodes + tok_v1 * 64 + (g ^ (tok_v1 & 4)) * 8;
-        bool first_piece = true;
         while (left > 0) {
-            const int take = static_cast<int>(min(left, static_cast<long long>(pages - page)));
+            const int take = min(left, pages - page);
             const int head = item / P.blocks, block = item % P.blocks, length = P.cache.length(seq);
-            Queries<NT> Q;
-            Q.load(P, seq, head, block, lane);
+            const Queries<NT>& Q = tm->q[pieces & 1];
+            wait(BAR(tm->q_full[pieces & 1]), (pieces / 2) & 1);
             float ref[NT][2], sum[NT][2], o[NT][8][4];
+            float2 factor[NT];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
+                factor[nt] = Q.factor[nt][lane];
                 ref[nt][0] = ref[nt][1] = -INFINITY;
                 sum[nt][0] = sum[nt][1] = 0.f;
 #pragma unroll
@@ -327,173 +406,197 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
 #pragma unroll
                     for (int c = 0; c < 4; ++c) o[nt][m][c] = 0.f;
             }
-#pragma unroll 1
-            for (int i = 0; i < take; ++i, ++k) {
-                if (kTeams > 1 && static_cast<int>(k % kTeams) != team) continue;
-                const uint32_t stage = k % kStages;
-                if (!bad) bad = __any_sync(0xffffffffu, !mbar_wait_role(BAR(sm->full[stage]), (k / kStages) & 1));
-                const int first = (page + i) * kPage;   // first token of the page
-                if (!bad && first + tile < length) {
-                    const uint32_t at = base + stage * kRecordBytes;
-                    const uint4 ka = ld_shared_v4(at + k_at), kb = ld_shared_v4(at + k_at + 8 * 64);
-                    float s[NT][4];
-                    Q.logits(s, ka, kb, ld_shared_v2(at + ks_at), ld_shared_v2(at + ks_at + 64));
-                    float va[4], vb[4];
-                    scales_of(ld_shared_v2(at + vs_at), va);
-                    scales_of(ld_shared_v2(at + vs_at + 64), vb);
-                    const bool edge = first + kPage > length - P.n + 1;
+            // Two tiles of 16 tokens.  EDGE: some of them are not seen by some row, or are not there (their bytes may be anything).
+            auto two_tiles = [&](auto edge, uint32_t at, int first) {
+                constexpr bool EDGE = decltype(edge)::value;
+                float s[2][NT][4];
+                {
+                    uint4 kc[2][2];
+                    uint2 ks[2][2];
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                    for (int j = 0; j < 2; ++j)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) s[nt][c] *= Q.factor[nt][c & 1];
-                    if (edge) {   // tokens that a row does not see, and those that are not there (whose bytes may be anything)
-                        const int pa = first + tok_a - length, pb = pa + 8;
+                        for (int y = 0; y < 2; ++y) {
+                            kc[j][y] = ld_shared_v4(at + k_at + (2 * j + y) * 512);
+                            ks[j][y] = ld_shared_v2(at + kKScales + s_at + (2 * j + y) * 64);
+                        }
+                    logits<NT, 2>(s, kc, ks, Q, lane);
+                }
+                uint32_t pb[2][NT][4][2];   // p * scale of the four groups, as the second operand
+                uint2 vs[2][2];
+                float x[NT][2];
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
+                for (int nt = 0; nt < NT; ++nt) x[nt][0] = x[nt][1] = -INFINITY;
 #pragma unroll
-                            for (int c = 0; c < 4; ++c)
-                                if ((c < 2 ? pa : pb) >= Q.limit[nt][c & 1]) s[nt][c] = -INFINITY;
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            if (pa >= 0) va[c] = 0.f;
-                            if (pb >= 0) vb[c] = 0.f;
+                    for (int y = 0; y < 2; ++y) {
+                        vs[j][y] = ld_shared_v2(at + kVScales + s_at + (2 * j + y) * 64);
+                        const int place = first + tok_a + 16 * j + 8 * y - length;
+                        if (EDGE && place >= 0) vs[j][y] = make_uint2(0, 0);
+                        // log2 of the largest scale (a word as it stands is its upper half and less than one of its steps)
+                        const float lg = fast_log2(fmaxf(fmax3(__uint_as_float(vs[j][y].x), __uint_as_float(vs[j][y].x << 16), __uint_as_float(vs[j][y].y)),
+                                                         fmaxf(__uint_as_float(vs[j][y].y << 16), 8.27e-25f)));
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            s[j][nt][2 * y] *= factor[nt].x;
+                            s[j][nt][2 * y + 1] *= factor[nt].y;
+                            if (EDGE) {
+                                const int2 lim = Q.limit[nt][lane];
+                                if (place >= lim.x) s[j][nt][2 * y] = -INFINITY;
+                                if (place >= lim.y) s[j][nt][2 * y + 1] = -INFINITY;
+                            }
+                            x[nt][0] = fmaxf(x[nt][0], s[j][nt][2 * y] + lg);
+                            x[nt][1] = fmaxf(x[nt][1], s[j][nt][2 * y + 1] + lg);
                         }
                     }
-                    // the reference: raised, for every row by what it needs, when one is exceeded by more than the slack
-                    const float ea = fast_log2(fmaxf(fmaxf(fmaxf(va[0], va[1]), fmaxf(va[2], va[3])), 8.27e-25f));
-                    const float eb = fast_log2(fmaxf(fmaxf(fmaxf(vb[0], vb[1]), fmaxf(vb[2], vb[3])), 8.27e-25f));
-                    float x[NT][2];
-                    bool raise = false;
+                // the reference: raised, for every row by what it needs, when one is exceeded by more than the slack
+                bool raise = false;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) raise |= x[nt][0] > ref[nt][0] + (kLift + kSlack) || x[nt][1] > ref[nt][1] + (kLift + kSlack);
+                if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            x[nt][c] = fmaxf(s[nt][c] + ea, s[nt][c + 2] + eb) - kLift;
-                            raise |= x[nt][c] > ref[nt][c] + kSlack;
-                        }
-                    if (__any_sync(0xffffffffu, raise)) {
+                            float top = x[nt][c];
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                            top = fmaxf(top - kLift, ref[nt][c]);
+                            const float by = ref[nt][c] == -INFINITY ? 0.f : fast_exp2(ref[nt][c] - top);
+                            ref[nt][c] = top;
+                            sum[nt][c] *= by;
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                            for (int c = 0; c < 2; ++c) {
-                                float top = x[nt][c];
-                                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                                top = fmaxf(top, ref[nt][c]);
-                                const float by = ref[nt][c] == -INFINITY ? 0.f : fast_exp2(ref[nt][c] - top);
-                                ref[nt][c] = top;
-                                sum[nt][c] *= by;
-#pragma unroll
-                                for (int m = 0; m < 8; ++m) {
-                                    o[nt][m][c] *= by;
-                                    o[nt][m][c + 2] *= by;
-                                }
+                            for (int m = 0; m < 8; ++m) {
+                                o[nt][m][c] *= by;
+                                o[nt][m][c + 2] *= by;
                             }
-                    }
-                    uint32_t pb0[NT][4], pb1[NT][4];   // p * scale of the four groups, as the second operand
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        const float r0 = ref[nt][0] == -INFINITY ? 0.f : ref[nt][0], r1 = ref[nt][1] == -INFINITY ? 0.f : ref[nt][1];
-                        const float p0 = fast_exp2(s[nt][0] - r0), p1 = fast_exp2(s[nt][1] - r1);
-                        const float p2 = fast_exp2(s[nt][2] - r0), p3 = fast_exp2(s[nt][3] - r1);
-                        sum[nt][0] += p0 + p2;
-                        sum[nt][1] += p1 + p3;
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            pb0[nt][c] = half2_bits(__floats2half2_rn(p0 * va[c], p1 * va[c]));
-                            pb1[nt][c] = half2_bits(__floats2half2_rn(p2 * vb[c], p3 * vb[c]));
                         }
-                        if (edge) {   // (0 * NaN: a token that is not finite is nothing to rows that do not see it)
+                }
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        float v[4];
+                        scales_of(vs[j][y], v);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const float r0 = EDGE && ref[nt][0] == -INFINITY ? 0.f : ref[nt][0], r1 = EDGE && ref[nt][1] == -INFINITY ? 0.f : ref[nt][1];
+                            const float p0 = fast_exp2(s[j][nt][2 * y] - r0), p1 = fast_exp2(s[j][nt][2 * y + 1] - r1);
+                            sum[nt][0] += p0;
+                            sum[nt][1] += p1;
 #pragma unroll
                             for (int c = 0; c < 4; ++c) {
-                                pb0[nt][c] &= (p0 == 0.f ? 0u : 0xffffu) | (p1 == 0.f ? 0u : 0xffff0000u);
-                                pb1[nt][c] &= (p2 == 0.f ? 0u : 0xffffu) | (p3 == 0.f ? 0u : 0xffff0000u);
+                                uint32_t w = half2_bits(__floats2half2_rn(p0 * v[c], p1 * v[c]));
+                                // (0 * NaN: a token that is not finite is nothing to rows that do not see it)
+                                if (EDGE) w &= (p0 == 0.f ? 0u : 0xffffu) | (p1 == 0.f ? 0u : 0xffff0000u);
+                                pb[j][nt][c][y] = transpose8x8(w);
                             }
-                        }
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            pb0[nt][c] = transpose8x8(pb0[nt][c]);
-                            pb1[nt][c] = transpose8x8(pb1[nt][c]);
                         }
                     }
-                    const uint2 v0 = ld_shared_v2(at + v0_at), v1 = ld_shared_v2(at + v1_at);
-                    const uint2 v2 = ld_shared_v2(at + v0_at + 8 * 64), v3 = ld_shared_v2(at + v1_at + 8 * 64);
-                    const __half2 off = __float2half2_rn(-1032.f), off16 = __float2half2_rn(-72.f), sixteenth = __float2half2_rn(0.0625f);
 #pragma unroll
-                    for (int i2 = 0; i2 < 4; ++i2) {
-                        const uint32_t sel = i2 & 1 ? 0x7632u : 0x5410u;
-                        uint32_t xx = __byte_perm(i2 < 2 ? v0.x : v0.y, i2 < 2 ? v1.x : v1.y, sel);   // four channels of tokens 2t, 2t + 1
-                        uint32_t yy = __byte_perm(i2 < 2 ? v2.x : v2.y, i2 < 2 ? v3.x : v3.y, sel);   // ... and of the two 8 further
+                for (int j = 0; j < 2; ++j) {
+                    const uint2 v0 = ld_shared_v2(at + v0_at + j * 1024), v1 = ld_shared_v2(at + v1_at + j * 1024);
+                    const uint2 v2 = ld_shared_v2(at + v0_at + j * 1024 + 512), v3 = ld_shared_v2(at + v1_at + j * 1024 + 512);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t sel = i & 1 ? 0x7632u : 0x5410u;
+                        const uint32_t xx = __byte_perm(i < 2 ? v0.x : v0.y, i < 2 ? v1.x : v1.y, sel);   // four channels of tokens 2t, 2t + 1
+                        const uint32_t yy = __byte_perm(i < 2 ? v2.x : v2.y, i < 2 ? v3.x : v3.y, sel);   // ... and of the two 8 further
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const uint32_t a0 = half2_bits(__hadd2(half2_from((xx & 0x000f000fu) | 0x64006400u), off));
-                            const uint32_t a1 = half2_bits(__hfma2(half2_from((xx & 0x00f000f0u) | 0x64006400u), sixteenth, off16));
-                            const uint32_t a2 = half2_bits(__hadd2(half2_from((yy & 0x000f000fu) | 0x64006400u), off));
-                            const uint32_t a3 = half2_bits(__hfma2(half2_from((yy & 0x00f000f0u) | 0x64006400u), sixteenth, off16));
+                            const uint32_t x1 = h ? xx >> 8 : xx, y1 = h ? yy >> 8 : yy;
+                            const uint32_t a0 = less_eight(x1, P.magic), a1 = less_eight_high(x1, P.magic);
+                            const uint32_t a2 = less_eight(y1, P.magic), a3 = less_eight_high(y1, P.magic);
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt) {
-                                float(&d)[4] = o[nt][2 * i2 + h];
-                                mma16816(d, a0, a1, a2, a3, pb0[nt][i2], pb1[nt][i2], d[0], d[1], d[2], d[3]);
+                                float(&d)[4] = o[nt][2 * i + h];
+                                mma16816(d, a0, a1, a2, a3, pb[j][nt][i][0], pb[j][nt][i][1], d[0], d[1], d[2], d[3]);
                             }
-                            xx >>= 8;
-                            yy >>= 8;
                         }
                     }
                 }
+            };
+#pragma unroll 1
+            for (int i = 0; i < take; ++i) {
+                wait(BAR(tm->full[stage]), phase);
+                const int first = (page + i) * kPage;   // first token of the page
+                if (!bad && first + tile < length) {
+                    const uint32_t at = ring + stage * kRecordBytes;
+                    if (first + kPage > length - P.n + 1) two_tiles(Bool<true>(), at, first);
+                    else two_tiles(Bool<false>(), at, first);
+                }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(BAR(sm->empty[stage]));
+                if (lane == 0) mbar_arrive(BAR(tm->empty[stage]));
+                step();
             }
-            // ---- the end of a piece: the warps' parts become one
+            if (lane == 0) mbar_arrive(BAR(tm->q_empty[pieces & 1]));
+            // ---- the end of a piece: warp w takes the channels of group w from the other three
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     float l = sum[nt][c];
                     l += __shfl_xor_sync(0xffffffffu, l, 4);
                     l += __shfl_xor_sync(0xffffffffu, l, 8);
                     l += __shfl_xor_sync(0xffffffffu, l, 16);
-                    const int r = nt * 8 + 2 * t + c;
-                    if (g == 0) sm->ml[warp][r] = make_float2(ref[nt][c], l);
-                    float* to = merge + (warp * kRows + r) * kMergeStride + 4 * g;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)   // channels 32 i + 4 g ..: rows g and g + 8 of two operand tiles
-                        *reinterpret_cast<float4*>(to + 32 * i) = make_float4(o[nt][2 * i][c], o[nt][2 * i][c + 2], o[nt][2 * i + 1][c], o[nt][2 * i + 1][c + 2]);
+                    if (g == 0) tm->ml[mine][nt * 8 + 2 * t + c] = make_float2(ref[nt][c], l);
                 }
-            }
-            named_barrier_sync(1, kNW * 32);
+            float4 own[NT][2] = {};   // channels 32 w + 4 g ..: rows g and g + 8 of two operand tiles
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const float4 x = make_float4(o[nt][2 * i][c], o[nt][2 * i][c + 2], o[nt][2 * i + 1][c], o[nt][2 * i + 1][c + 2]);
+                        if (i == mine) own[nt][c] = x;
+                        else tm->part[i][(mine - i + 3) & 3][nt][c][lane] = x;   // (warp i + 1 + y, modulo 4, is number y)
+                    }
+            named_barrier_sync(1 + team, 128);
             const bool whole = page == 0 && take == pages;
-            const int ch = tid & 127;
-            for (int r = tid >> 7; r < kRows; r += kNW / 4) {
-                const int row = block * kRows + r;
-                if (row >= P.rows) break;
-                float top = -INFINITY;
-#pragma unroll
-                for (int w = 0; w < kNW; ++w) top = fmaxf(top, sm->ml[w][r].x);
-                const float m = top == -INFINITY ? 0.f : top;
-                float l = 0.f, acc = 0.f;
-#pragma unroll
-                for (int w = 0; w < kNW; ++w) {
-                    const float2 ml = sm->ml[w][r];
-                    const float by = fast_exp2(ml.x - m);
-                    l = fmaf(ml.y, by, l);
-                    acc = fmaf(merge[(w * kRows + r) * kMergeStride + ch], by, acc);
-                }
-                if (whole) {
-                    const int hh = row / P.n, j = row - hh * P.n, h = head * P.group + hh;
-                    if (P.sinks) l += fast_exp2(P.sinks[h] * kLog2e - m);
-                    const float y = l == 0.f ? 0.f : acc / l;
-                    P.out[((static_cast<int64_t>(seq) * P.n + j) * P.Hq + h) * kHeadDim + ch] =
-                        static_cast<uint16_t>(P.fp16 ? pack_act<true>(y, 0.f) : pack_act<false>(y, 0.f));
-                    if (ch == 0) P.lse[(static_cast<int64_t>(seq) * P.cache.heads + head) * (P.blocks * kRows) + row] = m + fast_log2(l);
-                } else {
-                    const int64_t slot = 2LL * cta + (first_piece ? 0 : 1);
-                    P.o_part[(slot * kRows + r) * kHeadDim + ch] = acc;
-                    if (ch == 0) P.ml_part[slot * kRows + r] = make_float2(top, l);
-                }
+            if (page == 0 && mine == 0 && lane == 0) {   // (the part that begins a pair says where its parts are)
+                const long long r = static_cast<long long>(team) * P.grid + cta, last = begin_of(team) + (end_of(team) - begin_of(team) - left) + pages;
+                P.parts[(static_cast<int64_t>(seq) * P.cache.heads * P.blocks) + item] =
+                    make_int2(static_cast<int>(2 * r + (pieces ? 1 : 0)), whole ? 0 : static_cast<int>((last * ranges - 1) / units - r + 1));
             }
-            named_barrier_sync(1, kNW * 32);
-            first_piece = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int r = nt * 8 + 2 * t + c, row = block * kRows + r;
+                    const float2 ml[4] = {tm->ml[0][r], tm->ml[1][r], tm->ml[2][r], tm->ml[3][r]};
+                    const float top = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), m = top == -INFINITY ? 0.f : top;
+                    float l = 0.f;
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) l = fmaf(ml[y].y, fast_exp2(ml[y].x - m), l);
+                    float by = fast_exp2(ref[nt][c] - m);
+                    float4 acc = make_float4(own[nt][c].x * by, own[nt][c].y * by, own[nt][c].z * by, own[nt][c].w * by);
+#pragma unroll
+                    for (int y = 0; y < 3; ++y) {
+                        const float4 x = tm->part[mine][y][nt][c][lane];
+                        by = fast_exp2(tm->ml[(mine + 1 + y) & 3][r].x - m);
+                        acc = make_float4(fmaf(x.x, by, acc.x), fmaf(x.y, by, acc.y), fmaf(x.z, by, acc.z), fmaf(x.w, by, acc.w));
+                    }
+                    if (row >= P.rows) continue;
+                    const int ch = 32 * mine + 4 * g;
+                    if (whole) {
+                        const int hh = row / P.n, j = row - hh * P.n, h = head * P.group + hh;
+                        if (P.sinks) l += fast_exp2(P.sinks[h] * kLog2e - m);
+                        const float inv = l == 0.f ? 0.f : 1.f / l;
+                        uint2 y;
+                        y.x = P.fp16 ? pack_act<true>(acc.x * inv, acc.y * inv) : pack_act<false>(acc.x * inv, acc.y * inv);
+                        y.y = P.fp16 ? pack_act<true>(acc.z * inv, acc.w * inv) : pack_act<false>(acc.z * inv, acc.w * inv);
+                        *reinterpret_cast<uint2*>(P.out + ((static_cast<int64_t>(seq) * P.n + j) * P.Hq + h) * kHeadDim + ch) = y;
+                        if (ch == 0) P.lse[(static_cast<int64_t>(seq) * P.cache.heads + head) * (P.blocks * kRows) + row] = m + fast_log2(l);
+                    } else {
+                        const int64_t slot = 2LL * (team * P.grid + cta) + (pieces ? 1 : 0);
+                        *reinterpret_cast<float4*>(P.o_part + (slot * kRows + r) * kHeadDim + ch) = acc;
+                        if (ch == 0) P.ml_part[slot * kRows + r] = make_float2(top, l);
+                    }
+                }
+            named_barrier_sync(1 + team, 128);
             next(take);
         }
     }
@@ -504,66 +607,97 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
     }
 }
 
-// Merges what ranges cut: a block per (sequence, KV head, block of rows) and row.  Pairs that lay in one range are done; sequences without
-// a token get their zeros here.
-template <int NT>
-__global__ void __launch_bounds__(512) cache_combine_kernel(const AttendParams P) {
+// Merges what ranges cut.  A pair's parts are the slot its first range names, then slot 2 r of the ranges r behind it.  A warp has a row,
+// four channels a lane; WARPS: 1, or 16 that share the parts of one row where few pairs are cut into many.  Sequences without a token get
+// their zeros here.
+template <int NT, int WARPS>
+__global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS) cache_combine_kernel(const AttendParams P) {
     constexpr int kRows = 8 * NT;
-    __shared__ float factor[512], part[3][128], red[2][16];
+    __shared__ float4 acc_of[WARPS][32];
+    __shared__ float2 ml_of[WARPS];
     wait_for_previous_kernel();
-    const int per = P.cache.heads * P.blocks, r = blockIdx.y, tid = threadIdx.x, ch = tid & 127, lane = tid & 31;
-    const int seq = blockIdx.x / per, item = blockIdx.x % per, head = item / P.blocks, row = (item % P.blocks) * kRows + r;
-    if (row >= P.rows) return;
-    const long long total = P.prefix[P.cache.seqs], units = total * per, grid = min(static_cast<long long>(P.grid), units);
-    const long long at = P.prefix[seq], pages = P.prefix[seq + 1] - at, first = at * per + item * pages;
+    const int per = P.cache.heads * P.blocks, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int r = WARPS == 1 ? blockIdx.y * 4 + warp : blockIdx.y, seq = blockIdx.x / per, item = blockIdx.x % per;
+    const int head = item / P.blocks, row = (item % P.blocks) * kRows + r;
+    if (r >= kRows || row >= P.rows) return;
+    const int2 parts = P.parts[blockIdx.x];
+    const bool none = P.cache.length(seq) == 0;
+    if (!none && parts.y == 0) return;
     const int hh = row / P.n, j = row - hh * P.n, h = head * P.group + hh;
-    uint16_t* out = P.out + ((static_cast<int64_t>(seq) * P.n + j) * P.Hq + h) * kHeadDim;
-    float* lse = P.lse + (static_cast<int64_t>(seq) * P.cache.heads + head) * (P.blocks * kRows) + row;
-    if (pages == 0) {
-        if (tid < 128) out[tid] = 0;
-        if (tid == 0) *lse = P.sinks ? P.sinks[h] * kLog2e : -INFINITY;
-        return;
+    const float sink = P.sinks ? P.sinks[h] * kLog2e : -INFINITY;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float m = -INFINITY, l = 0.f;
+    if (!none) {
+        constexpr int kAtOnce = 4;
+        for (int i0 = WARPS == 1 ? 0 : warp; i0 < parts.y; i0 += kAtOnce * WARPS) {
+            float2 ml[kAtOnce];
+            float4 x[kAtOnce];
+#pragma unroll
+            for (int y = 0; y < kAtOnce; ++y) {
+                const int i = i0 + y * WARPS;
+                const int64_t at = static_cast<int64_t>(i == 0 ? parts.x : 2 * (parts.x / 2 + i)) * kRows + r;
+                ml[y] = i < parts.y ? P.ml_part[at] : make_float2(-INFINITY, 0.f);
+                x[y] = i < parts.y ? *reinterpret_cast<const float4*>(P.o_part + at * kHeadDim + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            float top = m;
+#pragma unroll
+            for (int y = 0; y < kAtOnce; ++y) top = fmaxf(top, ml[y].x);
+            const float ref = top == -INFINITY ? 0.f : top;
+            const float old = fast_exp2(m - ref);
+            acc = make_float4(acc.x * old, acc.y * old, acc.z * old, acc.w * old);
+            l *= old;
+            m = top;
+#pragma unroll
+            for (int y = 0; y < kAtOnce; ++y) {
+                const float by = fast_exp2(ml[y].x - ref);
+                l = fmaf(ml[y].y, by, l);
+                acc = make_float4(fmaf(x[y].x, by, acc.x), fmaf(x[y].y, by, acc.y), fmaf(x[y].z, by, acc.z), fmaf(x[y].w, by, acc.w));
+            }
+        }
+        if (WARPS > 1) {
+            acc_of[warp][lane] = acc;
+            if (lane == 0) ml_of[warp] = make_float2(m, l);
+            __syncthreads();
+            if (warp > 0) return;
+            float top = m;
+            for (int w = 1; w < WARPS; ++w) top = fmaxf(top, ml_of[w].x);
+            const float ref = top == -INFINITY ? 0.f : top;
+            const float old = fast_exp2(m - ref);
+            acc = make_float4(acc.x * old, acc.y * old, acc.z * old, acc.w * old);
+            l *= old;
+            m = top;
+#pragma unroll
+            for (int w = 1; w < WARPS; ++w) {
+                const float by = fast_exp2(ml_of[w].x - ref);
+                const float4 x = acc_of[w][lane];
+                l = fmaf(ml_of[w].y, by, l);
+                acc = make_float4(fmaf(x.x, by, acc.x), fmaf(x.y, by, acc.y), fmaf(x.z, by, acc.z), fmaf(x.w, by, acc.w));
+            }
+        }
     }
-    const int c0 = static_cast<int>(((first + 1) * grid - 1) / units), c1 = static_cast<int>(((first + pages) * grid - 1) / units);
-    if (c0 == c1) return;
-    const int n = c1 - c0 + 1;   // <= grid <= 512
-    const bool second = units * c0 / grid < first;   // in its range c0 had another piece before this one
-    auto slot = [&](int i) { return 2LL * (c0 + i) + (i == 0 && second ? 1 : 0); };
-    const float2 ml = tid < n ? P.ml_part[slot(tid) * kRows + r] : make_float2(-INFINITY, 0.f);
-    float top = ml.x;
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) red[0][tid >> 5] = top;
-    __syncthreads();
-    for (int w = 0; w < 16; ++w) top = fmaxf(top, red[0][w]);
-    const float m = top == -INFINITY ? 0.f : top, by = fast_exp2(ml.x - m);
-    factor[tid] = by;
-    float l = ml.y * by;
-    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    if (lane == 0) red[1][tid >> 5] = l;
-    __syncthreads();
-    l = 0.f;
-    for (int w = 0; w < 16; ++w) l += red[1][w];
-    float acc = 0.f;
-#pragma unroll 4
-    for (int i = tid >> 7; i < n; i += 4) acc = fmaf(P.o_part[(slot(i) * kRows + r) * kHeadDim + ch], factor[i], acc);
-    if (tid >= 128) part[(tid >> 7) - 1][ch] = acc;
-    __syncthreads();
-    if (tid < 128) {
-        acc += part[0][ch] + part[1][ch] + part[2][ch];
-        if (P.sinks) l += fast_exp2(P.sinks[h] * kLog2e - m);
-        const float y = l == 0.f ? 0.f : acc / l;
-        out[ch] = static_cast<uint16_t>(P.fp16 ? pack_act<true>(y, 0.f) : pack_act<false>(y, 0.f));
-        if (tid == 0) *lse = m + fast_log2(l);
-    }
+    if (WARPS > 1 && warp > 0) return;
+    m = m == -INFINITY ? 0.f : m;
+    l += fast_exp2(sink - m);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint2 y;
+    y.x = P.fp16 ? pack_act<true>(acc.x * inv, acc.y * inv) : pack_act<false>(acc.x * inv, acc.y * inv);
+    y.y = P.fp16 ? pack_act<true>(acc.z * inv, acc.w * inv) : pack_act<false>(acc.z * inv, acc.w * inv);
+    *reinterpret_cast<uint2*>(P.out + ((static_cast<int64_t>(seq) * P.n + j) * P.Hq + h) * kHeadDim + 4 * lane) = y;
+    if (lane == 0) P.lse[(static_cast<int64_t>(seq) * P.cache.heads + head) * (P.blocks * kRows) + row] = m + fast_log2(l);
 }
 
 // The probabilities of every token, summed over the query rows of its KV head: the logits once more (half of the cache's bytes, most of
 // them still in L2), relative to the log-sum-exps that are known now.  (Keeping the logits of the first kernel instead would move 4 bytes
-// per row and token twice, as much as K's 72 bytes from nine rows on, and needs a buffer for the longest lengths.)
+// per row and token twice, as much as K's 72 bytes from nine rows on, and needs a buffer for the longest lengths.)  A block takes a range
+// of the pages of all (sequence, KV head) pairs, a warp tiles of 16 tokens; all rows' queries lie in shared memory.
 constexpr int kWeightWarps = 8;
-template <int NT>
-__global__ void __launch_bounds__(kWeightWarps * 32) cache_weights_kernel(const AttendParams P) {
-    constexpr int kRows = 8 * NT;
+struct WeightRows {
+    Queries<1> q;
+    float2 lse[32];
+};
+__global__ void __launch_bounds__(kWeightWarps * 32, 2) cache_weights_kernel(const AttendParams P, int eights, int padded) {
+    extern __shared__ uint8_t smem_raw[];
+    WeightRows* rows = reinterpret_cast<WeightRows*>(smem_raw);   // [eights]: the rows, eight at a time
     wait_for_previous_kernel();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, heads = P.cache.heads;
     const long long units = static_cast<long long>(P.prefix[P.cache.seqs]) * heads;
@@ -574,7 +708,7 @@ __global__ void __launch_bounds__(kWeightWarps * 32) cache_weights_kernel(const 
         const int mid = (lo + hi) >> 1;
         if (static_cast<long long>(P.prefix[mid]) * heads <= u0) lo = mid; else hi = mid;
     }
-    const int tok_a = warp * 16 + token_of_row(g);
+    const int tok = token_of_row(g);
     long long u = u0;
     for (int seq = lo; u < u1; ++seq) {
         const long long begin = static_cast<long long>(P.prefix[seq]) * heads;
@@ -582,44 +716,61 @@ __global__ void __launch_bounds__(kWeightWarps * 32) cache_weights_kernel(const 
         while (u < u1 && u < begin + static_cast<long long>(pages) * heads) {
             const int head = static_cast<int>((u - begin) / pages), page = static_cast<int>((u - begin) % pages);
             const int take = static_cast<int>(min(u1 - u, static_cast<long long>(pages - page)));
-            for (int block = 0; block < P.blocks; ++block) {
-                Queries<NT> Q;
-                Q.load(P, seq, head, block, lane);
-                float lse[NT][2];
+            for (int lot = 0; lot < padded; lot += eights) {   // (more rows than shared memory holds go lot by lot)
+                const int n = min(eights, padded - lot);
+                __syncthreads();
+                for (int i = warp; i < n; i += kWeightWarps) {
+                    prepare_queries<1>(rows[i].q, P, seq, head, lot + i, 0, lane);
+                    const float* lse = P.lse + (static_cast<int64_t>(seq) * heads + head) * (padded * 8) + (lot + i) * 8 + 2 * t;
+                    rows[i].lse[lane] = make_float2((lot + i) * 8 + 2 * t < P.rows ? lse[0] : 0.f, (lot + i) * 8 + 2 * t + 1 < P.rows ? lse[1] : 0.f);
+                }
+                __syncthreads();
+                const int tiles = min(take * 8, (length - page * kPage + 15) / 16);
+                uint4 kc[1][2], kn[2] = {};
+                uint2 ks[1][2], kt[2] = {};
+                int pn = -1;
+                auto fetch = [&](int tile) {   // codes and scales of a tile's tokens
+                    pn = tile < tiles ? P.cache.page(seq, page + tile / 8) : -1;
+                    if (pn < 0) return;
+                    const uint8_t* from = P.cache.record(pn, head);
+                    const int at = tile % 8 * 16 + tok;
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                    for (int y = 0; y < 2; ++y) {
+                        kn[y] = *reinterpret_cast<const uint4*>(from + kKCodes + (at + 8 * y) * 64 + t * 16);
+                        kt[y] = *reinterpret_cast<const uint2*>(from + kKScales + (at + 8 * y) * 8);
+                    }
+                };
+                fetch(warp);
+                for (int tile = warp; tile < tiles; tile += kWeightWarps) {
+                    const int pg = pn, pa = page * kPage + tile * 16 + tok - length, pb = pa + 8;
 #pragma unroll
-                    for (int c = 0; c < 2; ++c)
-                        lse[nt][c] = P.lse[(static_cast<int64_t>(seq) * heads + head) * (P.blocks * kRows) + min(block * kRows + nt * 8 + 2 * t + c, P.rows - 1)];
-                for (int i = 0; i < take; ++i) {
-                    const int first = (page + i) * kPage;
-                    if (first + warp * 16 >= length) break;
-                    const int pg = P.cache.page(seq, page + i);
+                    for (int y = 0; y < 2; ++y) {
+                        kc[0][y] = kn[y];
+                        ks[0][y] = kt[y];
+                    }
+                    fetch(tile + kWeightWarps);
                     if (pg < 0) continue;
-                    const uint8_t* from = P.cache.record(pg, head);
-                    const uint4 ka = *reinterpret_cast<const uint4*>(from + kKCodes + tok_a * 64 + t * 16);
-                    const uint4 kb = *reinterpret_cast<const uint4*>(from + kKCodes + (tok_a + 8) * 64 + t * 16);
-                    const uint2 sa = *reinterpret_cast<const uint2*>(from + kKScales + tok_a * 8);
-                    const uint2 sb = *reinterpret_cast<const uint2*>(from + kKScales + (tok_a + 8) * 8);
-                    float s[NT][4];
-                    Q.logits(s, ka, kb, sa, sb);
-                    const int pa = first + tok_a - length, pb = pa + 8;
                     float wa = 0.f, wb = 0.f;
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            if (pa < Q.limit[nt][c]) wa += fast_exp2(fmaf(s[nt][c], Q.factor[nt][c], -lse[nt][c]));
-                            if (pb < Q.limit[nt][c]) wb += fast_exp2(fmaf(s[nt][c + 2], Q.factor[nt][c], -lse[nt][c]));
-                        }
+#pragma unroll 1
+                    for (int i = 0; i < n; ++i) {
+                        const Queries<1>& Q = rows[i].q;
+                        float s[1][1][4];
+                        logits<1, 1>(s, kc, ks, Q, lane);
+                        const float2 f = Q.factor[0][lane], lse = rows[i].lse[lane];
+                        const int2 lim = Q.limit[0][lane];
+                        wa += pa < lim.x ? fast_exp2(fmaf(s[0][0][0], f.x, -lse.x)) : 0.f;
+                        wa += pa < lim.y ? fast_exp2(fmaf(s[0][0][1], f.y, -lse.y)) : 0.f;
+                        wb += pb < lim.x ? fast_exp2(fmaf(s[0][0][2], f.x, -lse.x)) : 0.f;
+                        wb += pb < lim.y ? fast_exp2(fmaf(s[0][0][3], f.y, -lse.y)) : 0.f;
+                    }
                     wa += __shfl_xor_sync(0xffffffffu, wa, 1);
                     wb += __shfl_xor_sync(0xffffffffu, wb, 1);
                     wa += __shfl_xor_sync(0xffffffffu, wa, 2);
                     wb += __shfl_xor_sync(0xffffffffu, wb, 2);
                     if (t < 2 && (t ? pb : pa) < 0) {
-                        float* to = P.weights + (static_cast<int64_t>(pg) * heads + head) * kPage + tok_a + 8 * t;
+                        float* to = P.weights + (static_cast<int64_t>(pg) * heads + head) * kPage + tile % 8 * 16 + tok + 8 * t;
                         const float w = t ? wb : wa;
-                        *to = block || P.accumulate ? *to + w : w;
+                        *to = lot || P.accumulate ? *to + w : w;
                     }
                 }
             }
@@ -629,7 +780,7 @@ __global__ void __launch_bounds__(kWeightWarps * 32) cache_weights_kernel(const 
 }
 
 struct AttendSpace {
-    int64_t prefix, o_part, ml_part, lse, bytes;
+    int64_t prefix, parts, o_part, ml_part, lse, bytes;
 };
 int tiles_for(int64_t rows) { return rows <= 8 ? 1 : 2; }
 AttendSpace carve_attend(int seqs, int Hq, int heads, int n, int grid) {
@@ -642,24 +793,32 @@ AttendSpace carve_attend(int seqs, int Hq, int heads, int n, int grid) {
         return at;
     };
     w.prefix = take(4LL * (seqs + 1));
-    w.o_part = take(2LL * grid * block * kHeadDim * 4);
-    w.ml_part = take(2LL * grid * block * 8);
+    w.parts = take(8LL * seqs * heads * (round_up(rows, block) / block));
+    const int64_t ranges = static_cast<int64_t>(grid) * (block == 8 ? kTeams<1> : kTeams<2>);
+    w.o_part = take(2 * ranges * block * kHeadDim * 4);
+    w.ml_part = take(2 * ranges * block * 8);
     w.lse = take(4LL * seqs * heads * round_up(rows, block));
     w.bytes = off;
     return w;
 }
 
+constexpr int kWeightEights = 8;   // rows / 8 whose queries the weights kernel holds at once: 25 KB
 template <int NT>
-int launch_attend(const AttendParams& P, int weights, cudaStream_t st) {
+int launch_attend(const AttendParams& P, cudaStream_t st) {
     const int sms = device_sm_count();
     if (!ensure_smem_attr(reinterpret_cast<const void*>(cache_attend_kernel<NT>), kAttendSmem<NT>)) return FMSA_ERR_CUDA;
     launch_chained(cache_attend_kernel<NT>, P.grid, kAttendThreads<NT>, kAttendSmem<NT>, st, P);
-    launch_chained(cache_combine_kernel<NT>, dim3(static_cast<unsigned>(P.cache.seqs * P.cache.heads * P.blocks), 8 * NT), 512, 0, st, P);
-    if (weights) launch_chained(cache_weights_kernel<NT>, sms * 4, kWeightWarps * 32, 0, st, P);
+    // A pair is cut into about ranges / pairs parts (+ 1): 16 warps a row where that is many.
+    const int64_t pairs = static_cast<int64_t>(P.cache.seqs) * P.cache.heads * P.blocks;
+    const int rows = P.rows < 8 * NT ? P.rows : 8 * NT;
+    if (pairs * 16 < P.grid * kTeams<NT>) launch_chained(cache_combine_kernel<NT, 16>, dim3(static_cast<unsigned>(pairs), rows), 512, 0, st, P);
+    else launch_chained(cache_combine_kernel<NT, 1>, dim3(static_cast<unsigned>(pairs), (rows + 3) / 4), 128, 0, st, P);
+    if (P.weights) {
+        const int padded = P.blocks * NT, eights = padded < kWeightEights ? padded : kWeightEights;
+        launch_chained(cache_weights_kernel, sms * 2, kWeightWarps * 32, eights * sizeof(WeightRows), st, P, eights, padded);
+    }
     return check_launch();
 }
-
-constexpr int kMaxGrid = 512;   // ranges that the combine holds the factors of
 
 }  // namespace
 }  // namespace fmsa
@@ -668,14 +827,18 @@ extern "C" int64_t fmsa_cache_attend_workspace_bytes(int32_t seqs, int32_t Hq, i
     using namespace fmsa;
     const int sms = device_sm_count();
     if (seqs <= 0 || heads <= 0 || Hq <= 0 || Hq % heads || n <= 0 || sms <= 0) return -1;
-    return carve_attend(seqs, Hq, heads, n, sms < kMaxGrid ? sms : kMaxGrid).bytes;
+    return carve_attend(seqs, Hq, heads, n, sms).bytes;
 }
 
-extern "C" int fmsa_cache_attend(const fmsa_cache4* cache, const fmsa_tensor* q, int32_t Hq, int32_t n, float scale, int32_t dtype,
-                                 const float* sinks, float* weights, int32_t accumulate, void* out, void* workspace, int64_t workspace_bytes,
-                                 int32_t* status, void* stream) {
+extern "C" int fmsa_cache_attend(const fmsa_cache_attend_args* args, void* stream) {
     using namespace fmsa;
-    FMSA_REQUIRE(cache4_ok(cache) && q && q->ptr && out && workspace && status && Hq > 0 && n > 0 && Hq % cache->heads == 0);
+    FMSA_REQUIRE(args);
+    const fmsa_cache4* cache = &args->cache;
+    const fmsa_tensor* q = &args->q;
+    const int32_t Hq = args->Hq, n = args->n, dtype = args->dtype;
+    int32_t* status = args->status;
+    void *out = args->out, *workspace = args->workspace;
+    FMSA_REQUIRE(cache4_ok(cache) && q->ptr && out && workspace && status && Hq > 0 && n > 0 && Hq % cache->heads == 0);
     FMSA_REQUIRE(dtype == FMSA_DTYPE_BF16 || dtype == FMSA_DTYPE_FP16);
     FMSA_REQUIRE(aligned16(q->ptr) && q->stride_b % 8 == 0 && q->stride_h % 8 == 0 && q->stride_s % 8 == 0);
     const int64_t rows = static_cast<int64_t>(Hq / cache->heads) * n;
@@ -685,24 +848,26 @@ extern "C" int fmsa_cache_attend(const fmsa_cache4* cache, const fmsa_tensor* q,
     const int sms = device_sm_count();
     if (sms <= 0) return FMSA_ERR_CUDA;
     AttendParams P = {};
-    P.grid = sms < kMaxGrid ? sms : kMaxGrid;
+    P.grid = sms;
     const AttendSpace w = carve_attend(cache->seqs, Hq, cache->heads, n, P.grid);
-    if (workspace_bytes < w.bytes) return FMSA_ERR_WORKSPACE;
+    if (args->workspace_bytes < w.bytes) return FMSA_ERR_WORKSPACE;
     FMSA_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0);
     char* ws = static_cast<char*>(workspace);
     P.cache = device_cache(cache, status);
     P.q = static_cast<const uint16_t*>(q->ptr);
     P.qs[0] = q->stride_b; P.qs[1] = q->stride_h; P.qs[2] = q->stride_s;
-    P.sinks = sinks;
+    P.sinks = args->sinks;
     P.out = static_cast<uint16_t*>(out);
-    P.weights = weights;
+    P.weights = args->weights;
     P.prefix = reinterpret_cast<int32_t*>(ws + w.prefix);
+    P.parts = reinterpret_cast<int2*>(ws + w.parts);
     P.o_part = reinterpret_cast<float*>(ws + w.o_part);
     P.ml_part = reinterpret_cast<float2*>(ws + w.ml_part);
     P.lse = reinterpret_cast<float*>(ws + w.lse);
     P.Hq = Hq; P.n = n; P.group = Hq / cache->heads; P.rows = static_cast<int32_t>(rows); P.blocks = static_cast<int32_t>(blocks);
-    P.fp16 = dtype == FMSA_DTYPE_FP16; P.accumulate = accumulate ? 1 : 0;
-    P.scale_log2e = scale * kLog2e;
+    P.fp16 = dtype == FMSA_DTYPE_FP16; P.accumulate = args->accumulate ? 1 : 0;
+    P.scale_log2e = args->scale * kLog2e;
+    P.magic = 0x64006400u;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return nt == 1 ? launch_attend<1>(P, weights != nullptr, st) : launch_attend<2>(P, weights != nullptr, st);
+    return nt == 1 ? launch_attend<1>(P, st) : launch_attend<2>(P, st);
 }

@@ -187,10 +187,14 @@ __global__ void __launch_bounds__(256) cache_move_kernel(const EvictParams P) {
 }  // namespace
 }  // namespace fmsa
 
-extern "C" int fmsa_cache_evict(const fmsa_cache4* cache, float* weights, const int32_t* new_table, int64_t new_table_stride,
-                                int32_t new_width, int32_t keep, int32_t recent, int32_t* new_lengths, int32_t* kept, int32_t* status,
-                                void* stream) {
+extern "C" int fmsa_cache_evict(const fmsa_cache_evict_args* args, void* stream) {
     using namespace fmsa;
+    FMSA_REQUIRE(args);
+    const fmsa_cache4* cache = &args->cache;
+    const int32_t new_width = args->new_width, keep = args->keep, recent = args->recent, *new_table = args->new_table;
+    const int64_t new_table_stride = args->new_table_stride;
+    float* weights = args->weights;
+    int32_t *new_lengths = args->new_lengths, *kept = args->kept, *status = args->status;
     FMSA_REQUIRE(cache4_ok(cache) && weights && new_table && new_lengths && kept && status);
     FMSA_REQUIRE(keep > 0 && recent >= 0 && recent <= keep && new_width > 0 && static_cast<int64_t>(new_width) * kPage >= keep);
     FMSA_REQUIRE(new_table_stride >= 0 && new_table_stride < (1LL << 31));

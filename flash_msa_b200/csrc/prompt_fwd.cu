@@ -613,19 +613,24 @@ extern "C" int64_t fmsa_prompt_workspace_bytes(int32_t B, int32_t S, int32_t Hq,
     return fmsa::prompt_space(B, S, Hq, Hkv, n_seqs, &w) ? w.bytes : -1;
 }
 
-extern "C" int fmsa_prompt_fwd(const fmsa_tensor* q, const fmsa_tensor* k, const fmsa_tensor* v, int32_t B, int32_t S, int32_t Hq, int32_t Hkv,
-                               const int32_t* cu_seqlens, int32_t n_seqs, int32_t per_batch, float scale, int32_t dtype, const float* sinks,
-                               void* out, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
+extern "C" int fmsa_prompt_fwd(const fmsa_prompt_args* args, void* stream) {
     using namespace fmsa;
+    FMSA_REQUIRE(args);
+    const fmsa_tensor *q = &args->q, *k = &args->k, *v = &args->v;
+    const int32_t B = args->B, S = args->S, Hq = args->Hq, Hkv = args->Hkv, dtype = args->dtype, *cu_seqlens = args->cu_seqlens;
+    int32_t n_seqs = args->n_seqs;
+    const float scale = args->scale;
+    void *out = args->out, *workspace = args->workspace;
+    int32_t* status = args->status;
     if (!cu_seqlens) n_seqs = 1;
     PromptSpace w;
-    FMSA_REQUIRE(q && k && v && q->ptr && k->ptr && v->ptr && out && workspace && status && aligned16(out));
+    FMSA_REQUIRE(q->ptr && k->ptr && v->ptr && out && workspace && status && aligned16(out));
     FMSA_REQUIRE(B > 0 && S > 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && n_seqs > 0 && scale > 0.f);
     FMSA_REQUIRE(dtype == FMSA_DTYPE_BF16 || dtype == FMSA_DTYPE_FP16);
     if (!prompt_space(B, S, Hq, Hkv, n_seqs, &w)) return FMSA_ERR_UNSUPPORTED;
     if (S > (1 << 30) || w.cap * Hkv >= 0x7f000000LL || static_cast<int64_t>(B) * n_seqs >= 0x7f000000LL) return FMSA_ERR_UNSUPPORTED;
     FMSA_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0);
-    if (workspace_bytes < w.bytes) return FMSA_ERR_WORKSPACE;
+    if (args->workspace_bytes < w.bytes) return FMSA_ERR_WORKSPACE;
     for (const fmsa_tensor* t : {q, k, v}) FMSA_REQUIRE(tma_compatible(t->ptr, t->stride_b, t->stride_h, t->stride_s));
     CUtensorMap tq, tk, tv;
     if (!make_tmap_heads(&tq, q->ptr, B, Hq, S, q->stride_b, q->stride_h, q->stride_s, w.group, w.tokens) ||
@@ -634,7 +639,7 @@ extern "C" int fmsa_prompt_fwd(const fmsa_tensor* q, const fmsa_tensor* k, const
         return FMSA_ERR_CUDA;
     PromptParams P = {};
     P.cu = cu_seqlens;
-    P.sinks = sinks;
+    P.sinks = args->sinks;
     P.v = static_cast<const __nv_bfloat16*>(v->ptr);
     P.vs[0] = v->stride_b; P.vs[1] = v->stride_h; P.vs[2] = v->stride_s;
     P.out = static_cast<__nv_bfloat16*>(out);
@@ -642,7 +647,7 @@ extern "C" int fmsa_prompt_fwd(const fmsa_tensor* q, const fmsa_tensor* k, const
     P.tiles = reinterpret_cast<int4*>(static_cast<char*>(workspace) + 256);
     P.status = status;
     P.B = B; P.S = S; P.Hq = Hq; P.Hkv = Hkv; P.group = w.group; P.tokens = w.tokens;
-    P.n_seqs = n_seqs; P.per_batch = per_batch ? 1 : 0; P.cap = static_cast<int32_t>(w.cap);
+    P.n_seqs = n_seqs; P.per_batch = args->per_batch ? 1 : 0; P.cap = static_cast<int32_t>(w.cap);
     while (((S + kBlock - 1) / kBlock >> P.shift) >= kPlanBins) ++P.shift;
     P.scale_log2e = scale * kLog2e;
     const int sms = device_sm_count();

@@ -281,6 +281,9 @@ def backward(p: Plan, inputs, out, grad_out, saved, grad_kl, kl_value, doc_start
     return [g.transpose(1, 2) if bshd else g for g, (_, bshd) in zip(grads, p.grad_shapes)] + [dsinks]
 
 
+_NO_TROUBLE = bytes(64)
+
+
 class StatusBoard:
     """Status words of the calls of this process, in pinned host memory that the kernels write directly (only ever when
     something is wrong), so that a call needs no word of its own, no copy and no event.  There is one word for each of a few
@@ -299,13 +302,15 @@ class StatusBoard:
             with self._lock:   # of several first calls one makes the words; kernels hold on to their address
                 if self._words is None:
                     self._keep = torch.zeros(16, dtype=torch.int32).pin_memory()
-                    self._words = (c_int32 * 16).from_address(self._keep.data_ptr())
+                    words = (c_int32 * 16).from_address(self._keep.data_ptr())
+                    self._bytes = memoryview(words)
+                    self._words = words
         self._devices.add(device)
         self.poll()
         return ctypes.addressof(self._words) + 4 * kind
 
     def poll(self) -> None:
-        if self._words is not None and any(self._words):
+        if self._words is not None and self._bytes.tobytes() != _NO_TROUBLE:
             for i, what in enumerate(self.KINDS):
                 code = self._words[i]
                 if code:

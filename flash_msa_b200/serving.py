@@ -7,12 +7,12 @@ waits for the device, and all of them can be captured in a CUDA graph (after a f
 4-bit codes with a bf16 scale per token and group of 32 channels, 144 bytes per token and head instead of 512."""
 from __future__ import annotations
 
-import contextlib
+import struct
 
 import numpy as np
 import torch
 
-from . import _lib, api, ops
+from . import _lib, api, ops, passes
 
 PAGE = 128              # FMSA_CACHE_PAGE: tokens of a page
 RECORD_BYTES = 18432    # FMSA_CACHE_RECORD_BYTES: a page of one KV head
@@ -20,12 +20,41 @@ HEAD_DIM = 128
 
 _KIND_APPEND, _KIND_ATTEND, _KIND_EVICT, _KIND_PROMPT = 4, 5, 6, 7   # passes.StatusBoard.KINDS
 
+# The argument blocks of the header.  One call packs a block: a ctypes structure filled field by field and as many arguments as a block has
+# fields took a third of a small call's host time (28 us of which the GPU needs 11, one sequence of 1000 tokens).
+_CACHE, _TENSOR = "PPPqiiii", "Pqqq"
+_APPEND_ARGS = struct.Struct("@" + _CACHE + 4 * _TENSOR + "PPP" + "iiii")
+_ATTEND_ARGS = struct.Struct("@" + _CACHE + _TENSOR + "PPPPqP" + "iiiifi")
+_EVICT_ARGS = struct.Struct("@" + _CACHE + "PPqPPP" + "iiii")
+_PROMPT_ARGS = struct.Struct("@" + 3 * _TENSOR + "PPPPqP" + "iiiiiiif")
+_NO_TENSOR = (0, 0, 0, 0)
 
-def _on(device):
-    """Kernels are launched on `device`, whichever device is the current one."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+
+def _call(what, launches, fn, block, device):
+    """Launches on `device`, whichever device is the current one, on its current stream."""
+    if device.index is not None and device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _call(what, launches, fn, block, torch.device("cuda"))
+    if ops.KERNEL_EVENTS is None:
+        status = fn(block, ops._stream(device))
+    else:
+        with ops._Timed(what, device):
+            status = fn(block, ops._stream(device))
+    if status:
+        _lib.check(status, what)
+    ops.LAUNCHES += launches
+
+
+class _Word:
+    """Address of the status word of a call of this kind (see `api._Status`, whose word of its own it uses for debugging)."""
+
+    def __init__(self, kind, device):
+        self.own = api._Status(kind, device) if api.DEBUG_CHECK_STATUS else None
+        self.ptr = self.own.ptr if self.own else passes.status_board.pointer(kind, device)
+
+    def check(self):
+        if self.own:
+            self.own.check()
 
 
 def _no_gradients(what, *tensors):
@@ -34,57 +63,74 @@ def _no_gradients(what, *tensors):
 
 
 def _activation(name, t):
-    if t.ndim != 4:
+    """The shape of an activation."""
+    shape = t.shape
+    if len(shape) != 4:
         raise ValueError(f"{name} must have shape (B, H, S, D)")
-    if t.shape[3] != HEAD_DIM:
+    if shape[3] != HEAD_DIM:
         raise NotImplementedError("Headdim must be 128")
-    if t.dtype not in (torch.bfloat16, torch.float16):
+    if t.dtype is not torch.bfloat16 and t.dtype is not torch.float16:
         raise TypeError(f"flash_msa_b200 supports bf16 and fp16 activations, got {t.dtype}")
+    return shape
 
 
 def _readable(t):
-    """`t` as kernels with plain 16-byte loads read it, copied once if it has to be."""
-    t = t.detach()
-    if t.stride(3) == 1 and not any(s % 8 for s in t.stride()[:3]) and t.data_ptr() % 16 == 0:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+    """(`t` as kernels with plain 16-byte loads read it, copied once if it has to be; address and strides)."""
+    sb, sh, ss, sd = t.stride()
+    ptr = t.data_ptr()
+    if sd != 1 or (sb | sh | ss) & 7 or ptr & 15:
+        t = t.detach().clone(memory_format=torch.contiguous_format)
+        sb, sh, ss, _ = t.stride()
+        ptr = t.data_ptr()
+    return t, (ptr, sb, sh, ss)
 
 
-def _check_cache(cache):
-    if cache.dtype != torch.uint8 or cache.ndim != 3 or cache.shape[2] != RECORD_BYTES or not cache.is_contiguous():
+def _tma_readable(t):
+    """The same for tile loads."""
+    sb, sh, ss, sd = t.stride()
+    ptr = t.data_ptr()
+    if sd != 1 or (sb | sh | ss) & 7 or ptr & 15 or sb <= 0 or sh <= 0 or ss < HEAD_DIM:
+        t = t.detach().clone(memory_format=torch.contiguous_format)
+        sb, sh, ss, _ = t.stride()
+        ptr = t.data_ptr()
+    return t, (ptr, sb, sh, ss)
+
+
+def _check_cache(cache, table, lengths, weights, seqs=None):
+    """Checks what the calls on a cache share, and returns the fields of its argument block and the number of sequences."""
+    shape = cache.shape
+    if cache.dtype is not torch.uint8 or len(shape) != 3 or shape[2] != RECORD_BYTES or not cache.is_contiguous():
         raise ValueError(f"cache must be a contiguous uint8 tensor [pages, KV heads, {RECORD_BYTES}] (see cache_empty)")
-    if cache.shape[0] == 0 or cache.shape[1] == 0 or cache.data_ptr() % 16:
+    pages, heads, _ = shape
+    records = cache.data_ptr()
+    if pages == 0 or heads == 0 or records & 15:
         raise ValueError("cache must hold at least one page and one head, on a 16-byte boundary")
+    dev = cache.device
+    stride = _check_table("block_table", table, dev)
+    n, width = table.shape
+    if seqs is not None and n != seqs:
+        raise ValueError("block_table must have a row for every sequence")
+    if lengths.dtype is not torch.int32 or lengths.ndim != 1:
+        raise TypeError("lengths must be int32 [sequences]")
+    if lengths.shape[0] != n or lengths.device != dev or not lengths.is_contiguous():
+        raise ValueError("lengths must hold one length per row of block_table, contiguous, on the cache's device")
+    if weights is not None:
+        if weights.dtype is not torch.float32 or weights.shape != (pages, heads, PAGE) or not weights.is_contiguous():
+            raise ValueError("weights must be a contiguous fp32 tensor [pages, KV heads, 128]")
+        if weights.device != dev:
+            raise ValueError("weights must be on the cache's device")
+    return (records, table.data_ptr(), lengths.data_ptr(), stride, pages, heads, n, width), n
 
 
-def _check_table(name, table, device, seqs=None):
-    if table.dtype != torch.int32 or table.ndim != 2:
+def _check_table(name, table, device):
+    if table.dtype is not torch.int32 or table.ndim != 2:
         raise TypeError(f"{name} must be int32 [sequences, pages]")
     if table.device != device:
         raise ValueError(f"{name} must be on the cache's device")
-    if table.shape[1] == 0 or (table.shape[1] > 1 and table.stride(1) != 1) or (seqs is not None and table.shape[0] != seqs):
+    stride, inner = table.stride()
+    if table.shape[1] == 0 or (inner != 1 and table.shape[1] > 1) or stride < 0:
         raise ValueError(f"{name} must have a row of at least one page for every sequence, contiguous in itself")
-
-
-def _check_lengths(lengths, seqs, device):
-    if lengths.dtype != torch.int32 or lengths.ndim != 1:
-        raise TypeError("lengths must be int32 [sequences]")
-    if lengths.device != device or lengths.shape[0] != seqs or not lengths.is_contiguous():
-        raise ValueError("lengths must hold one length per row of block_table, contiguous, on the cache's device")
-
-
-def _check_weights(weights, cache):
-    if weights is None:
-        return
-    if weights.dtype != torch.float32 or weights.shape != (cache.shape[0], cache.shape[1], PAGE) or not weights.is_contiguous():
-        raise ValueError("weights must be a contiguous fp32 tensor [pages, KV heads, 128]")
-    if weights.device != cache.device:
-        raise ValueError("weights must be on the cache's device")
-
-
-def _cache_arg(cache, table, lengths):
-    return _lib.FmsaCache4(cache.data_ptr(), table.data_ptr(), lengths.data_ptr(), table.stride(0), cache.shape[0], cache.shape[1],
-                           table.shape[0], table.shape[1])
+    return stride
 
 
 def _boundaries(cu_seqlens, total, device):
@@ -105,7 +151,8 @@ def _boundaries(cu_seqlens, total, device):
     if cu.size > ops.MAX_HOST_BOUNDARIES:
         return torch.from_numpy(cu).to(device)
     out = torch.empty(cu.shape, dtype=torch.int32, device=device)
-    ops._launch("fmsa_boundaries", 1, _lib.load().fmsa_boundaries(cu.ctypes.data, cu.size, out.data_ptr(), ops._stream(device)), device)
+    with torch.cuda.device(device):
+        ops._launch("fmsa_boundaries", 1, _lib.load().fmsa_boundaries(cu.ctypes.data, cu.size, out.data_ptr(), ops._stream(device)), device)
     return out
 
 
@@ -137,43 +184,45 @@ def cache_append(cache, k, v, block_table, lengths, cu_seqlens=None, weights=Non
     the steps that follow (zeros for skipped rows).
     The largest magnitude of 32 channels is stored exactly to bf16's rounding of a seventh of it; others are within half a scale.  A group
     that holds a value that is not finite reads as NaN, one whose values are all below 2^-80 as zeros.  Values are meant to stay below 2^100."""
-    _activation("k", k)
-    _activation("v", v)
-    _no_gradients("flash_msa_cache_append", k, v)
-    _check_cache(cache)
-    dev = cache.device
-    b, h, n, _ = k.shape
-    if v.shape != k.shape or h != cache.shape[1]:
+    shape = _activation("k", k)
+    if _activation("v", v) != shape:
         raise ValueError("k and v must agree, and have the cache's KV heads")
-    if v.dtype != k.dtype:
+    if v.dtype is not k.dtype:
         raise TypeError("k and v must have one dtype")
+    _no_gradients("flash_msa_cache_append", k, v)
+    b, h, n, _ = shape
+    fields, seqs = _check_cache(cache, block_table, lengths, weights)
+    dev = cache.device
+    if h != fields[5]:
+        raise ValueError("k and v must agree, and have the cache's KV heads")
     if k.device != dev or v.device != dev:
         raise ValueError("k, v and the cache must be on one CUDA device")
-    _check_table("block_table", block_table, dev)
-    seqs = block_table.shape[0]
-    _check_lengths(lengths, seqs, dev)
-    _check_weights(weights, cache)
-    if cu_seqlens is None and b != seqs:
-        raise ValueError("k and v must have one batch element per row of block_table (or one, with cu_seqlens)")
-    if cu_seqlens is not None and b != 1:
+    if cu_seqlens is None:
+        if b != seqs:
+            raise ValueError("k and v must have one batch element per row of block_table (or one, with cu_seqlens)")
+    elif b != 1:
         raise ValueError("packed k and v must have one batch element")
-    if cu_seqlens is not None and tuple(torch.as_tensor(cu_seqlens).shape) != (seqs + 1,):
+    elif tuple(torch.as_tensor(cu_seqlens).shape) != (seqs + 1,):
         raise ValueError("cu_seqlens must hold one boundary more than block_table has rows")
     api._require_cuda(cache)
-    with _on(dev):
+    values, to = None, _NO_TENSOR + _NO_TENSOR
+    if return_values:
+        values = (ops._grad_like(k), ops._grad_like(v))
+        to = tuple(x for t in values for x in (t.data_ptr(), *t.stride()[:3]))
+    if b and h and n:
         if cu_seqlens is not None:
             cu_seqlens = _boundaries(cu_seqlens, n, dev)
-        values = (ops._grad_like(k.detach()), ops._grad_like(v.detach())) if return_values else None
-        if k.numel() and seqs:
-            kr, vr = _readable(k), _readable(v)
-            status = api._Status(_KIND_APPEND, dev)
-            arg = ops._tensor_arg
-            ops._launch("fmsa_cache_append", 1, _lib.load().fmsa_cache_append(
-                _cache_arg(cache, block_table, lengths), arg(kr), arg(vr), b, n, ops._dtype_code(k.dtype),
-                None if cu_seqlens is None else cu_seqlens.data_ptr(), None if weights is None else weights.data_ptr(),
-                arg(values[0]) if values else None, arg(values[1]) if values else None, status.ptr, ops._stream(dev)), dev)
-            status.check()
+        k, kf = _readable(k)
+        v, vf = _readable(v)
+        word = _Word(_KIND_APPEND, dev)
+        _call("fmsa_cache_append", 1, _lib.load().fmsa_cache_append, _APPEND_ARGS.pack(
+            *fields, *kf, *vf, *to, 0 if cu_seqlens is None else cu_seqlens.data_ptr(), 0 if weights is None else weights.data_ptr(), word.ptr,
+            b, n, ops._dtype_code(k.dtype), 0), dev)
+        word.check()
     return values
+
+
+_attend_bytes = {}   # by (sequences, heads, KV heads, tokens, device): at most as many as there are batch shapes
 
 
 def cache_attention(q, cache, block_table, lengths, scale: float, sinks=None, weights=None, accumulate=True):
@@ -181,34 +230,36 @@ def cache_attention(q, cache, block_table, lengths, scale: float, sinks=None, we
     sequence i sees its first lengths[i] - n + 1 + j tokens.  Returns [B, n, Hq*128]; a row that sees no token is zero.  `sinks` as in
     `flash_msa_func`.  `weights`: fp32 [pages, Hkv, 128]: the probability every token got from this call, summed over its KV head's query
     rows, is added, or written with `accumulate=False` (what `cache_evict` goes by).  With weights, no two sequences may name one page."""
-    _activation("q", q)
+    b, hq, n, _ = _activation("q", q)
     _no_gradients("flash_msa_cache_func", q, sinks)
-    _check_cache(cache)
+    fields, _ = _check_cache(cache, block_table, lengths, weights, b)
     dev = cache.device
-    b, hq, n, _ = q.shape
     if q.device != dev:
         raise ValueError("q and the cache must be on one CUDA device")
-    if hq == 0 or hq % cache.shape[1]:
+    hkv = fields[5]
+    if hq == 0 or hq % hkv:
         raise ValueError("n_heads must be divisible by n_kv_heads")
-    _check_table("block_table", block_table, dev, b)
-    _check_lengths(lengths, b, dev)
-    _check_weights(weights, cache)
-    sinks = api._check_sinks(sinks, q)
+    logits = api._sink_logits(api._check_sinks(sinks, q))
     api._require_cuda(cache)
-    out = torch.empty(b, n, hq * HEAD_DIM, dtype=q.dtype, device=dev)
-    if not out.numel():
+    out = torch.empty((b, n, hq * HEAD_DIM), dtype=q.dtype, device=dev)
+    if b == 0 or n == 0:
         return out
-    with _on(dev):
-        lib = _lib.load()
-        qr, logits = _readable(q), api._sink_logits(sinks)
-        nbytes = lib.fmsa_cache_attend_workspace_bytes(b, hq, cache.shape[1], n)
-        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
-        status = api._Status(_KIND_ATTEND, dev)
-        ops._launch("fmsa_cache_attend", 2 if weights is None else 3, lib.fmsa_cache_attend(
-            _cache_arg(cache, block_table, lengths), ops._tensor_arg(qr), hq, n, float(scale), ops._dtype_code(q.dtype),
-            None if logits is None else logits.data_ptr(), None if weights is None else weights.data_ptr(), int(bool(accumulate)),
-            out.data_ptr(), ws.data_ptr(), nbytes, status.ptr, ops._stream(dev)), dev)
-        status.check()
+    lib = _lib.load()
+    key = (b, hq, hkv, n, dev)
+    nbytes = _attend_bytes.get(key)
+    if nbytes is None:
+        with torch.cuda.device(dev):
+            nbytes = lib.fmsa_cache_attend_workspace_bytes(b, hq, hkv, n)
+        if len(_attend_bytes) > 1024:
+            _attend_bytes.clear()
+        _attend_bytes[key] = nbytes
+    q, qf = _readable(q)
+    ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+    word = _Word(_KIND_ATTEND, dev)
+    _call("fmsa_cache_attend", 2 if weights is None else 3, lib.fmsa_cache_attend, _ATTEND_ARGS.pack(
+        *fields, *qf, 0 if logits is None else logits.data_ptr(), 0 if weights is None else weights.data_ptr(), out.data_ptr(), ws.data_ptr(),
+        nbytes, word.ptr, hq, n, ops._dtype_code(q.dtype), 1 if accumulate else 0, scale, 0), dev)
+    word.check()
     return out
 
 
@@ -218,41 +269,28 @@ def cache_evict(cache, weights, block_table, lengths, new_block_table, keep: int
     [sequences, at least keep/128 pages]) names; a sequence of at most `keep` tokens is copied whole.  Those pages must be named by no
     other row of either table; the old ones are only read, so pages that sequences share stay what they are.
     Returns (new lengths int32 [B], kept int32 [B, Hkv, keep]: the places the tokens had, -1 behind the last)."""
-    _check_cache(cache)
-    dev = cache.device
     keep, recent = int(keep), int(recent)
     if weights is None:
         raise ValueError("weights must be a contiguous fp32 tensor [pages, KV heads, 128]")
-    _check_weights(weights, cache)
-    _check_table("block_table", block_table, dev)
-    b = block_table.shape[0]
-    _check_lengths(lengths, b, dev)
-    _check_table("new_block_table", new_block_table, dev, b)
+    fields, b = _check_cache(cache, block_table, lengths, weights)
+    dev = cache.device
+    stride = _check_table("new_block_table", new_block_table, dev)
+    if new_block_table.shape[0] != b:
+        raise ValueError("new_block_table must have a row for every sequence")
     if keep < 1 or not 0 <= recent <= keep:
         raise ValueError("keep must be positive and recent between 0 and keep")
-    if new_block_table.shape[1] * PAGE < keep:
-        raise ValueError(f"new_block_table has room for {new_block_table.shape[1] * PAGE} tokens, keep is {keep}")
+    width = new_block_table.shape[1]
+    if width * PAGE < keep:
+        raise ValueError(f"new_block_table has room for {width * PAGE} tokens, keep is {keep}")
     api._require_cuda(cache)
     new_lengths = torch.empty(b, dtype=torch.int32, device=dev)
-    kept = torch.empty(b, cache.shape[1], keep, dtype=torch.int32, device=dev)
-    if not b:
-        return new_lengths, kept
-    with _on(dev):
-        status = api._Status(_KIND_EVICT, dev)
-        ops._launch("fmsa_cache_evict", 2, _lib.load().fmsa_cache_evict(
-            _cache_arg(cache, block_table, lengths), weights.data_ptr(), new_block_table.data_ptr(), new_block_table.stride(0),
-            new_block_table.shape[1], keep, recent, new_lengths.data_ptr(), kept.data_ptr(), status.ptr, ops._stream(dev)), dev)
-        status.check()
+    kept = torch.empty((b, fields[5], keep), dtype=torch.int32, device=dev)
+    if b:
+        word = _Word(_KIND_EVICT, dev)
+        _call("fmsa_cache_evict", 2, _lib.load().fmsa_cache_evict, _EVICT_ARGS.pack(
+            *fields, weights.data_ptr(), new_block_table.data_ptr(), stride, new_lengths.data_ptr(), kept.data_ptr(), word.ptr, width, keep, recent, 0), dev)
+        word.check()
     return new_lengths, kept
-
-
-def _tma_readable(t):
-    """`t` as tile loads read it, copied once if it has to be."""
-    t = t.detach()
-    st = t.stride()
-    if st[3] == 1 and all(s > 0 and s % 8 == 0 for s in st[:3]) and st[2] >= HEAD_DIM and t.data_ptr() % 16 == 0:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
 
 
 def prompt_attention(q, k, v, cu_seqlens, scale: float, sinks=None):
@@ -262,46 +300,45 @@ def prompt_attention(q, k, v, cu_seqlens, scale: float, sinks=None):
     at 0 and may end before S (rows behind the last sequence come back zero, whatever they hold).  Boundaries in host memory are checked;
     those in device memory are not waited for, and have to rise from 0 to at most S.  `sinks` as in `flash_msa_func`; scale > 0.
     For serving: it keeps nothing for a backward (training: `flash_msa_func`, `flash_msa_warmup_func`)."""
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        _activation(name, t)
-    _no_gradients("flash_msa_prompt_func", q, k, v, sinks)
-    b, hq, s, _ = q.shape
-    hkv = k.shape[1]
-    if k.shape != v.shape or k.shape[0] != b or k.shape[2] != s:
+    b, hq, s, _ = _activation("q", q)
+    shape = _activation("k", k)
+    if _activation("v", v) != shape or shape[0] != b or shape[2] != s:
         raise ValueError("q, k, and v must agree on batch, sequence, head dimension, and KV head count")
+    hkv = shape[1]
     if hkv == 0 or hq == 0 or hq % hkv:
         raise ValueError("n_heads must be divisible by n_kv_heads")
     if hq // hkv > 128:
         raise NotImplementedError("at most 128 heads may share a KV head")
-    if not q.dtype == k.dtype == v.dtype:
+    if k.dtype is not q.dtype or v.dtype is not q.dtype:
         raise TypeError("q, k, and v must have one dtype")
     dev = q.device
     if k.device != dev or v.device != dev:
         raise ValueError("q, k, and v must be on one CUDA device")
     if not scale > 0:
         raise ValueError("scale must be positive")
-    sinks = api._check_sinks(sinks, q)
+    _no_gradients("flash_msa_prompt_func", q, k, v, sinks)
+    logits = api._sink_logits(api._check_sinks(sinks, q))
+    n_seqs, per_batch = 1, 0
     if cu_seqlens is not None:
         shape = tuple(torch.as_tensor(cu_seqlens).shape)
         if len(shape) not in (1, 2) or shape[-1] < 2 or (len(shape) == 2 and shape[0] != b):
             raise ValueError("cu_seqlens must have shape [n+1] or [B, n+1]")
+        n_seqs, per_batch = shape[-1] - 1, len(shape) - 1
     api._require_cuda(q)
-    out = torch.empty(b, s, hq * HEAD_DIM, dtype=q.dtype, device=dev)
-    if not out.numel():
+    out = torch.empty((b, s, hq * HEAD_DIM), dtype=q.dtype, device=dev)
+    if b == 0 or s == 0:
         return out
-    with _on(dev):
-        lib = _lib.load()
-        n_seqs, per_batch = 1, 0
-        if cu_seqlens is not None:
-            cu_seqlens = _boundaries(cu_seqlens, s, dev)
-            n_seqs, per_batch = cu_seqlens.shape[-1] - 1, int(cu_seqlens.ndim == 2)
-        qr, kr, vr, logits = _tma_readable(q), _tma_readable(k), _tma_readable(v), api._sink_logits(sinks)
-        nbytes = lib.fmsa_prompt_workspace_bytes(b, s, hq, hkv, n_seqs)
-        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
-        status = api._Status(_KIND_PROMPT, dev)
-        ops._launch("fmsa_prompt_fwd", 2, lib.fmsa_prompt_fwd(
-            ops._tensor_arg(qr), ops._tensor_arg(kr), ops._tensor_arg(vr), b, s, hq, hkv,
-            None if cu_seqlens is None else cu_seqlens.data_ptr(), n_seqs, per_batch, float(scale), ops._dtype_code(q.dtype),
-            None if logits is None else logits.data_ptr(), out.data_ptr(), ws.data_ptr(), nbytes, status.ptr, ops._stream(dev)), dev)
-        status.check()
+    lib = _lib.load()
+    if cu_seqlens is not None:
+        cu_seqlens = _boundaries(cu_seqlens, s, dev)
+    q, qf = _tma_readable(q)
+    k, kf = _tma_readable(k)
+    v, vf = _tma_readable(v)
+    nbytes = lib.fmsa_prompt_workspace_bytes(b, s, hq, hkv, n_seqs)
+    ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+    word = _Word(_KIND_PROMPT, dev)
+    _call("fmsa_prompt_fwd", 2, lib.fmsa_prompt_fwd, _PROMPT_ARGS.pack(
+        *qf, *kf, *vf, 0 if cu_seqlens is None else cu_seqlens.data_ptr(), 0 if logits is None else logits.data_ptr(), out.data_ptr(),
+        ws.data_ptr(), nbytes, word.ptr, b, s, hq, hkv, n_seqs, per_batch, ops._dtype_code(q.dtype), scale), dev)
+    word.check()
     return out

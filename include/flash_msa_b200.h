@@ -359,34 +359,66 @@ typedef struct {
 /* Stores new keys and values (B,heads,n,128).  `lengths` count them already.  cu_seqlens NULL: the n rows of batch element i are the last
  * n tokens of sequence i (B = seqs); rows for which a sequence has no place (lengths[i] < n) are left out.  cu_seqlens [seqs+1] (B = 1):
  * rows cu_seqlens[i] .. cu_seqlens[i+1]-1 are the last tokens of sequence i; rows in no sequence are left out.
- * weights fp32 [pages][heads][128] or NULL: set to zero for the stored tokens.  k_values, v_values: NULL, or (B,heads,n,128) views that
- * receive the values the cache now holds (zero for rows left out). */
-int fmsa_cache_append(const fmsa_cache4* cache, const fmsa_tensor* k, const fmsa_tensor* v, int32_t B, int32_t n, int32_t dtype,
-                      const int32_t* cu_seqlens, float* weights, const fmsa_tensor* k_values, const fmsa_tensor* v_values, int32_t* status,
-                      void* stream);
+ * weights fp32 [pages][heads][128] or NULL: set to zero for the stored tokens.  k_values, v_values: views (B,heads,n,128) that receive the
+ * values the cache now holds (zero for rows left out), or with null pointers.  One launch. */
+typedef struct {
+    fmsa_cache4 cache;
+    fmsa_tensor k, v, k_values, v_values;
+    const int32_t* cu_seqlens;
+    float* weights;
+    int32_t* status;
+    int32_t B, n, dtype, reserved;
+} fmsa_cache_append_args;
+int fmsa_cache_append(const fmsa_cache_append_args* args, void* stream);
 
 /* Attention of the last n tokens of every sequence over the cache: query j of q (seqs,Hq,n,128) sees the first lengths[i] - n + 1 + j
  * tokens; a row that sees none is zero.  out [seqs][n][Hq*128] contiguous.  sinks fp32 [Hq] or NULL, as in fmsa_forward_args.
  * weights fp32 [pages][heads][128] or NULL: for every token below lengths[i] the probability it got, summed over the rows of its KV
  * head, is added (accumulate = 1) or written (0).  Two launches, three with weights.  workspace 256-byte aligned. */
+typedef struct {
+    fmsa_cache4 cache;
+    fmsa_tensor q;
+    const float* sinks;
+    float* weights;
+    void *out, *workspace;
+    int64_t workspace_bytes;
+    int32_t* status;
+    int32_t Hq, n, dtype, accumulate;
+    float scale;
+    int32_t reserved;
+} fmsa_cache_attend_args;
 int64_t fmsa_cache_attend_workspace_bytes(int32_t seqs, int32_t Hq, int32_t heads, int32_t n);
-int fmsa_cache_attend(const fmsa_cache4* cache, const fmsa_tensor* q, int32_t Hq, int32_t n, float scale, int32_t dtype, const float* sinks,
-                      float* weights, int32_t accumulate, void* out, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+int fmsa_cache_attend(const fmsa_cache_attend_args* args, void* stream);
 
 /* Eviction by accumulated attention weight: of every sequence and KV head min(lengths[i], keep) tokens stay, the last `recent` ones and
  * the others of largest weight (of equal ones the first, NaN above everything), in their order; they are copied, weights with them, to
  * new_table [seqs][new_width] (pages that no row of block_table names; new_width * 128 >= keep).  new_lengths [seqs];
  * kept int32 [seqs][heads][keep]: where they were, -1 behind the last.  Two launches. */
-int fmsa_cache_evict(const fmsa_cache4* cache, float* weights, const int32_t* new_table, int64_t new_table_stride, int32_t new_width,
-                     int32_t keep, int32_t recent, int32_t* new_lengths, int32_t* kept, int32_t* status, void* stream);
+typedef struct {
+    fmsa_cache4 cache;
+    float* weights;
+    const int32_t* new_table;
+    int64_t new_table_stride;
+    int32_t *new_lengths, *kept, *status;
+    int32_t new_width, keep, recent, reserved;
+} fmsa_cache_evict_args;
+int fmsa_cache_evict(const fmsa_cache_evict_args* args, void* stream);
 
 /* Causal attention over whole prompts of any length, grouped heads: q (B,Hq,S,128), k, v (B,Hkv,S,128); out [B][S][Hq*128] contiguous.
  * cu_seqlens NULL: every batch element is one sequence; else int32 [n_seqs+1] on the device (per_batch = 1: [B][n_seqs+1]), rising from
  * 0: rows cu[i] .. cu[i+1]-1 are sequence i, rows behind the last one are set to zero.  Hq/Hkv <= 128.  Two launches. */
+typedef struct {
+    fmsa_tensor q, k, v;
+    const int32_t* cu_seqlens;
+    const float* sinks;
+    void *out, *workspace;
+    int64_t workspace_bytes;
+    int32_t* status;
+    int32_t B, S, Hq, Hkv, n_seqs, per_batch, dtype;
+    float scale;
+} fmsa_prompt_args;
 int64_t fmsa_prompt_workspace_bytes(int32_t B, int32_t S, int32_t Hq, int32_t Hkv, int32_t n_seqs);
-int fmsa_prompt_fwd(const fmsa_tensor* q, const fmsa_tensor* k, const fmsa_tensor* v, int32_t B, int32_t S, int32_t Hq, int32_t Hkv,
-                    const int32_t* cu_seqlens, int32_t n_seqs, int32_t per_batch, float scale, int32_t dtype, const float* sinks, void* out,
-                    void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+int fmsa_prompt_fwd(const fmsa_prompt_args* args, void* stream);
 
 /* Boundaries in HOST memory to the device, as a kernel parameter (at most FMSA_MAX_HOST_BOUNDARIES). */
 int fmsa_boundaries(const int32_t* boundaries, int32_t n, int32_t* dst, void* stream);

@@ -103,25 +103,65 @@ def test_boundaries_that_are_refused(cu):
         serving._boundaries(cu, 8, torch.device("cpu"))
 
 
-def test_c_entries_refuse_before_they_touch_anything():
+def _block(kind, **change):
+    """An argument block that is right but for what `change` replaces (pointers that are never dereferenced)."""
+    a = dict(cache=(16, 16, 16, 2, 4, 2, 3, 2), k=(16, 256, 128, 128), v=(16, 256, 128, 128), values=(0,) * 8, q=(16, 256, 128, 128), cu=0, weights=16,
+             status=16, b=3, n=1, dtype=0, hq=4, out=256, ws=256, ws_bytes=1 << 40, scale=0.1, new=16, stride=1, width=1, keep=100, recent=10, s=100, hkv=1,
+             n_seqs=1)
+    a.update(change)
+    if kind == "append":
+        return serving._APPEND_ARGS.pack(*a["cache"], *a["k"], *a["v"], *a["values"], a["cu"], a["weights"], a["status"], a["b"], a["n"], a["dtype"], 0)
+    if kind == "attend":
+        return serving._ATTEND_ARGS.pack(*a["cache"], *a["q"], 0, a["weights"], a["out"], a["ws"], a["ws_bytes"], a["status"], a["hq"], a["n"], a["dtype"],
+                                         1, a["scale"], 0)
+    if kind == "evict":
+        return serving._EVICT_ARGS.pack(*a["cache"], a["weights"], a["new"], a["stride"], 16, 16, a["status"], a["width"], a["keep"], a["recent"], 0)
+    return serving._PROMPT_ARGS.pack(*a["q"], *a["k"], *a["v"], a["cu"], 0, a["out"], a["ws"], a["ws_bytes"], a["status"], 1, a["s"], a["hq"], a["hkv"],
+                                     a["n_seqs"], 0, a["dtype"], a["scale"])
+
+
+ODD = (0x12, 256, 128, 128)          # off the 16-byte grid
+CACHE = (16, 16, 16, 2, 4, 2, 3, 2)
+ENTRIES = {"append": "fmsa_cache_append", "attend": "fmsa_cache_attend", "evict": "fmsa_cache_evict", "prompt": "fmsa_prompt_fwd"}
+C_REFUSALS = [
+    ("append", dict(b=2), -1), ("append", dict(dtype=7), -1), ("append", dict(values=(16, 256, 128, 128, 0, 0, 0, 0)), -1), ("append", dict(k=ODD), -1),
+    ("append", dict(v=(0, 256, 128, 128)), -1), ("append", dict(v=(16, 256, 128, 12)), -1), ("append", dict(n=1 << 30), -2), ("append", dict(n=0), -1),
+    ("append", dict(status=0), -1), ("append", dict(cu=16), -1),
+    ("attend", dict(hq=5), -1), ("attend", dict(q=ODD), -1), ("attend", dict(dtype=-1), -1), ("attend", dict(out=0), -1), ("attend", dict(ws=0), -1),
+    ("evict", dict(keep=129, recent=0), -1), ("evict", dict(recent=101), -1), ("evict", dict(keep=0, recent=0), -1), ("evict", dict(weights=0), -1),
+    ("evict", dict(new=0), -1), ("evict", dict(cache=CACHE[:6] + (70000, 2)), -2),
+    ("prompt", dict(scale=0.0), -1), ("prompt", dict(scale=float("nan")), -1), ("prompt", dict(ws_bytes=100), -3), ("prompt", dict(k=ODD), -1),
+    ("prompt", dict(v=(16, 256, 128, 64)), -1), ("prompt", dict(s=(1 << 30) + 1), -2), ("prompt", dict(hq=258), -2), ("prompt", dict(hkv=3), -1),
+    ("prompt", dict(out=8), -1), ("prompt", dict(cu=16, n_seqs=0), -1)]
+C_REFUSALS += [(k, dict(cache=c), -1) for k in ("append", "attend", "evict") for c in
+               ((0,) + CACHE[1:], (8,) + CACHE[1:], (16, 0) + CACHE[2:], CACHE[:4] + (0, 2, 3, 2), CACHE[:7] + (0,), CACHE[:3] + (-1,) + CACHE[4:])]
+
+
+@pytest.mark.parametrize("kind,change,status", C_REFUSALS)
+def test_c_entries_refuse_before_they_touch_anything(kind, change, status):
     lib = _lib.load()
-    c = _lib.FmsaCache4(0x10, 0x10, 0x10, 2, 4, 2, 3, 2)     # (never dereferenced)
-    t = _lib.FmsaTensor(0x10, 256, 128, 128)
-    r = ctypes.byref
-    assert lib.fmsa_cache_append(r(c), r(t), r(t), 2, 1, 0, None, None, None, None, 0x10, None) == -1        # B is not seqs
-    assert lib.fmsa_cache_append(r(c), r(t), r(t), 3, 1, 7, None, None, None, None, 0x10, None) == -1        # type
-    assert lib.fmsa_cache_append(r(c), r(t), r(t), 3, 1, 0, None, None, r(t), None, 0x10, None) == -1        # one of two outputs
-    odd = _lib.FmsaTensor(0x12, 256, 128, 128)
-    assert lib.fmsa_cache_append(r(c), r(odd), r(t), 3, 1, 0, None, None, None, None, 0x10, None) == -1      # off the 16-byte grid
-    assert lib.fmsa_cache_append(r(c), r(t), r(t), 3, 1 << 30, 0, None, None, None, None, 0x10, None) == -2
-    assert lib.fmsa_cache_evict(r(c), 0x10, 0x10, 1, 1, 129, 0, 0x10, 0x10, 0x10, None) == -1                # no room for keep
-    assert lib.fmsa_cache_evict(r(c), 0x10, 0x10, 1, 1, 100, 101, 0x10, 0x10, 0x10, None) == -1
-    assert lib.fmsa_cache_attend(r(c), r(t), 5, 1, 1.0, 0, None, None, 0, 0x10, 0x100, 1 << 30, 0x10, None) == -1
-    bad = _lib.FmsaCache4(0x10, 0x10, 0x10, 2, 0, 2, 3, 2)
-    assert lib.fmsa_cache_evict(r(bad), 0x10, 0x10, 1, 1, 100, 0, 0x10, 0x10, 0x10, None) == -1
-    prompt = lambda s, scale, ws, k=t: lib.fmsa_prompt_fwd(r(t), r(k), r(t), 1, s, 1, 1, None, 1, 0, scale, 0, None, 0x100, 0x100, ws, 0x10, None)
-    assert prompt(100, 0.0, 1 << 20) == -1 and prompt(100, 0.1, 100) == -3 and prompt(100, 0.1, 1 << 20, odd) == -1
-    assert prompt((1 << 30) + 1, 0.1, 1 << 40) == -2
-    assert lib.fmsa_prompt_workspace_bytes(1, 100, 3, 2, 1) == -1
+    assert getattr(lib, ENTRIES[kind])(_block(kind, **change), None) == status
+    assert getattr(lib, ENTRIES[kind])(None, None) == -1
+
+
+def test_other_c_entries():
+    lib = _lib.load()
+    assert lib.fmsa_prompt_workspace_bytes(1, 100, 3, 2, 1) == -1 and lib.fmsa_prompt_workspace_bytes(2, 100, 4, 2, 3) > 0
+    assert lib.fmsa_cache_attend_workspace_bytes(1, 3, 2, 1) == -1
     assert lib.fmsa_boundaries(None, 3, None, None) == -1
     assert lib.fmsa_boundaries((ctypes.c_int32 * 4)(), 897, 0x10, None) == -2
+
+
+def test_argument_blocks_have_the_size_of_the_headers_structures(tmp_path):
+    import shutil
+    import subprocess
+    cc = shutil.which("gcc") or shutil.which("cc")
+    assert cc
+    names = [("fmsa_cache_append_args", serving._APPEND_ARGS), ("fmsa_cache_attend_args", serving._ATTEND_ARGS),
+             ("fmsa_cache_evict_args", serving._EVICT_ARGS), ("fmsa_prompt_args", serving._PROMPT_ARGS)]
+    src = tmp_path / "sizes.c"
+    src.write_text('#include <stdio.h>\n#include "%s"\nint main(void) { printf("%s\\n", %s); return 0; }\n' % (
+        _lib.HEADER_PATH, " ".join(["%zu"] * len(names)), ", ".join(f"sizeof({n})" for n, _ in names)))
+    subprocess.run([cc, str(src), "-o", str(tmp_path / "sizes")], check=True)
+    got = subprocess.run([str(tmp_path / "sizes")], check=True, capture_output=True, text=True).stdout.split()
+    assert [int(x) for x in got] == [s.size for _, s in names]
