@@ -3,11 +3,12 @@
 // copy is independent of every other one, pages that sequences share stay what they are, and order is kept: `recent` means the same the
 // next time.)
 //
-// First kernel, a block per (sequence, KV head): the weight of rank keep - recent by three passes of a radix selection over the weights as
-// ordered whole numbers (11 + 11 + 10 bits, one histogram in shared memory), then the list of kept tokens: every warp owns a run of
-// tokens, counts, and writes behind what the warps before it count.  The weights are read from memory once (up to kKeysHeld of them are
-// held in shared memory; of longer sequences they come from L2 again).  Second kernel, a block per page that is written: 144 + 4 bytes per
-// token, bound by HBM.
+// First kernel, a block per (sequence, KV head): the weight of rank keep - recent among the weights as ordered whole numbers by up to three
+// passes of a radix selection (11 + 11 + 10 bits, one histogram in shared memory), then the list of kept tokens in order.  Up to kHeld * 512
+// tokens the numbers stay in registers, a selection ends with the digit whose keys are just those still needed, and the list comes from one
+// scan of (larger, equal) counts.  (Bit by bit, one count over the block each, it took SELECT_BITS.)  Of longer sequences kKeysHeld numbers
+// are held in shared memory and more come from L2 again; every warp counts and writes a run of tokens.
+// Second kernel, a block per page that is written: 144 + 4 bytes per token, bound by HBM, which reads 128 bytes where 64 are wanted.
 #include "cache4.cuh"
 #include "host_common.h"
 #include "sm100.cuh"
@@ -24,13 +25,142 @@ struct EvictParams {
     int32_t to_stride, to_width, keep, recent, held;
 };
 
-constexpr int kSelectThreads = 1024, kBins = 2048, kKeysHeld = 24576;
+constexpr int kSelectThreads = 1024, kBins = 2048, kKeysHeld = 24576, kHeldThreads = 512, kHeld = 64;
 
 // Larger weight, larger number; NaN above everything, the two zeros alike.
 __device__ __forceinline__ uint32_t ordered(float w) {
-    if (w != w) return 0xffffffffu;
     const uint32_t u = __float_as_uint(w + 0.f);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
+    const uint32_t v = u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
+    return w != w ? 0xffffffffu : v;
+}
+
+// Weights of the first `others` tokens of a sequence, as ordered numbers (all of them above 0).
+__device__ __forceinline__ uint32_t weight_of(const EvictParams& P, int seq, int head, int i) {
+    const int p = P.cache.page(seq, i / kPage);
+    return p < 0 ? 1u : ordered(P.weights[(static_cast<int64_t>(p) * P.cache.heads + head) * kPage + i % kPage]);
+}
+// What both forms begin with: new lengths, the end of the list, sequences that are short enough.  True if there is nothing left to do.
+__device__ __forceinline__ bool short_enough(const EvictParams& P, int seq, int head, int length, int32_t* kept) {
+    const int left = min(length, P.keep), tid = threadIdx.x;
+    if (head == 0 && tid == 0) P.new_lengths[seq] = left;
+    for (int i = left + tid; i < P.keep; i += blockDim.x) kept[i] = -1;
+    if (length > P.keep) return false;
+    for (int i = tid; i < left; i += blockDim.x) kept[i] = i;
+    return true;
+}
+
+// Sequences of up to HELD * kHeldThreads tokens.
+template <int HELD>
+__global__ void __launch_bounds__(kHeldThreads, HELD <= 16 ? 2 : 1) cache_select_held_kernel(const EvictParams P) {
+    constexpr int kWarps = kHeldThreads / 32;
+    __shared__ uint32_t bins[kBins], sums[kWarps], counts[HELD * kWarps];
+    __shared__ uint3 digit;   // the wanted one, keys of larger ones, its own keys
+    wait_for_previous_kernel();
+    const int seq = blockIdx.x / P.cache.heads, head = blockIdx.x % P.cache.heads, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int length = P.cache.length(seq);
+    int32_t* kept = P.kept + static_cast<int64_t>(blockIdx.x) * P.keep;
+    if (short_enough(P, seq, head, length, kept)) return;
+    const int others = length - P.recent;    // (recent <= keep < length)
+    const uint32_t need = P.keep - P.recent; // of these
+    uint32_t key[HELD];                      // of token kHeldThreads * j + tid; 0 behind the last
+    // (all pages, then all weights, then what they are: with a branch between two loads each would wait for the one before, 16000 cycles
+    // instead of 2000 for 8192 tokens.  A page that does not exist is page 0 until it is found out.)
+    const int32_t* table = P.cache.table + static_cast<int64_t>(seq) * P.cache.table_stride;
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) key[j] = static_cast<uint32_t>(table[min(j * kHeldThreads + tid, others - 1) / kPage]);
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) {
+        const bool fine = key[j] < static_cast<uint32_t>(P.cache.pages);
+        bad |= !fine;
+        const int64_t page = fine ? key[j] : 0u;
+        key[j] = __float_as_uint(P.weights[(page * P.cache.heads + head) * kPage + (j * kHeldThreads + tid) % kPage]);
+    }
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) key[j] = j * kHeldThreads + tid < others ? ordered(__uint_as_float(key[j])) : 0u;
+    if (bad) atomicMax(P.cache.status, kStatusBadIndex);
+    // the largest number that `need` keys reach: digit by digit, until a digit's keys are just the ones that are still needed
+    uint32_t rank = need ? 0u : 0xffffffffu, mask = 0, rest = need;
+    for (int pass = 0; pass < 3 && need; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+        for (int i = tid; i < kBins; i += kHeldThreads) bins[i] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < HELD; ++j)
+            if (key[j] && (key[j] & mask) == rank) atomicAdd(&bins[(key[j] >> shift) & ((1u << bits) - 1)], 1u);
+        __syncthreads();
+        // from the largest digit down: a thread has kRun bins
+        constexpr int kRun = kBins / kHeldThreads;
+        uint32_t n[kRun], sum = 0;
+#pragma unroll
+        for (int y = 0; y < kRun; ++y) sum += n[y] = bins[kBins - 1 - kRun * tid - y];
+        uint32_t at = sum;
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, at, o);
+            if (lane >= o) at += v;
+        }
+        if (lane == 31) sums[warp] = at;
+        __syncthreads();
+        const uint32_t w = lane < kWarps ? sums[lane] : 0;
+        at += __reduce_add_sync(0xffffffffu, lane < warp ? w : 0) - sum;   // keys of larger digits
+#pragma unroll
+        for (int y = 0; y < kRun; ++y) {
+            if (at < rest && rest <= at + n[y]) digit = make_uint3(kBins - 1 - kRun * tid - y, at, n[y]);
+            at += n[y];
+        }
+        __syncthreads();
+        const uint3 d = digit;
+        rank |= d.x << shift;
+        mask |= ((1u << bits) - 1) << shift;
+        rest -= d.y;
+        if (rest == d.z) {
+            --rank;       // (all keys from here on: none is equal to the number below)
+            break;
+        }
+    }
+    // Kept: keys above `rank`, the first ones equal to it as far as there is room, and the last tokens.  Counts of both in one word.
+    uint32_t mine[HELD];       // before this token, in its row of 32
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) {
+        const int i = j * kHeldThreads + tid;
+        const uint32_t more = __ballot_sync(0xffffffffu, i < length && (i >= others || key[j] > rank));
+        const uint32_t equal = __ballot_sync(0xffffffffu, i < others && key[j] == rank);
+        const uint32_t before = (1u << lane) - 1;
+        mine[j] = __popc(more & before) | __popc(equal & before) << 16;
+        if (lane == 0) counts[j * kWarps + warp] = __popc(more) | __popc(equal) << 16;
+    }
+    __syncthreads();
+    // exclusive sums of the counts, of which a lane of the first warp has a run (at most 32K tokens: the halves do not run over)
+    if (warp == 0) {
+        constexpr int kRun = HELD * kWarps / 32;
+        uint32_t c[kRun], sum = 0;
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) {
+            c[j] = counts[lane * kRun + j];
+            sum += c[j];
+        }
+        uint32_t at = sum;
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, at, o);
+            if (lane >= o) at += v;
+        }
+        if (lane == 31) sums[0] = at;
+        at -= sum;
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) {
+            counts[lane * kRun + j] = at;
+            at += c[j];
+        }
+    }
+    __syncthreads();
+    const uint32_t room = P.keep - (sums[0] & 0xffffu);
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) {
+        const int i = j * kHeldThreads + tid;
+        const bool more = i < length && (i >= others || key[j] > rank), equal = i < others && key[j] == rank;
+        const uint32_t at = counts[j * kWarps + warp] + mine[j], equals = at >> 16;
+        if (more || (equal && equals < room)) kept[(at & 0xffffu) + min(equals, room)] = i;
+    }
 }
 
 __global__ void __launch_bounds__(kSelectThreads) cache_select_kernel(const EvictParams P) {
@@ -39,20 +169,12 @@ __global__ void __launch_bounds__(kSelectThreads) cache_select_kernel(const Evic
     __shared__ uint32_t found, above;    // digit of the wanted rank, numbers above that digit
     wait_for_previous_kernel();
     const int seq = blockIdx.x / P.cache.heads, head = blockIdx.x % P.cache.heads, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int length = P.cache.length(seq), left = min(length, P.keep);
+    const int length = P.cache.length(seq);
     int32_t* kept = P.kept + static_cast<int64_t>(blockIdx.x) * P.keep;
-    if (head == 0 && tid == 0) P.new_lengths[seq] = left;
-    for (int i = left + tid; i < P.keep; i += kSelectThreads) kept[i] = -1;
-    if (length <= P.keep) {
-        for (int i = tid; i < left; i += kSelectThreads) kept[i] = i;
-        return;
-    }
+    if (short_enough(P, seq, head, length, kept)) return;
     const int others = length - P.recent;    // (recent <= keep < length)
     uint32_t need = P.keep - P.recent;       // of these
-    auto weight = [&](int i) {
-        const int p = P.cache.page(seq, i / kPage);
-        return p < 0 ? 0u : ordered(P.weights[(static_cast<int64_t>(p) * P.cache.heads + head) * kPage + i % kPage]);
-    };
+    auto weight = [&](int i) { return weight_of(P, seq, head, i); };
     const bool held = others <= P.held;
     if (held)
         for (int i = tid; i < others; i += kSelectThreads) keys[i] = weight(i);
@@ -136,23 +258,21 @@ __global__ void __launch_bounds__(256) cache_move_kernel(const EvictParams P) {
     __shared__ int64_t from[kPage];      // record index * 128 + slot, or -1
     wait_for_previous_kernel();
     const int tid = threadIdx.x, head = blockIdx.y, seq = blockIdx.z, first = blockIdx.x * kPage;
-    const int left = P.new_lengths[seq], tokens = min(left - first, kPage);
-    if (tokens <= 0) return;
     const int page = P.to[static_cast<int64_t>(seq) * P.to_stride + blockIdx.x];
+    bool some = false;
+    if (tid < kPage) {
+        int64_t f = -1;
+        const int at = first + tid < P.keep ? P.kept[(static_cast<int64_t>(seq) * P.cache.heads + head) * P.keep + first + tid] : -1;
+        const int p = at >= 0 ? P.cache.page(seq, at / kPage) : -1;
+        if (p >= 0) f = (static_cast<int64_t>(p) * P.cache.heads + head) * kPage + at % kPage;
+        from[tid] = f;
+        some = f >= 0;
+    }
+    if (!__syncthreads_or(some)) return;
     if (page < 0 || page >= P.cache.pages) {
         if (tid == 0) atomicMax(P.cache.status, kStatusBadIndex);
         return;
     }
-    if (tid < kPage) {
-        int64_t f = -1;
-        if (tid < tokens) {
-            const int at = P.kept[(static_cast<int64_t>(seq) * P.cache.heads + head) * P.keep + first + tid];
-            const int p = at >= 0 ? P.cache.page(seq, at / kPage) : -1;
-            if (p >= 0) f = (static_cast<int64_t>(p) * P.cache.heads + head) * kPage + at % kPage;
-        }
-        from[tid] = f;
-    }
-    __syncthreads();
     uint8_t* to = P.cache.record(page, head);
     const int part = tid & 7;            // 16 bytes of a row: four of K, four of V
     uint4 x[4];
@@ -210,11 +330,21 @@ extern "C" int fmsa_cache_evict(const fmsa_cache_evict_args* args, void* stream)
     P.keep = keep;
     P.recent = recent;
     const int64_t longest = static_cast<int64_t>(cache->width) * kPage;
-    P.held = static_cast<int32_t>(longest < kKeysHeld ? longest : kKeysHeld);
-    const size_t smem = static_cast<size_t>(P.held) * 4;
-    if (!ensure_smem_attr(reinterpret_cast<const void*>(cache_select_kernel), static_cast<size_t>(kKeysHeld) * 4)) return FMSA_ERR_CUDA;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    launch_chained(cache_select_kernel, static_cast<unsigned>(cache->seqs * cache->heads), kSelectThreads, smem, st, P);
+    const unsigned blocks = static_cast<unsigned>(cache->seqs * cache->heads);
+    // (by the longest sequence that the table can hold, which is what the host knows)
+    if (longest <= 4 * kHeldThreads) {
+        launch_chained(cache_select_held_kernel<4>, blocks, kHeldThreads, 0, st, P);
+    } else if (longest <= 16 * kHeldThreads) {
+        launch_chained(cache_select_held_kernel<16>, blocks, kHeldThreads, 0, st, P);
+    } else if (longest <= kHeld * kHeldThreads) {
+        launch_chained(cache_select_held_kernel<kHeld>, blocks, kHeldThreads, 0, st, P);
+    } else {
+        P.held = kKeysHeld;
+        const size_t smem = static_cast<size_t>(P.held) * 4;
+        if (!ensure_smem_attr(reinterpret_cast<const void*>(cache_select_kernel), smem)) return FMSA_ERR_CUDA;
+        launch_chained(cache_select_kernel, blocks, kSelectThreads, smem, st, P);
+    }
     const unsigned pages = static_cast<unsigned>((keep + kPage - 1) / kPage);
     launch_chained(cache_move_kernel, dim3(pages, static_cast<unsigned>(cache->heads), static_cast<unsigned>(cache->seqs)), 256, 0, st, P);
     return check_launch();
