@@ -8,9 +8,10 @@
 // draw (tile, KV head) from it.
 //
 // Values that no row of a tile sees - later tokens, the next sequence, whatever lies behind the last one - must not reach it, not as
-// 0 * NaN either: where the causal edge crosses a block, the group that turns its scores into probabilities first clears V's rows behind
-// the tile's last token in shared memory, and looks for values that are not finite in the others.  There are none, as a rule; where there
-// are, they are set to zero in the tile and added, after the last block, to the rows that do see them.
+// 0 * NaN either.  A tile is first done as if there were none that is not finite.  Where a result is not finite the tile is done once more,
+// carefully: where the causal edge crosses a block, the group that turns its scores into probabilities first clears V's rows behind the
+// tile's last token in shared memory, sets values that are not finite to zero in the others, and they are added, after the last block, to
+// the rows that do see them.  (Every tile done carefully: B=1 S=8100 Hq=20 Hkv=4 as eleven sequences 72 us, first like this 65.)
 #include "host_common.h"
 #include "sm100.cuh"
 #include "tma_host.h"
@@ -105,9 +106,12 @@ struct PromptItem {
     int32_t b, head, row0, count;   // batch element, KV head, first token, tokens
     int32_t lo;                     // first token of the sequence
     int32_t steps;                  // visited key blocks; < 0: no more work
+    int32_t careful;
+    // 32-key pieces of the first visited block (the last of the sequence) that the tile sees
+    __device__ __forceinline__ int pieces() const { return (row0 + count - lo - (steps - 1) * kBlock + 31) >> 5; }
 };
 
-constexpr int kPrKvStages = 5, kPrBuffers = 3, kPrRing = 2;
+constexpr int kPrKvStages = 5, kPrBuffers = 3, kPrRing = 4;
 constexpr int kPrThreads = 3 * 128;
 // Registers per thread after the warpgroups re-divide the register file: 384 threads are launched with 168.
 constexpr int kPrRegsLaunch = 168, kPrRegsSoftmax = 208, kPrRegsMisc = 88;
@@ -121,13 +125,15 @@ struct PromptCtrl {
     uint64_t sum_full[2], o_free;                // [group]
     uint64_t item_full[kPrRing], item_empty[kPrRing];
     PromptItem items[kPrRing];
-    uint32_t odd[kPrRing][2][4];                 // keys of the item's first two blocks that hold a value that is not finite
+    uint32_t odd[kPrRing][2][4];                 // careful: keys of the item's first two blocks that hold a value that is not finite
+    uint32_t again[kPrRing];                     // a result of the item is not finite
     float top[128];                              // running maximum of every row (log2 domain)
     float2 part[2][128];                         // [group] (max, sum) at the end of an item
     uint32_t tmem_slot;
 };
 constexpr size_t kPrTileBytes = static_cast<size_t>(1 + kPrKvStages) * kTileBytes;
-constexpr size_t kPrSmemBytes = kPrTileBytes + 1024 + sizeof(PromptCtrl);
+constexpr int kPrStaging = 32 * 64;              // of a softmax warp: 32 columns of its rows on their way out
+constexpr size_t kPrSmemBytes = kPrTileBytes + 8 * kPrStaging + 1024 + sizeof(PromptCtrl);
 static_assert(kPrSmemBytes <= 232448, "shared memory budget of one CTA");
 
 // As in tile_fwd.cu: rows whose maximum grows by less than this (log2) keep the old one; fp16 P are 2^7 times larger.
@@ -160,7 +166,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
     extern __shared__ uint8_t smem_raw[];
     const uint32_t tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t tile_q = tiles, tile_kv = tiles + kTileBytes;
-    PromptCtrl* sm = reinterpret_cast<PromptCtrl*>(smem_raw + (tiles - smem_u32(smem_raw)) + kPrTileBytes);
+    PromptCtrl* sm = reinterpret_cast<PromptCtrl*>(smem_raw + (tiles - smem_u32(smem_raw)) + kPrTileBytes + 8 * kPrStaging);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
@@ -228,30 +234,62 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
         if (warp == 10) {
             // =========================== items ===========================
             const uint32_t n_items = static_cast<uint32_t>(P.counter[1]) * P.Hkv;
-            for (uint32_t draw = 0;; ++draw) {
-                const uint32_t slot = draw % kPrRing;
-                if (draw >= kPrRing) wait(BAR(sm->item_empty[slot]), (draw / kPrRing - 1) & 1);
-                if (bad) break;
-                PromptItem it = {};
-                it.steps = -1;
+            uint32_t draw = 0;
+            auto publish = [&](const PromptItem& it) {   // (lane 0 has it)
+                const uint32_t slot = draw++ % kPrRing;
                 if (lane == 0) {
-                    const uint32_t u = static_cast<uint32_t>(atomicAdd(P.counter, 1));
-                    if (u < n_items) {
-                        const int4 t = P.tiles[u / P.Hkv];
-                        it.b = t.x;
-                        it.head = static_cast<int>(u % P.Hkv);
-                        it.row0 = t.y;
-                        it.count = t.z;
-                        it.lo = t.w;
-                        it.steps = (t.y + t.z - t.w + kBlock - 1) / kBlock;
-                    }
                     sm->items[slot] = it;
+                    sm->again[slot] = 0;
                     for (int i = 0; i < 8; ++i) sm->odd[slot][i >> 2][i & 3] = 0;
                 }
-                const int steps = __shfl_sync(0xffffffffu, it.steps, 0);
                 warp_arrive(BAR(sm->item_full[slot]));
-                if (steps < 0) break;
+            };
+            auto finished = [&](uint32_t d) { wait(BAR(sm->item_empty[d % kPrRing]), (d / kPrRing) & 1); };
+            for (bool more = true; more;) {
+                if (draw >= kPrRing) finished(draw - kPrRing);
+                if (bad) break;
+                PromptItem it = {};
+                if (lane == 0) {
+                    it = sm->items[draw % kPrRing];
+                    if (draw >= kPrRing && sm->again[draw % kPrRing]) {
+                        it.careful = 1;
+                    } else {
+                        it = {};
+                        it.steps = -1;
+                        const uint32_t u = static_cast<uint32_t>(atomicAdd(P.counter, 1));
+                        if (u < n_items) {
+                            const int4 t = P.tiles[u / P.Hkv];
+                            it.b = t.x;
+                            it.head = static_cast<int>(u % P.Hkv);
+                            it.row0 = t.y;
+                            it.count = t.z;
+                            it.lo = t.w;
+                            it.steps = (t.y + t.z - t.w + kBlock - 1) / kBlock;
+                        }
+                    }
+                }
+                more = __shfl_sync(0xffffffffu, it.steps, 0) >= 0;
+                if (more) publish(it);
             }
+            // the items still worked on (in the other slots), those of them that are done again, and the end
+            PromptItem last[kPrRing - 1] = {};
+            const uint32_t drawn = draw;
+#pragma unroll
+            for (uint32_t i = 1; i < kPrRing; ++i) {
+                if (drawn < i || bad) continue;
+                finished(drawn - i);
+                const uint32_t slot = (drawn - i) % kPrRing;
+                if (!bad && sm->again[slot]) last[i - 1] = sm->items[slot];
+            }
+            __syncwarp();
+#pragma unroll
+            for (uint32_t i = 1; i < kPrRing; ++i) {
+                last[i - 1].careful = 1;
+                if (last[i - 1].steps > 0 && !bad) publish(last[i - 1]);
+            }
+            PromptItem none = {};
+            none.steps = -1;
+            if (!bad) publish(none);
         } else if (warp == 8 && elect_one()) {
             // =========================== tile loads ===========================
             uint32_t st = 0, ph = 1, items = 0;   // stage of the ring, phase bit of its kv_empty, items so far
@@ -294,7 +332,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
                 const uint32_t slot = draw % kPrRing;
                 wait1(BAR(sm->item_full[slot]), (draw / kPrRing) & 1);
                 if (bad) break;
-                const int steps = sm->items[slot].steps;
+                const int steps = sm->items[slot].steps, pieces = sm->items[slot].pieces();
                 if (steps < 0) break;
                 if (!pv) wait1(BAR(sm->q_full), draw & 1);
                 // position of K_t: t, and one for every V before it (V_u comes before K_{u + 3}); of V_t: the K up to t + 2 and the V before it
@@ -324,11 +362,15 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
                         wait1(BAR(sm->kv_full[st]), ph);
                         if (bad) break;
                         tc_fence_after_sync();
-                        umma_ts<4, 8, FP16>(tmem_o, sbuf, at, t > 0);                 // O += P V_j
+                        // O += P V_j, of the first block the keys that are seen
+                        const bool part = t == 0 && pieces < 4;
+                        if (part && pieces == 1) umma_ts<2, 8, FP16>(tmem_o, sbuf, at, false);
+                        else umma_ts<4, 8, FP16>(tmem_o, sbuf, at, t > 0);
                         wait1(BAR(sm->p_full[buf][1]), bph);
                         if (bad) break;
                         tc_fence_after_sync();
-                        umma_ts<4, 8, FP16>(tmem_o, sbuf + 32, at + 64 * 128, true);
+                        if (!part) umma_ts<4, 8, FP16>(tmem_o, sbuf + 32, at + 64 * 128, true);
+                        else if (pieces == 3) umma_ts<2, 8, FP16>(tmem_o, sbuf + 32, at + 64 * 128, true);
                         umma_commit(BAR(sm->pv_done[buf]));
                         umma_commit(BAR(sm->kv_empty[st]));
                         skip(t + kPrBuffers < steps ? 2 : 1);
@@ -368,6 +410,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
             const int steps = sm->items[slot].steps;
             if (steps < 0) break;
             const int ahead = sm->items[slot].row0 - sm->items[slot].lo, count = sm->items[slot].count;   // tokens before the tile; its own
+            const bool careful = sm->items[slot].careful;
             float m = -INFINITY, l = 0.f;   // running maximum (log2 domain), and this group's sum relative to it
             const uint32_t prev = last, prev_ph = last_ph;   // of the last step of the item before
 #pragma unroll 1
@@ -377,7 +420,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
                     const int first = (steps - 1 - t) * kBlock;        // the block's first key in the sequence
                     const bool edge = first + kBlock > ahead + 1;      // (the tile's first row does not see all of it)
                     wait(BAR(sm->s_full[buf]), bph);
-                    if (edge) {
+                    if (edge && careful) {
                         // V before it is multiplied: rows behind the tile's last token become zero, values that are not finite too.  (A stage
                         // is waited for when what it held before has come: this item's first K with S, the V of the item before with its
                         // last product.  Before that the barrier's phase bit would still mean the use before.)
@@ -410,10 +453,11 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
                     }
                     if (bad) break;
                     tc_fence_after_sync();
-                    if (edge) {   // hidden logits become -inf
+                    const int seen = t == 0 ? (ahead + count - first + 31) >> 5 : 4;   // pieces of 32 keys that the tile sees
+                    if (edge) {   // logits that one row sees and another does not become -inf where they are hidden
                         const int limit = ahead + tok - first;
 #pragma unroll 1
-                        for (int c = 0; c < 128; c += 16) {
+                        for (int c = max(ahead - first + 1, 0) & ~15; c < 32 * seen; c += 16) {
                             uint32_t v[16];
                             tmem_ld16(tmem_addr(ts, quarter, c), v);
                             tmem_ld_wait();
@@ -434,6 +478,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         if (c == 2) tmem_ld_wait();
+                        if (c >= seen) continue;
 #pragma unroll
                         for (int y = 0; y < 32; y += 4) {
                             mx0 = fmax3(mx0, __uint_as_float(s[c][y]), __uint_as_float(s[c][y + 1]));
@@ -479,6 +524,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         uint32_t pk[16];
+                        if (c < seen) {
 #pragma unroll
                         for (int y = 0; y < 32; y += 4) {
                             const float2 a = f2_fma(f2_from_bits(s[c][y], s[c][y + 1]), sc2, nm2);
@@ -490,6 +536,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
                             pk[(y >> 1) + 1] = pack_act<FP16>(pb.x, pb.y);
                         }
                         tmem_st16(tmem_addr(ts, quarter, 16 * c), pk);
+                        }
                         if (c & 1) {
                             // the first product of an item overwrites O: the rows of the item before must have been read
                             if (c == 1 && t == 0 && draw > 0) wait(BAR(sm->o_free), (draw - 1) & 1);
@@ -532,32 +579,49 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
                 tc_fence_after_sync();
                 __nv_bfloat16* to = P.out + (static_cast<int64_t>(it.b) * P.S + it.row0 + tok) * (static_cast<int64_t>(P.Hq) * kHeadDim) +
                                     static_cast<int64_t>(head) * kHeadDim;
+                // Rows leave through shared memory, 32 columns at a time, so that four lanes write 64 bytes of a row: a lane with a row of its
+                // own wrote 16 bytes here and there and took 4000 cycles a tile, EPILOGUE_AFTER this way.
+                const uint32_t staged = tiles + kPrTileBytes + warp * kPrStaging;
+                int64_t out_of[4];               // where this lane's pieces of rows 8 i + lane / 4 go, or -1
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int64_t at = real ? to - P.out : -1;
+                    out_of[i] = __shfl_sync(0xffffffffu, at, 8 * i + (lane >> 2));
+                }
+                uint32_t finite = 0;             // 0 or NaN
 #pragma unroll 1
-                for (int c = 0; c < 128; c += 64) {
-                    uint32_t o[2][32];
-                    tmem_ld32(tmem_addr(tmem_o, quarter, c), o[0]);
-                    tmem_ld32(tmem_addr(tmem_o, quarter, c + 32), o[1]);
+                for (int c = 0; c < 128; c += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(tmem_addr(tmem_o, quarter, c), o);
                     tmem_ld_wait();
-                    if (c == 64) {
+                    if (c == 96) {
                         tc_fence_before_sync();
                         warp_arrive(BAR(sm->o_free));
                     }
-                    if (real) {
 #pragma unroll
-                        for (int y = 0; y < 64; y += 8) {
-                            uint32_t pk[4];
+                    for (int y = 0; y < 4; ++y) {
+                        uint32_t pk[4];
 #pragma unroll
-                            for (int z = 0; z < 8; z += 2) {
-                                const float2 r = f2_mul(f2_from_bits(o[y >> 5][(y & 31) + z], o[y >> 5][(y & 31) + z + 1]), inv2);
-                                pk[z >> 1] = pack_act<FP16>(r.x, r.y);
-                            }
-                            *reinterpret_cast<uint4*>(to + c + y) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                        for (int z = 0; z < 4; ++z) {
+                            const float2 r = f2_mul(f2_from_bits(o[8 * y + 2 * z], o[8 * y + 2 * z + 1]), inv2);
+                            pk[z] = pack_act<FP16>(r.x, r.y);
+                            finite = times_zero<FP16>(pk[z], finite);
                         }
+                        st_shared_v4(staged + lane * 64 + ((y ^ (lane >> 1 & 3)) << 4), pk[0], pk[1], pk[2], pk[3]);
                     }
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = 8 * i + (lane >> 2);
+                        const uint4 x = ld_shared_v4(staged + r * 64 + (((lane & 3) ^ (r >> 1 & 3)) << 4));
+                        if (out_of[i] >= 0) *reinterpret_cast<uint4*>(P.out + out_of[i] + c + 8 * (lane & 3)) = x;
+                    }
+                    __syncwarp();
                 }
+                if (!careful && __any_sync(0xffffffffu, real && (finite & 0x7fff7fffu)) && lane == 0) sm->again[slot] = 1;
                 // values that are not finite, for the rows that see them (what they were multiplied with does not matter)
 #pragma unroll 1
-                for (int t = 0; t < 2; ++t) {
+                for (int t = 0; careful && t < 2; ++t) {
 #pragma unroll 1
                     for (int w = 0; w < 4; ++w) {
 #pragma unroll 1
