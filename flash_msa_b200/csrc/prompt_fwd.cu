@@ -29,6 +29,7 @@ struct PromptParams {
     int4* tiles;                // [cap]: batch element, first token, tokens, first token of the sequence
     int32_t* status;
     int32_t B, S, Hq, Hkv, group, tokens, n_seqs, per_batch, cap, shift;   // tokens: of a full tile
+    int32_t direct;             // CTA u does item u: there is no list
     float scale_log2e;
 };
 
@@ -44,20 +45,24 @@ __device__ __forceinline__ void sequence_of(const PromptParams& P, int b, int i,
     }
 }
 
+// Sets the rows behind the last sequences to zero: thread `at` of `threads`.
+__device__ __forceinline__ void clear_tails(const PromptParams& P, int64_t at, int64_t threads) {
+    for (int b = 0; b < P.B; ++b) {
+        int lo, hi;
+        sequence_of(P, b, P.n_seqs - 1, lo, hi);
+        const int64_t row = static_cast<int64_t>(P.Hq) * 16;   // 16-byte pieces
+        uint4* to = reinterpret_cast<uint4*>(P.out) + (static_cast<int64_t>(b) * P.S + hi) * row;
+        for (int64_t i = at; i < (P.S - hi) * row; i += threads) to[i] = make_uint4(0, 0, 0, 0);
+    }
+}
+
 // Block 0 lists the tiles, by a counting sort on the key blocks they visit; the others set the rows behind the last sequences to zero.
 __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const PromptParams P) {
     __shared__ uint32_t bins[kPlanBins], sums[32];
     wait_for_previous_kernel();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (blockIdx.x > 0) {
-        for (int b = 0; b < P.B; ++b) {
-            int lo, hi;
-            sequence_of(P, b, P.n_seqs - 1, lo, hi);
-            const int64_t row = static_cast<int64_t>(P.Hq) * 16;   // 16-byte pieces
-            uint4* to = reinterpret_cast<uint4*>(P.out) + (static_cast<int64_t>(b) * P.S + hi) * row;
-            for (int64_t i = static_cast<int64_t>(blockIdx.x - 1) * kPlanThreads + tid; i < (P.S - hi) * row; i += static_cast<int64_t>(gridDim.x - 1) * kPlanThreads)
-                to[i] = make_uint4(0, 0, 0, 0);
-        }
+        clear_tails(P, static_cast<int64_t>(blockIdx.x - 1) * kPlanThreads + tid, static_cast<int64_t>(gridDim.x - 1) * kPlanThreads);
         return;
     }
     for (int i = tid; i < kPlanBins; i += kPlanThreads) bins[i] = 0;
@@ -233,8 +238,34 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
         reg_dec<kPrRegsMisc>();
         if (warp == 10) {
             // =========================== items ===========================
-            const uint32_t n_items = static_cast<uint32_t>(P.counter[1]) * P.Hkv;
-            uint32_t draw = 0;
+            uint32_t n_items = 0, draw = 0;
+            int4 tile = make_int4(0, 0, 0, 0);   // direct: this CTA's
+            if (!P.direct) {
+                n_items = static_cast<uint32_t>(P.counter[1]) * P.Hkv;
+            } else {
+                const int wanted = blockIdx.x / P.Hkv, pairs = P.B * P.n_seqs;
+                for (int p0 = 0, before = 0; p0 < pairs && before <= wanted; p0 += 32) {
+                    const int p = p0 + lane, b = p / P.n_seqs;
+                    int lo = 0, hi = 0;
+                    if (p < pairs) sequence_of(P, b, p - b * P.n_seqs, lo, hi);
+                    const int n = (hi - lo + P.tokens - 1) / P.tokens;
+                    int upto = n;
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                        if (lane >= o) upto += v;
+                    }
+                    const int mine = wanted - (before + upto - n);
+                    const uint32_t who = __ballot_sync(0xffffffffu, mine >= 0 && mine < n);
+                    if (who) {
+                        const int at = lo + mine * P.tokens, from = __ffs(who) - 1;
+                        tile = make_int4(__shfl_sync(0xffffffffu, b, from), __shfl_sync(0xffffffffu, at, from),
+                                         __shfl_sync(0xffffffffu, min(P.tokens, hi - at), from), __shfl_sync(0xffffffffu, lo, from));
+                        n_items = 1;
+                        break;
+                    }
+                    before += __shfl_sync(0xffffffffu, upto, 31);
+                }
+            }
             auto publish = [&](const PromptItem& it) {   // (lane 0 has it)
                 const uint32_t slot = draw++ % kPrRing;
                 if (lane == 0) {
@@ -256,11 +287,11 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
                     } else {
                         it = {};
                         it.steps = -1;
-                        const uint32_t u = static_cast<uint32_t>(atomicAdd(P.counter, 1));
+                        const uint32_t u = P.direct ? draw : static_cast<uint32_t>(atomicAdd(P.counter, 1));
                         if (u < n_items) {
-                            const int4 t = P.tiles[u / P.Hkv];
+                            const int4 t = P.direct ? tile : P.tiles[u / P.Hkv];
                             it.b = t.x;
-                            it.head = static_cast<int>(u % P.Hkv);
+                            it.head = static_cast<int>(P.direct ? blockIdx.x % P.Hkv : u % P.Hkv);
                             it.row0 = t.y;
                             it.count = t.z;
                             it.lo = t.w;
@@ -270,7 +301,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
                 }
                 more = __shfl_sync(0xffffffffu, it.steps, 0) >= 0;
                 if (more) publish(it);
+                if (more && draw == 1 && P.direct && P.cu) clear_tails(P, blockIdx.x * 32 + lane, static_cast<int64_t>(gridDim.x) * 32);
             }
+            if (draw == 0 && P.direct && P.cu) clear_tails(P, blockIdx.x * 32 + lane, static_cast<int64_t>(gridDim.x) * 32);
             // the items still worked on (in the other slots), those of them that are done again, and the end
             PromptItem last[kPrRing - 1] = {};
             const uint32_t drawn = draw;
@@ -589,12 +622,14 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
                     out_of[i] = __shfl_sync(0xffffffffu, at, 8 * i + (lane >> 2));
                 }
                 uint32_t finite = 0;             // 0 or NaN
-#pragma unroll 1
-                for (int c = 0; c < 128; c += 32) {
-                    uint32_t o[32];
-                    tmem_ld32(tmem_addr(tmem_o, quarter, c), o);
+                uint32_t o[2][32];
+                tmem_ld32(tmem_addr(tmem_o, quarter, 0), o[0]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {    // (the columns after these are on their way meanwhile)
                     tmem_ld_wait();
-                    if (c == 96) {
+                    if (c < 3) {
+                        tmem_ld32(tmem_addr(tmem_o, quarter, 32 * c + 32), o[(c + 1) & 1]);
+                    } else {
                         tc_fence_before_sync();
                         warp_arrive(BAR(sm->o_free));
                     }
@@ -603,7 +638,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
                         uint32_t pk[4];
 #pragma unroll
                         for (int z = 0; z < 4; ++z) {
-                            const float2 r = f2_mul(f2_from_bits(o[8 * y + 2 * z], o[8 * y + 2 * z + 1]), inv2);
+                            const float2 r = f2_mul(f2_from_bits(o[c & 1][8 * y + 2 * z], o[c & 1][8 * y + 2 * z + 1]), inv2);
                             pk[z] = pack_act<FP16>(r.x, r.y);
                             finite = times_zero<FP16>(pk[z], finite);
                         }
@@ -614,7 +649,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
                     for (int i = 0; i < 4; ++i) {
                         const int r = 8 * i + (lane >> 2);
                         const uint4 x = ld_shared_v4(staged + r * 64 + (((lane & 3) ^ (r >> 1 & 3)) << 4));
-                        if (out_of[i] >= 0) *reinterpret_cast<uint4*>(P.out + out_of[i] + c + 8 * (lane & 3)) = x;
+                        if (out_of[i] >= 0) *reinterpret_cast<uint4*>(P.out + out_of[i] + 32 * c + 8 * (lane & 3)) = x;
                     }
                     __syncwarp();
                 }
@@ -669,8 +704,19 @@ bool prompt_space(int B, int S, int Hq, int Hkv, int n_seqs, PromptSpace* w) {
     return true;
 }
 
+// As many CTAs as there can be tiles: each finds its own, and nothing is listed.  (Searching the sequences takes a few loads per 32 of them.)
+bool prompt_direct(const PromptSpace& w, int B, int Hkv, int n_seqs, int sms) {
+    return w.cap * Hkv <= sms && static_cast<int64_t>(B) * n_seqs <= 256;
+}
+
 }  // namespace
 }  // namespace fmsa
+
+extern "C" int32_t fmsa_prompt_launches(int32_t B, int32_t S, int32_t Hq, int32_t Hkv, int32_t n_seqs) {
+    fmsa::PromptSpace w;
+    if (!fmsa::prompt_space(B, S, Hq, Hkv, n_seqs, &w)) return -1;
+    return fmsa::prompt_direct(w, B, Hkv, n_seqs, fmsa::device_sm_count()) ? 1 : 2;
+}
 
 extern "C" int64_t fmsa_prompt_workspace_bytes(int32_t B, int32_t S, int32_t Hq, int32_t Hkv, int32_t n_seqs) {
     fmsa::PromptSpace w;
@@ -718,8 +764,9 @@ extern "C" int fmsa_prompt_fwd(const fmsa_prompt_args* args, void* stream) {
     auto kernel = dtype == FMSA_DTYPE_FP16 ? prompt_fwd_kernel<true> : prompt_fwd_kernel<false>;
     if (sms <= 0 || !ensure_smem_attr(reinterpret_cast<const void*>(kernel), kPrSmemBytes)) return FMSA_ERR_CUDA;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    launch_chained(prompt_plan_kernel, cu_seqlens ? 33 : 1, kPlanThreads, 0, st, P);
     const int64_t items = w.cap * Hkv;
+    P.direct = prompt_direct(w, B, Hkv, n_seqs, sms);
+    if (!P.direct) launch_chained(prompt_plan_kernel, cu_seqlens ? 33 : 1, kPlanThreads, 0, st, P);
     launch_chained(kernel, static_cast<unsigned>(items < sms ? items : sms), kPrThreads, kPrSmemBytes, st, tq, tk, tv, P);
     return check_launch();
 }

@@ -222,7 +222,18 @@ def cache_append(cache, k, v, block_table, lengths, cu_seqlens=None, weights=Non
     return values
 
 
-_attend_bytes = {}   # by (sequences, heads, KV heads, tokens, device): at most as many as there are batch shapes
+_sizes = {}   # what the library says of (operator, sizes, device)
+
+
+def _size(device, entry, *sizes):
+    key = (entry, device, *sizes)
+    got = _sizes.get(key)
+    if got is None:
+        if len(_sizes) >= 1024:
+            _sizes.clear()
+        with torch.cuda.device(device):
+            got = _sizes[key] = getattr(_lib.load(), entry)(*sizes)
+    return got
 
 
 def cache_attention(q, cache, block_table, lengths, scale: float, sinks=None, weights=None, accumulate=True):
@@ -241,20 +252,13 @@ def cache_attention(q, cache, block_table, lengths, scale: float, sinks=None, we
         raise ValueError("n_heads must be divisible by n_kv_heads")
     logits = api._sink_logits(api._check_sinks(sinks, q))
     api._require_cuda(cache)
-    out = torch.empty((b, n, hq * HEAD_DIM), dtype=q.dtype, device=dev)
+    out = q.new_empty((b, n, hq * HEAD_DIM))
     if b == 0 or n == 0:
         return out
     lib = _lib.load()
-    key = (b, hq, hkv, n, dev)
-    nbytes = _attend_bytes.get(key)
-    if nbytes is None:
-        with torch.cuda.device(dev):
-            nbytes = lib.fmsa_cache_attend_workspace_bytes(b, hq, hkv, n)
-        if len(_attend_bytes) > 1024:
-            _attend_bytes.clear()
-        _attend_bytes[key] = nbytes
+    nbytes = _size(dev, "fmsa_cache_attend_workspace_bytes", b, hq, hkv, n)
     q, qf = _readable(q)
-    ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+    ws = cache.new_empty(max(nbytes, 1))
     word = _Word(_KIND_ATTEND, dev)
     _call("fmsa_cache_attend", 2 if weights is None else 3, lib.fmsa_cache_attend, _ATTEND_ARGS.pack(
         *fields, *qf, 0 if logits is None else logits.data_ptr(), 0 if weights is None else weights.data_ptr(), out.data_ptr(), ws.data_ptr(),
@@ -283,8 +287,7 @@ def cache_evict(cache, weights, block_table, lengths, new_block_table, keep: int
     if width * PAGE < keep:
         raise ValueError(f"new_block_table has room for {width * PAGE} tokens, keep is {keep}")
     api._require_cuda(cache)
-    new_lengths = torch.empty(b, dtype=torch.int32, device=dev)
-    kept = torch.empty((b, fields[5], keep), dtype=torch.int32, device=dev)
+    new_lengths, kept = lengths.new_empty(b), lengths.new_empty((b, fields[5], keep))
     if b:
         word = _Word(_KIND_EVICT, dev)
         _call("fmsa_cache_evict", 2, _lib.load().fmsa_cache_evict, _EVICT_ARGS.pack(
@@ -325,7 +328,7 @@ def prompt_attention(q, k, v, cu_seqlens, scale: float, sinks=None):
             raise ValueError("cu_seqlens must have shape [n+1] or [B, n+1]")
         n_seqs, per_batch = shape[-1] - 1, len(shape) - 1
     api._require_cuda(q)
-    out = torch.empty((b, s, hq * HEAD_DIM), dtype=q.dtype, device=dev)
+    out = q.new_empty((b, s, hq * HEAD_DIM))
     if b == 0 or s == 0:
         return out
     lib = _lib.load()
@@ -334,10 +337,10 @@ def prompt_attention(q, k, v, cu_seqlens, scale: float, sinks=None):
     q, qf = _tma_readable(q)
     k, kf = _tma_readable(k)
     v, vf = _tma_readable(v)
-    nbytes = lib.fmsa_prompt_workspace_bytes(b, s, hq, hkv, n_seqs)
+    nbytes = _size(dev, "fmsa_prompt_workspace_bytes", b, s, hq, hkv, n_seqs)
     ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
     word = _Word(_KIND_PROMPT, dev)
-    _call("fmsa_prompt_fwd", 2, lib.fmsa_prompt_fwd, _PROMPT_ARGS.pack(
+    _call("fmsa_prompt_fwd", _size(dev, "fmsa_prompt_launches", b, s, hq, hkv, n_seqs), lib.fmsa_prompt_fwd, _PROMPT_ARGS.pack(
         *qf, *kf, *vf, 0 if cu_seqlens is None else cu_seqlens.data_ptr(), 0 if logits is None else logits.data_ptr(), out.data_ptr(),
         ws.data_ptr(), nbytes, word.ptr, b, s, hq, hkv, n_seqs, per_batch, ops._dtype_code(q.dtype), scale), dev)
     word.check()

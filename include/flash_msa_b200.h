@@ -406,7 +406,7 @@ int fmsa_cache_evict(const fmsa_cache_evict_args* args, void* stream);
 
 /* Causal attention over whole prompts of any length, grouped heads: q (B,Hq,S,128), k, v (B,Hkv,S,128); out [B][S][Hq*128] contiguous.
  * cu_seqlens NULL: every batch element is one sequence; else int32 [n_seqs+1] on the device (per_batch = 1: [B][n_seqs+1]), rising from
- * 0: rows cu[i] .. cu[i+1]-1 are sequence i, rows behind the last one are set to zero.  Hq/Hkv <= 128.  Two launches. */
+ * 0: rows cu[i] .. cu[i+1]-1 are sequence i, rows behind the last one are set to zero.  Hq/Hkv <= 128.  fmsa_prompt_launches() launches. */
 typedef struct {
     fmsa_tensor q, k, v;
     const int32_t* cu_seqlens;
@@ -418,6 +418,7 @@ typedef struct {
     float scale;
 } fmsa_prompt_args;
 int64_t fmsa_prompt_workspace_bytes(int32_t B, int32_t S, int32_t Hq, int32_t Hkv, int32_t n_seqs);
+int32_t fmsa_prompt_launches(int32_t B, int32_t S, int32_t Hq, int32_t Hkv, int32_t n_seqs);   /* one for few tiles, or two */
 int fmsa_prompt_fwd(const fmsa_prompt_args* args, void* stream);
 
 /* Boundaries in HOST memory to the device, as a kernel parameter (at most FMSA_MAX_HOST_BOUNDARIES). */
