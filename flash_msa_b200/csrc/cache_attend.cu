@@ -109,11 +109,6 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
                  : "memory");
 }
-__device__ __forceinline__ uint2 ld_shared_v2(uint32_t addr) {
-    uint2 v;
-    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
-    return v;
-}
 __device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ void scales_of(uint2 w, float (&s)[4]) {   // four bf16
     s[0] = __uint_as_float(w.x << 16);
@@ -407,7 +402,7 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
                     for (int c = 0; c < 4; ++c) o[nt][m][c] = 0.f;
             }
             // Two tiles of 16 tokens.  EDGE: some of them are not seen by some row, or are not there (their bytes may be anything).
-            auto two_tiles = [&](auto edge, uint32_t at, int first) {
+            auto two_tiles = [&](auto edge, const uint8_t* at, int first) {
                 constexpr bool EDGE = decltype(edge)::value;
                 float s[2][NT][4];
                 {
@@ -417,8 +412,8 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
                     for (int j = 0; j < 2; ++j)
 #pragma unroll
                         for (int y = 0; y < 2; ++y) {
-                            kc[j][y] = ld_shared_v4(at + k_at + (2 * j + y) * 512);
-                            ks[j][y] = ld_shared_v2(at + kKScales + s_at + (2 * j + y) * 64);
+                            kc[j][y] = *reinterpret_cast<const uint4*>(at + k_at + (2 * j + y) * 512);
+                            ks[j][y] = *reinterpret_cast<const uint2*>(at + kKScales + s_at + (2 * j + y) * 64);
                         }
                     logits<NT, 2>(s, kc, ks, Q, lane);
                 }
@@ -431,7 +426,7 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
-                        vs[j][y] = ld_shared_v2(at + kVScales + s_at + (2 * j + y) * 64);
+                        vs[j][y] = *reinterpret_cast<const uint2*>(at + kVScales + s_at + (2 * j + y) * 64);
                         const int place = first + tok_a + 16 * j + 8 * y - length;
                         if (EDGE && place >= 0) vs[j][y] = make_uint2(0, 0);
                         // log2 of the largest scale (a word as it stands is its upper half and less than one of its steps)
@@ -497,8 +492,8 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
                     }
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const uint2 v0 = ld_shared_v2(at + v0_at + j * 1024), v1 = ld_shared_v2(at + v1_at + j * 1024);
-                    const uint2 v2 = ld_shared_v2(at + v0_at + j * 1024 + 512), v3 = ld_shared_v2(at + v1_at + j * 1024 + 512);
+                    const uint2 v0 = *reinterpret_cast<const uint2*>(at + v0_at + j * 1024), v1 = *reinterpret_cast<const uint2*>(at + v1_at + j * 1024);
+                    const uint2 v2 = *reinterpret_cast<const uint2*>(at + v0_at + j * 1024 + 512), v3 = *reinterpret_cast<const uint2*>(at + v1_at + j * 1024 + 512);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const uint32_t sel = i & 1 ? 0x7632u : 0x5410u;
@@ -523,7 +518,7 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
                 wait(BAR(tm->full[stage]), phase);
                 const int first = (page + i) * kPage;   // first token of the page
                 if (!bad && first + tile < length) {
-                    const uint32_t at = ring + stage * kRecordBytes;
+                    const uint8_t* at = smem_raw + (ring - smem_u32(smem_raw)) + stage * kRecordBytes;
                     if (first + kPage > length - P.n + 1) two_tiles(Bool<true>(), at, first);
                     else two_tiles(Bool<false>(), at, first);
                 }
@@ -628,7 +623,7 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS) cache_combine_k
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float m = -INFINITY, l = 0.f;
     if (!none) {
-        constexpr int kAtOnce = 4;
+        constexpr int kAtOnce = WARPS == 1 ? 4 : 8;
         for (int i0 = WARPS == 1 ? 0 : warp; i0 < parts.y; i0 += kAtOnce * WARPS) {
             float2 ml[kAtOnce];
             float4 x[kAtOnce];
@@ -691,84 +686,91 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS) cache_combine_k
 // per row and token twice, as much as K's 72 bytes from nine rows on, and needs a buffer for the longest lengths.)  A block takes a range
 // of the pages of all (sequence, KV head) pairs, a warp tiles of 16 tokens; all rows' queries lie in shared memory.
 constexpr int kWeightWarps = 8;
+template <int NT>
 struct WeightRows {
-    Queries<1> q;
-    float2 lse[32];
+    Queries<NT> q;
+    float2 lse[NT][32];
 };
-__global__ void __launch_bounds__(kWeightWarps * 32, 2) cache_weights_kernel(const AttendParams P, int eights, int padded) {
+template <int NT>
+__global__ void __launch_bounds__(kWeightWarps * 32, 2) cache_weights_kernel(const AttendParams P, int held) {
     extern __shared__ uint8_t smem_raw[];
-    WeightRows* rows = reinterpret_cast<WeightRows*>(smem_raw);   // [eights]: the rows, eight at a time
+    WeightRows<NT>* rows = reinterpret_cast<WeightRows<NT>*>(smem_raw);   // [held]: blocks of rows
     wait_for_previous_kernel();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, heads = P.cache.heads;
     const long long units = static_cast<long long>(P.prefix[P.cache.seqs]) * heads;
     const long long u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
     if (u0 == u1) return;
-    int lo = 0, hi = P.cache.seqs;   // the sequence whose pages begin at or before u0
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (static_cast<long long>(P.prefix[mid]) * heads <= u0) lo = mid; else hi = mid;
-    }
+    __shared__ int begins;   // the sequence in whose pages the range begins
+    for (int b = threadIdx.x; b < P.cache.seqs; b += kWeightWarps * 32)
+        if (static_cast<long long>(P.prefix[b]) * heads <= u0 && u0 < static_cast<long long>(P.prefix[b + 1]) * heads) begins = b;
+    __syncthreads();
     const int tok = token_of_row(g);
     long long u = u0;
-    for (int seq = lo; u < u1; ++seq) {
+    for (int seq = begins; u < u1; ++seq) {
         const long long begin = static_cast<long long>(P.prefix[seq]) * heads;
         const int pages = P.prefix[seq + 1] - P.prefix[seq], length = P.cache.length(seq);
         while (u < u1 && u < begin + static_cast<long long>(pages) * heads) {
             const int head = static_cast<int>((u - begin) / pages), page = static_cast<int>((u - begin) % pages);
             const int take = static_cast<int>(min(u1 - u, static_cast<long long>(pages - page)));
-            for (int lot = 0; lot < padded; lot += eights) {   // (more rows than shared memory holds go lot by lot)
-                const int n = min(eights, padded - lot);
+            for (int lot = 0; lot < P.blocks; lot += held) {   // (more rows than shared memory holds go lot by lot)
+                const int n = min(held, P.blocks - lot);
                 __syncthreads();
-                for (int i = warp; i < n; i += kWeightWarps) {
-                    prepare_queries<1>(rows[i].q, P, seq, head, lot + i, 0, lane);
-                    const float* lse = P.lse + (static_cast<int64_t>(seq) * heads + head) * (padded * 8) + (lot + i) * 8 + 2 * t;
-                    rows[i].lse[lane] = make_float2((lot + i) * 8 + 2 * t < P.rows ? lse[0] : 0.f, (lot + i) * 8 + 2 * t + 1 < P.rows ? lse[1] : 0.f);
+                for (int i = warp; i < n * NT; i += kWeightWarps) {
+                    prepare_queries<NT>(rows[i / NT].q, P, seq, head, lot + i / NT, i % NT, lane);
+                    const int row = (lot * NT + i) * 8 + 2 * t;
+                    const float* lse = P.lse + (static_cast<int64_t>(seq) * heads + head) * (P.blocks * NT * 8) + row;
+                    rows[i / NT].lse[i % NT][lane] = make_float2(row < P.rows ? lse[0] : 0.f, row + 1 < P.rows ? lse[1] : 0.f);
                 }
                 __syncthreads();
-                const int tiles = min(take * 8, (length - page * kPage + 15) / 16);
+                // Warp w has tile w of every page.
                 uint4 kc[1][2], kn[2] = {};
                 uint2 ks[1][2], kt[2] = {};
-                int pn = -1;
-                auto fetch = [&](int tile) {   // codes and scales of a tile's tokens
-                    pn = tile < tiles ? P.cache.page(seq, page + tile / 8) : -1;
-                    if (pn < 0) return;
+                int ids = -1, pn = -1;
+                auto fetch = [&](int i) {   // codes and scales of page i's tokens
+                    if ((i & 31) == 0) ids = i + lane < take ? P.cache.page(seq, page + i + lane) : -1;
+                    pn = __shfl_sync(0xffffffffu, ids, i & 31);
+                    if (i >= take || pn < 0) return;
                     const uint8_t* from = P.cache.record(pn, head);
-                    const int at = tile % 8 * 16 + tok;
+                    const int at = warp * 16 + tok;
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
                         kn[y] = *reinterpret_cast<const uint4*>(from + kKCodes + (at + 8 * y) * 64 + t * 16);
                         kt[y] = *reinterpret_cast<const uint2*>(from + kKScales + (at + 8 * y) * 8);
                     }
                 };
-                fetch(warp);
-                for (int tile = warp; tile < tiles; tile += kWeightWarps) {
-                    const int pg = pn, pa = page * kPage + tile * 16 + tok - length, pb = pa + 8;
+                fetch(0);
+                for (int i0 = 0; i0 < take; ++i0) {
+                    const int pg = pn, pa = (page + i0) * kPage + warp * 16 + tok - length, pb = pa + 8;
+                    if (pa - tok >= 0) break;   // (no token of the tile is there)
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
                         kc[0][y] = kn[y];
                         ks[0][y] = kt[y];
                     }
-                    fetch(tile + kWeightWarps);
+                    fetch(i0 + 1);
                     if (pg < 0) continue;
                     float wa = 0.f, wb = 0.f;
 #pragma unroll 1
                     for (int i = 0; i < n; ++i) {
-                        const Queries<1>& Q = rows[i].q;
-                        float s[1][1][4];
-                        logits<1, 1>(s, kc, ks, Q, lane);
-                        const float2 f = Q.factor[0][lane], lse = rows[i].lse[lane];
-                        const int2 lim = Q.limit[0][lane];
-                        wa += pa < lim.x ? fast_exp2(fmaf(s[0][0][0], f.x, -lse.x)) : 0.f;
-                        wa += pa < lim.y ? fast_exp2(fmaf(s[0][0][1], f.y, -lse.y)) : 0.f;
-                        wb += pb < lim.x ? fast_exp2(fmaf(s[0][0][2], f.x, -lse.x)) : 0.f;
-                        wb += pb < lim.y ? fast_exp2(fmaf(s[0][0][3], f.y, -lse.y)) : 0.f;
+                        const Queries<NT>& Q = rows[i].q;
+                        float s[1][NT][4];
+                        logits<NT, 1>(s, kc, ks, Q, lane);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const float2 f = Q.factor[nt][lane], lse = rows[i].lse[nt][lane];
+                            const int2 lim = Q.limit[nt][lane];
+                            wa += pa < lim.x ? fast_exp2(fmaf(s[0][nt][0], f.x, -lse.x)) : 0.f;
+                            wa += pa < lim.y ? fast_exp2(fmaf(s[0][nt][1], f.y, -lse.y)) : 0.f;
+                            wb += pb < lim.x ? fast_exp2(fmaf(s[0][nt][2], f.x, -lse.x)) : 0.f;
+                            wb += pb < lim.y ? fast_exp2(fmaf(s[0][nt][3], f.y, -lse.y)) : 0.f;
+                        }
                     }
                     wa += __shfl_xor_sync(0xffffffffu, wa, 1);
                     wb += __shfl_xor_sync(0xffffffffu, wb, 1);
                     wa += __shfl_xor_sync(0xffffffffu, wa, 2);
                     wb += __shfl_xor_sync(0xffffffffu, wb, 2);
                     if (t < 2 && (t ? pb : pa) < 0) {
-                        float* to = P.weights + (static_cast<int64_t>(pg) * heads + head) * kPage + tile % 8 * 16 + tok + 8 * t;
+                        float* to = P.weights + (static_cast<int64_t>(pg) * heads + head) * kPage + warp * 16 + tok + 8 * t;
                         const float w = t ? wb : wa;
                         *to = lot || P.accumulate ? *to + w : w;
                     }
@@ -802,7 +804,8 @@ AttendSpace carve_attend(int seqs, int Hq, int heads, int n, int grid) {
     return w;
 }
 
-constexpr int kWeightEights = 8;   // rows / 8 whose queries the weights kernel holds at once: 25 KB
+constexpr int kWeightBlocks = 7;   // blocks of rows whose queries the weights kernel holds at once: 44 KB
+static_assert(kWeightBlocks * sizeof(WeightRows<2>) <= 48 * 1024, "more needs an attribute");
 template <int NT>
 int launch_attend(const AttendParams& P, cudaStream_t st) {
     const int sms = device_sm_count();
@@ -814,8 +817,8 @@ int launch_attend(const AttendParams& P, cudaStream_t st) {
     if (pairs * 16 < P.grid * kTeams<NT>) launch_chained(cache_combine_kernel<NT, 16>, dim3(static_cast<unsigned>(pairs), rows), 512, 0, st, P);
     else launch_chained(cache_combine_kernel<NT, 1>, dim3(static_cast<unsigned>(pairs), (rows + 3) / 4), 128, 0, st, P);
     if (P.weights) {
-        const int padded = P.blocks * NT, eights = padded < kWeightEights ? padded : kWeightEights;
-        launch_chained(cache_weights_kernel, sms * 2, kWeightWarps * 32, eights * sizeof(WeightRows), st, P, eights, padded);
+        const int held = P.blocks < kWeightBlocks ? P.blocks : kWeightBlocks;
+        launch_chained(cache_weights_kernel<NT>, sms * 2, kWeightWarps * 32, held * sizeof(WeightRows<NT>), st, P, held);
     }
     return check_launch();
 }
