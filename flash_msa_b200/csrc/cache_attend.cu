@@ -53,7 +53,9 @@ template <bool V> struct Bool { static constexpr bool value = V; };
 // tokens of a page.  (One range and one ring for all warps of an SM, which then wait for one another at the end of every pair: B=32 Hq=32
 // Hkv=8, lengths to 8192, TEAMS_BEFORE.)
 template <int NT> constexpr int kTeams = NT == 1 ? 4 : 3;
-constexpr int kStages = 2;          // records of a team
+constexpr int kParts = 4;           // halves of a record (K or V: codes and scales) of a team; K's goes back as soon as the logits are known
+constexpr int kPartBytes = kRecordBytes / 2, kPartScales = 8192;   // scales behind the codes
+static_assert(kKScales == kPartScales && kVCodes == kPartBytes && kVScales == kPartBytes + kPartScales, "the halves look alike");
 template <int NT> constexpr int kAttendThreads = (kTeams<NT> + 1) * 128;
 // Registers per thread after the warpgroups re-divide the register file.
 template <int NT> constexpr int kRegsLaunch = NT == 1 ? 96 : 128;
@@ -77,16 +79,15 @@ struct AttendTeam {
     Queries<NT> q[2];
     float4 part[4][3][NT][2][32];    // [channels of a group, warp number][other warp][][row 2t, 2t + 1][lane]: what they have of these channels
     float2 ml[4][8 * NT];            // [warp][row]: (reference, sum)
-    uint64_t full[kStages], empty[kStages], q_full[2], q_empty[2];
-    long long rest;
-    int32_t first;
+    uint64_t full[kParts], empty[kParts], q_full[2], q_empty[2];
+    int32_t first, rest, length;     // sequence in which the range begins, units of it before, its length
 };
 template <int NT>
 struct AttendCtrl {
     AttendTeam<NT> team[kTeams<NT>];
     int32_t sums[32];
 };
-template <int NT> constexpr size_t kAttendSmem = static_cast<size_t>(kStages) * kTeams<NT> * kRecordBytes + sizeof(AttendCtrl<NT>) + 128;
+template <int NT> constexpr size_t kAttendSmem = static_cast<size_t>(kParts) * kTeams<NT> * kPartBytes + sizeof(AttendCtrl<NT>) + 128;
 static_assert(kAttendSmem<1> <= 232448 && kAttendSmem<2> <= 232448, "shared memory budget of one CTA");
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0,
@@ -208,7 +209,20 @@ __device__ __forceinline__ void logits(float (&s)[J][NT][4], const uint4 (&k)[J]
     }
 }
 
-__device__ __forceinline__ int pages_of(const Cache4& c, int seq) { return (c.length(seq) + kPage - 1) / kPage; }
+// `units` pages in at most `most` ranges, the first ones one page longer: unit begin(r) is the first of range r (or `units` behind the last).
+struct Ranges {
+    int units, size, longer, n;
+    __device__ Ranges() {}
+    __device__ __forceinline__ Ranges(int all, int most) : units(all), n(min(all, most)) {
+        size = n ? all / n : 0;
+        longer = all - size * n;
+    }
+    __device__ __forceinline__ int begin(int r) const { return r < n ? size * r + min(r, longer) : units; }
+    __device__ __forceinline__ int owner(int u) const {
+        const int split = longer * (size + 1);
+        return u < split ? u / (size + 1) : longer + (u - split) / size;
+    }
+};
 
 // Logits (log2 domain) that a tile keeps below 2^kSlack times the reference before the reference is raised, and how far below the largest
 // (logit + log2 scale) the reference is set: fp16 holds p * s up to 2^(kSlack + kLift) and, at full precision, down to 2^-14.
@@ -235,14 +249,16 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
     extern __shared__ uint8_t smem_raw[];
     constexpr int kRows = 8 * NT, kT = kTeams<NT>, kThreads = kAttendThreads<NT>;
     const uint32_t base = (smem_u32(smem_raw) + 127u) & ~127u;
-    AttendCtrl<NT>* sm = reinterpret_cast<AttendCtrl<NT>*>(smem_raw + (base - smem_u32(smem_raw)) + kStages * kT * kRecordBytes);
+    AttendCtrl<NT>* sm = reinterpret_cast<AttendCtrl<NT>*>(smem_raw + (base - smem_u32(smem_raw)) + kParts * kT * kPartBytes);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     auto BAR = [&](uint64_t& b) { return smem_u32(&b); };
 
     if (tid < kT) {
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < kParts; ++i) {
             mbar_init(BAR(sm->team[tid].full[i]), 1);
             mbar_init(BAR(sm->team[tid].empty[i]), 4);
+        }
+        for (int i = 0; i < 2; ++i) {
             mbar_init(BAR(sm->team[tid].q_full[i]), 1);
             mbar_init(BAR(sm->team[tid].q_empty[i]), 4);
         }
@@ -253,18 +269,11 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
     // ---- the line of pages, and the teams' ranges of it (a unit is a page of a (sequence, KV head, block of rows)); ranges are numbered
     // team by team, so that few units go to as many SMs
     const int seqs = P.cache.seqs, per = P.cache.heads * P.blocks, cta = blockIdx.x;
-    long long units = 0, ranges = 0;
-    auto begin_of = [&](int team) {   // of the range; the end is the next one's begin
-        const long long r = static_cast<long long>(team) * P.grid + cta;
-        return r < ranges ? units * r / ranges : units;
-    };
-    auto end_of = [&](int team) {
-        const long long r = static_cast<long long>(team) * P.grid + cta;
-        return r < ranges ? units * (r + 1) / ranges : units;
-    };
-    // Pages of up to kThreads sequences, from c0 on: what(sequence, its first page, its pages, sum so far) for the thread's own; returns the sum.
-    auto scan = [&](int c0, long long before, auto&& what) {
-        const int b = c0 + tid, p = b < seqs ? pages_of(P.cache, b) : 0;
+    int units = 0;
+    Ranges R = {};
+    // Pages of up to kThreads sequences, from c0 on: what(sequence, its first page, its length, sum so far) for the thread's own; returns the sum.
+    auto scan = [&](int c0, int before, auto&& what) {
+        const int b = c0 + tid, length = b < seqs ? P.cache.length(b) : 0, p = (length + kPage - 1) / kPage;
         int sum = p;
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, sum, o);
@@ -274,50 +283,54 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
         __syncthreads();
         const int w = lane < kThreads / 32 ? sm->sums[lane] : 0;
         const int ahead = __reduce_add_sync(0xffffffffu, lane < warp ? w : 0), all = __reduce_add_sync(0xffffffffu, w);
-        what(b, before + ahead + sum - p, p, before + all);
+        what(b, before + ahead + sum - p, length, before + all);
         __syncthreads();
         return before + all;
     };
-    auto divide = [&](long long pages) {
+    auto divide = [&](int pages) {
         units = pages * per;
-        ranges = min(static_cast<long long>(P.grid) * kT, units);
+        R = Ranges(units, P.grid * kT);
     };
-    auto claim = [&](int b, long long at, int p) {
-        if (b < seqs && cta == 0) P.prefix[b] = static_cast<int32_t>(at);
+    auto claim = [&](int b, int at, int length) {
+        const int p = (length + kPage - 1) / kPage;
+        if (b < seqs && cta == 0) P.prefix[b] = at;
 #pragma unroll
         for (int i = 0; i < kT; ++i) {
-            const long long u = begin_of(i);
+            const int u = R.begin(i * P.grid + cta);
             if (at * per <= u && u < (at + p) * per) {
                 sm->team[i].first = b;
                 sm->team[i].rest = u - at * per;
+                sm->team[i].length = length;
             }
         }
     };
-    long long pages_all = 0;
+    int pages_all = 0;
     if (seqs <= kThreads) {
-        pages_all = scan(0, 0, [&](int b, long long at, int p, long long all) { divide(all); claim(b, at, p); });
+        pages_all = scan(0, 0, [&](int b, int at, int length, int all) { divide(all); claim(b, at, length); });
     } else {
-        for (int c0 = 0; c0 < seqs; c0 += kThreads) pages_all = scan(c0, pages_all, [](int, long long, int, long long) {});
+        for (int c0 = 0; c0 < seqs; c0 += kThreads) pages_all = scan(c0, pages_all, [](int, int, int, int) {});
         divide(pages_all);
-        long long before = 0;
-        for (int c0 = 0; c0 < seqs; c0 += kThreads) before = scan(c0, before, [&](int b, long long at, int p, long long) { claim(b, at, p); });
+        int before = 0;
+        for (int c0 = 0; c0 < seqs; c0 += kThreads) before = scan(c0, before, [&](int b, int at, int length, int) { claim(b, at, length); });
     }
-    if (cta == 0 && tid == 0) P.prefix[seqs] = static_cast<int32_t>(pages_all);
-    if (begin_of(0) == units) return;   // (nothing for any team)
+    if (cta == 0 && tid == 0) P.prefix[seqs] = pages_all;
+    if (R.begin(cta) == units) return;   // (nothing for any team)
 
     const bool loads = warp >= 4 * kT;
     const int team = loads ? warp - 4 * kT : warp >> 2;
     AttendTeam<NT>* tm = &sm->team[min(team, kT - 1)];
-    const uint32_t ring = base + team * kStages * kRecordBytes;
-    int left = team < kT ? static_cast<int>(end_of(team) - begin_of(team)) : 0;
-    int seq = 0, pages = 1, item = 0, page = 0;   // item: KV head * blocks + block of rows
+    const uint32_t ring = base + team * kParts * kPartBytes;
+    const int range = team * P.grid + cta;
+    int left = team < kT ? R.begin(range + 1) - R.begin(range) : 0;
+    int seq = 0, length = 0, pages = 1, item = 0, page = 0;   // item: KV head * blocks + block of rows
     if (left > 0) {
         seq = tm->first;
-        pages = pages_of(P.cache, seq);
-        item = static_cast<int>(tm->rest / pages);
-        page = static_cast<int>(tm->rest % pages);
+        length = tm->length;
+        pages = (length + kPage - 1) / kPage;
+        item = tm->rest / pages;
+        page = tm->rest - item * pages;
     }
-    uint32_t stage = 0, phase = 0, pieces = 0;   // ring position; pieces so far
+    uint32_t part = 0, phase = 0, pieces = 0;    // ring position of the next page's K (V's is one further); pieces so far
     bool bad = false;
     auto next = [&](int took) {
         left -= took;
@@ -325,12 +338,13 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
         ++pieces;
         if (left > 0 && ++item == per) {
             item = 0;
-            do ++seq; while ((pages = pages_of(P.cache, seq)) == 0);
+            do length = P.cache.length(++seq); while (length == 0);
+            pages = (length + kPage - 1) / kPage;
         }
     };
     auto step = [&]() {
-        stage ^= 1;
-        phase ^= stage ^ 1;
+        part ^= 2;
+        phase ^= part == 0;
     };
     auto wait = [&](uint32_t bar, uint32_t parity) {   // every lane of the warp calls it; after one that ran out nothing is waited for
         if (!bad) bad = __any_sync(0xffffffffu, !mbar_wait_role(bar, parity));
@@ -340,33 +354,33 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
         // =========================== pages and queries ===========================
         reg_dec<kRegsLoad<NT>>();
         while (left > 0) {
-            const int take = min(left, pages - page), head = item / P.blocks, length = P.cache.length(seq);
+            const int take = min(left, pages - page), head = item / P.blocks;
             int id = -1;
             for (int i = 0; i < take; ++i) {
                 if ((i & 31) == 0) id = i + lane < take ? P.cache.page(seq, page + i + lane) : -1;
                 const int pg = __shfl_sync(0xffffffffu, id, i & 31);
-                const uint32_t bar = BAR(tm->full[stage]);
-                wait(BAR(tm->empty[stage]), phase ^ 1);   // (the first round finds both records free)
-                if (!bad && lane == 0) {                  // (after a wait that ran out nothing is asked for; the others give up in the same way)
-                    const uint32_t to = ring + stage * kRecordBytes;
-                    const uint32_t tokens = min(kPage, (length - (page + i) * kPage + 15) & ~15);
-                    if (pg < 0) {
-                        mbar_arrive(bar);
-                    } else if (tokens == kPage) {
-                        mbar_arrive_expect_tx(bar, kRecordBytes);
-                        bulk_load(to, P.cache.record(pg, head), kRecordBytes, bar);
-                    } else {   // the last page: what of it is in use
-                        const uint8_t* from = P.cache.record(pg, head);
-                        mbar_arrive_expect_tx(bar, tokens * 144);
-                        bulk_load(to + kKCodes, from + kKCodes, tokens * 64, bar);
-                        bulk_load(to + kKScales, from + kKScales, tokens * 8, bar);
-                        bulk_load(to + kVCodes, from + kVCodes, tokens * 64, bar);
-                        bulk_load(to + kVScales, from + kVScales, tokens * 8, bar);
+                const uint32_t tokens = min(kPage, (length - (page + i) * kPage + 15) & ~15);   // of the last page what is in use
+                for (int v = 0; v < 2; ++v) {
+                    const uint32_t bar = BAR(tm->full[part + v]), to = ring + (part + v) * kPartBytes;
+                    wait(BAR(tm->empty[part + v]), phase ^ 1);   // (the first round finds all parts free)
+                    if (!bad && lane == 0) {                     // (after a wait that ran out nothing is asked for; the others give up too)
+                        if (pg < 0) {
+                            mbar_arrive(bar);
+                        } else {
+                            const uint8_t* from = P.cache.record(pg, head) + v * kPartBytes;
+                            mbar_arrive_expect_tx(bar, tokens * 72);
+                            if (tokens == kPage) {
+                                bulk_load(to, from, kPartBytes, bar);
+                            } else {
+                                bulk_load(to, from, tokens * 64, bar);
+                                bulk_load(to + kPartScales, from + kPartScales, tokens * 8, bar);
+                            }
+                        }
                     }
                 }
                 __syncwarp();
                 step();
-                if (i == min(take, kStages) - 1) {
+                if (i == min(take, kParts / 2) - 1) {
                     const uint32_t slot = pieces & 1;
                     if (pieces >= 2) wait(BAR(tm->q_empty[slot]), (pieces / 2 - 1) & 1);
 #pragma unroll 1
@@ -382,11 +396,11 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
         reg_inc<kRegsMath<NT>>();
         const int g = lane >> 2, t = lane & 3, mine = warp & 3, tile = mine * 32;
         const int tok_a = tile + token_of_row(g), tok_v0 = tile + token_of_row(2 * t), tok_v1 = tile + token_of_row(2 * t + 1);
-        const uint32_t k_at = kKCodes + tok_a * 64 + t * 16, s_at = tok_a * 8;
-        const uint32_t v0_at = kVCodes + tok_v0 * 64 + (g ^ (tok_v0 & 4)) * 8, v1_at = kVCodes + tok_v1 * 64 + (g ^ (tok_v1 & 4)) * 8;
+        const uint32_t k_at = tok_a * 64 + t * 16, s_at = kPartScales + tok_a * 8;
+        const uint32_t v0_at = kPartBytes + tok_v0 * 64 + (g ^ (tok_v0 & 4)) * 8, v1_at = kPartBytes + tok_v1 * 64 + (g ^ (tok_v1 & 4)) * 8;
         while (left > 0) {
             const int take = min(left, pages - page);
-            const int head = item / P.blocks, block = item % P.blocks, length = P.cache.length(seq);
+            const int head = item / P.blocks, block = item - head * P.blocks;
             const Queries<NT>& Q = tm->q[pieces & 1];
             wait(BAR(tm->q_full[pieces & 1]), (pieces / 2) & 1);
             float ref[NT][2], sum[NT][2], o[NT][8][4];
@@ -413,10 +427,13 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
 #pragma unroll
                         for (int y = 0; y < 2; ++y) {
                             kc[j][y] = *reinterpret_cast<const uint4*>(at + k_at + (2 * j + y) * 512);
-                            ks[j][y] = *reinterpret_cast<const uint2*>(at + kKScales + s_at + (2 * j + y) * 64);
+                            ks[j][y] = *reinterpret_cast<const uint2*>(at + s_at + (2 * j + y) * 64);
                         }
                     logits<NT, 2>(s, kc, ks, Q, lane);
                 }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(BAR(tm->empty[part]));
+                wait(BAR(tm->full[part + 1]), phase);
                 uint32_t pb[2][NT][4][2];   // p * scale of the four groups, as the second operand
                 uint2 vs[2][2];
                 float x[NT][2];
@@ -426,7 +443,7 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
-                        vs[j][y] = *reinterpret_cast<const uint2*>(at + kVScales + s_at + (2 * j + y) * 64);
+                        vs[j][y] = *reinterpret_cast<const uint2*>(at + kPartBytes + s_at + (2 * j + y) * 64);
                         const int place = first + tok_a + 16 * j + 8 * y - length;
                         if (EDGE && place >= 0) vs[j][y] = make_uint2(0, 0);
                         // log2 of the largest scale (a word as it stands is its upper half and less than one of its steps)
@@ -515,15 +532,19 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
             };
 #pragma unroll 1
             for (int i = 0; i < take; ++i) {
-                wait(BAR(tm->full[stage]), phase);
+                wait(BAR(tm->full[part]), phase);
                 const int first = (page + i) * kPage;   // first token of the page
                 if (!bad && first + tile < length) {
-                    const uint8_t* at = smem_raw + (ring - smem_u32(smem_raw)) + stage * kRecordBytes;
+                    const uint8_t* at = smem_raw + (ring - smem_u32(smem_raw)) + part * kPartBytes;
                     if (first + kPage > length - P.n + 1) two_tiles(Bool<true>(), at, first);
                     else two_tiles(Bool<false>(), at, first);
+                } else {
+                    wait(BAR(tm->full[part + 1]), phase);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(BAR(tm->empty[part]));
                 }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(BAR(tm->empty[stage]));
+                if (lane == 0) mbar_arrive(BAR(tm->empty[part + 1]));
                 step();
             }
             if (lane == 0) mbar_arrive(BAR(tm->q_empty[pieces & 1]));
@@ -552,9 +573,8 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
             named_barrier_sync(1 + team, 128);
             const bool whole = page == 0 && take == pages;
             if (page == 0 && mine == 0 && lane == 0) {   // (the part that begins a pair says where its parts are)
-                const long long r = static_cast<long long>(team) * P.grid + cta, last = begin_of(team) + (end_of(team) - begin_of(team) - left) + pages;
-                P.parts[(static_cast<int64_t>(seq) * P.cache.heads * P.blocks) + item] =
-                    make_int2(static_cast<int>(2 * r + (pieces ? 1 : 0)), whole ? 0 : static_cast<int>((last * ranges - 1) / units - r + 1));
+                const int behind = R.begin(range + 1) - left + pages;   // the unit behind the pair's last
+                P.parts[static_cast<int64_t>(seq) * per + item] = make_int2(2 * range + (pieces ? 1 : 0), whole ? 0 : R.owner(behind - 1) - range + 1);
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -586,7 +606,7 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
                         *reinterpret_cast<uint2*>(P.out + ((static_cast<int64_t>(seq) * P.n + j) * P.Hq + h) * kHeadDim + ch) = y;
                         if (ch == 0) P.lse[(static_cast<int64_t>(seq) * P.cache.heads + head) * (P.blocks * kRows) + row] = m + fast_log2(l);
                     } else {
-                        const int64_t slot = 2LL * (team * P.grid + cta) + (pieces ? 1 : 0);
+                        const int64_t slot = 2LL * range + (pieces ? 1 : 0);
                         *reinterpret_cast<float4*>(P.o_part + (slot * kRows + r) * kHeadDim + ch) = acc;
                         if (ch == 0) P.ml_part[slot * kRows + r] = make_float2(top, l);
                     }
@@ -847,7 +867,7 @@ extern "C" int fmsa_cache_attend(const fmsa_cache_attend_args* args, void* strea
     const int64_t rows = static_cast<int64_t>(Hq / cache->heads) * n;
     const int nt = tiles_for(rows);
     const int64_t blocks = (rows + 8 * nt - 1) / (8 * nt), items = blocks * cache->heads * cache->seqs;
-    if (items > 0x7fffffffLL || static_cast<int64_t>(cache->seqs) * cache->width > 0x7fffffffLL) return FMSA_ERR_UNSUPPORTED;
+    if (items > 0x7fffffffLL || items * cache->width > 0x7fffffffLL) return FMSA_ERR_UNSUPPORTED;   // (units are counted in 32 bits)
     const int sms = device_sm_count();
     if (sms <= 0) return FMSA_ERR_CUDA;
     AttendParams P = {};

@@ -30,16 +30,20 @@ _PROMPT_ARGS = struct.Struct("@" + 3 * _TENSOR + "PPPPqP" + "iiiiiiif")
 _NO_TENSOR = (0, 0, 0, 0)
 
 
+_current_device = torch._C._cuda_getDevice
+_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _call(what, launches, fn, block, device):
-    """Launches on `device`, whichever device is the current one, on its current stream."""
-    if device.index is not None and device.index != torch.cuda.current_device():
+    """Launches on `device` (an index), whichever device is the current one, on its current stream."""
+    if device != _current_device():
         with torch.cuda.device(device):
-            return _call(what, launches, fn, block, torch.device("cuda"))
+            return _call(what, launches, fn, block, device)
     if ops.KERNEL_EVENTS is None:
-        status = fn(block, ops._stream(device))
+        status = fn(block, _stream(device))
     else:
-        with ops._Timed(what, device):
-            status = fn(block, ops._stream(device))
+        with ops._Timed(what, torch.device("cuda", device)):
+            status = fn(block, _stream(device))
     if status:
         _lib.check(status, what)
     ops.LAUNCHES += launches
@@ -48,8 +52,10 @@ def _call(what, launches, fn, block, device):
 class _Word:
     """Address of the status word of a call of this kind (see `api._Status`, whose word of its own it uses for debugging)."""
 
+    __slots__ = ("own", "ptr")
+
     def __init__(self, kind, device):
-        self.own = api._Status(kind, device) if api.DEBUG_CHECK_STATUS else None
+        self.own = api._Status(kind, torch.device("cuda", device)) if api.DEBUG_CHECK_STATUS else None
         self.ptr = self.own.ptr if self.own else passes.status_board.pointer(kind, device)
 
     def check(self):
@@ -58,7 +64,12 @@ class _Word:
 
 
 def _no_gradients(what, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                break
+        else:
+            return
         raise RuntimeError(f"{what} has no backward: call it under torch.no_grad(), or with tensors that need no gradient")
 
 
@@ -97,7 +108,7 @@ def _tma_readable(t):
 
 
 def _check_cache(cache, table, lengths, weights, seqs=None):
-    """Checks what the calls on a cache share, and returns the fields of its argument block and the number of sequences."""
+    """Checks what the calls on a cache share.  Returns the fields of its argument block, the number of sequences and the device's index."""
     shape = cache.shape
     if cache.dtype is not torch.uint8 or len(shape) != 3 or shape[2] != RECORD_BYTES or not cache.is_contiguous():
         raise ValueError(f"cache must be a contiguous uint8 tensor [pages, KV heads, {RECORD_BYTES}] (see cache_empty)")
@@ -105,32 +116,37 @@ def _check_cache(cache, table, lengths, weights, seqs=None):
     records = cache.data_ptr()
     if pages == 0 or heads == 0 or records & 15:
         raise ValueError("cache must hold at least one page and one head, on a 16-byte boundary")
-    dev = cache.device
-    stride = _check_table("block_table", table, dev)
-    n, width = table.shape
+    device = cache.get_device()   # (-1: host memory)
+    (n, width), stride = _check_table("block_table", table, device)
     if seqs is not None and n != seqs:
         raise ValueError("block_table must have a row for every sequence")
     if lengths.dtype is not torch.int32 or lengths.ndim != 1:
         raise TypeError("lengths must be int32 [sequences]")
-    if lengths.shape[0] != n or lengths.device != dev or not lengths.is_contiguous():
+    if lengths.shape[0] != n or lengths.get_device() != device or not lengths.is_contiguous():
         raise ValueError("lengths must hold one length per row of block_table, contiguous, on the cache's device")
     if weights is not None:
         if weights.dtype is not torch.float32 or weights.shape != (pages, heads, PAGE) or not weights.is_contiguous():
             raise ValueError("weights must be a contiguous fp32 tensor [pages, KV heads, 128]")
-        if weights.device != dev:
+        if weights.get_device() != device:
             raise ValueError("weights must be on the cache's device")
-    return (records, table.data_ptr(), lengths.data_ptr(), stride, pages, heads, n, width), n
+    return (records, table.data_ptr(), lengths.data_ptr(), stride, pages, heads, n, width), n, device
 
 
 def _check_table(name, table, device):
-    if table.dtype is not torch.int32 or table.ndim != 2:
+    shape = table.shape
+    if table.dtype is not torch.int32 or len(shape) != 2:
         raise TypeError(f"{name} must be int32 [sequences, pages]")
-    if table.device != device:
+    if table.get_device() != device:
         raise ValueError(f"{name} must be on the cache's device")
     stride, inner = table.stride()
-    if table.shape[1] == 0 or (inner != 1 and table.shape[1] > 1) or stride < 0:
+    if shape[1] == 0 or (inner != 1 and shape[1] > 1) or stride < 0:
         raise ValueError(f"{name} must have a row of at least one page for every sequence, contiguous in itself")
-    return stride
+    return shape, stride
+
+
+def _require_cuda(device):
+    if device < 0:
+        raise RuntimeError("flash_msa_b200 requires CUDA tensors (there is no CPU path)")
 
 
 def _boundaries(cu_seqlens, total, device):
@@ -141,7 +157,7 @@ def _boundaries(cu_seqlens, total, device):
             raise ValueError("cu_seqlens must be on the inputs' device")
         if cu_seqlens.dtype not in (torch.int32, torch.int64):
             raise TypeError("cu_seqlens must be int32 or int64")
-        return cu_seqlens.to(torch.int32).contiguous()
+        return cu_seqlens if cu_seqlens.dtype is torch.int32 and cu_seqlens.is_contiguous() else cu_seqlens.to(torch.int32).contiguous()
     cu = torch.as_tensor(cu_seqlens).to(torch.int64).numpy()
     if cu.ndim not in (1, 2) or cu.shape[-1] < 2:
         raise ValueError("cu_seqlens must have shape [n+1] or [B, n+1]")
@@ -191,27 +207,26 @@ def cache_append(cache, k, v, block_table, lengths, cu_seqlens=None, weights=Non
         raise TypeError("k and v must have one dtype")
     _no_gradients("flash_msa_cache_append", k, v)
     b, h, n, _ = shape
-    fields, seqs = _check_cache(cache, block_table, lengths, weights)
-    dev = cache.device
+    fields, seqs, dev = _check_cache(cache, block_table, lengths, weights)
     if h != fields[5]:
         raise ValueError("k and v must agree, and have the cache's KV heads")
-    if k.device != dev or v.device != dev:
+    if k.get_device() != dev or v.get_device() != dev:
         raise ValueError("k, v and the cache must be on one CUDA device")
     if cu_seqlens is None:
         if b != seqs:
             raise ValueError("k and v must have one batch element per row of block_table (or one, with cu_seqlens)")
     elif b != 1:
         raise ValueError("packed k and v must have one batch element")
-    elif tuple(torch.as_tensor(cu_seqlens).shape) != (seqs + 1,):
+    elif tuple(cu_seqlens.shape if isinstance(cu_seqlens, torch.Tensor) else torch.as_tensor(cu_seqlens).shape) != (seqs + 1,):
         raise ValueError("cu_seqlens must hold one boundary more than block_table has rows")
-    api._require_cuda(cache)
+    _require_cuda(dev)
     values, to = None, _NO_TENSOR + _NO_TENSOR
     if return_values:
         values = (ops._grad_like(k), ops._grad_like(v))
         to = tuple(x for t in values for x in (t.data_ptr(), *t.stride()[:3]))
     if b and h and n:
         if cu_seqlens is not None:
-            cu_seqlens = _boundaries(cu_seqlens, n, dev)
+            cu_seqlens = _boundaries(cu_seqlens, n, cache.device)
         k, kf = _readable(k)
         v, vf = _readable(v)
         word = _Word(_KIND_APPEND, dev)
@@ -243,15 +258,14 @@ def cache_attention(q, cache, block_table, lengths, scale: float, sinks=None, we
     rows, is added, or written with `accumulate=False` (what `cache_evict` goes by).  With weights, no two sequences may name one page."""
     b, hq, n, _ = _activation("q", q)
     _no_gradients("flash_msa_cache_func", q, sinks)
-    fields, _ = _check_cache(cache, block_table, lengths, weights, b)
-    dev = cache.device
-    if q.device != dev:
+    fields, _, dev = _check_cache(cache, block_table, lengths, weights, b)
+    if q.get_device() != dev:
         raise ValueError("q and the cache must be on one CUDA device")
     hkv = fields[5]
     if hq == 0 or hq % hkv:
         raise ValueError("n_heads must be divisible by n_kv_heads")
-    logits = api._sink_logits(api._check_sinks(sinks, q))
-    api._require_cuda(cache)
+    logits = None if sinks is None else api._sink_logits(api._check_sinks(sinks, q))
+    _require_cuda(dev)
     out = q.new_empty((b, n, hq * HEAD_DIM))
     if b == 0 or n == 0:
         return out
@@ -276,17 +290,15 @@ def cache_evict(cache, weights, block_table, lengths, new_block_table, keep: int
     keep, recent = int(keep), int(recent)
     if weights is None:
         raise ValueError("weights must be a contiguous fp32 tensor [pages, KV heads, 128]")
-    fields, b = _check_cache(cache, block_table, lengths, weights)
-    dev = cache.device
-    stride = _check_table("new_block_table", new_block_table, dev)
-    if new_block_table.shape[0] != b:
+    fields, b, dev = _check_cache(cache, block_table, lengths, weights)
+    (rows, width), stride = _check_table("new_block_table", new_block_table, dev)
+    if rows != b:
         raise ValueError("new_block_table must have a row for every sequence")
     if keep < 1 or not 0 <= recent <= keep:
         raise ValueError("keep must be positive and recent between 0 and keep")
-    width = new_block_table.shape[1]
     if width * PAGE < keep:
         raise ValueError(f"new_block_table has room for {width * PAGE} tokens, keep is {keep}")
-    api._require_cuda(cache)
+    _require_cuda(dev)
     new_lengths, kept = lengths.new_empty(b), lengths.new_empty((b, fields[5], keep))
     if b:
         word = _Word(_KIND_EVICT, dev)
@@ -314,31 +326,31 @@ def prompt_attention(q, k, v, cu_seqlens, scale: float, sinks=None):
         raise NotImplementedError("at most 128 heads may share a KV head")
     if k.dtype is not q.dtype or v.dtype is not q.dtype:
         raise TypeError("q, k, and v must have one dtype")
-    dev = q.device
-    if k.device != dev or v.device != dev:
+    dev = q.get_device()
+    if k.get_device() != dev or v.get_device() != dev:
         raise ValueError("q, k, and v must be on one CUDA device")
     if not scale > 0:
         raise ValueError("scale must be positive")
     _no_gradients("flash_msa_prompt_func", q, k, v, sinks)
-    logits = api._sink_logits(api._check_sinks(sinks, q))
+    logits = None if sinks is None else api._sink_logits(api._check_sinks(sinks, q))
     n_seqs, per_batch = 1, 0
     if cu_seqlens is not None:
-        shape = tuple(torch.as_tensor(cu_seqlens).shape)
+        shape = tuple(cu_seqlens.shape if isinstance(cu_seqlens, torch.Tensor) else torch.as_tensor(cu_seqlens).shape)
         if len(shape) not in (1, 2) or shape[-1] < 2 or (len(shape) == 2 and shape[0] != b):
             raise ValueError("cu_seqlens must have shape [n+1] or [B, n+1]")
         n_seqs, per_batch = shape[-1] - 1, len(shape) - 1
-    api._require_cuda(q)
+    _require_cuda(dev)
     out = q.new_empty((b, s, hq * HEAD_DIM))
     if b == 0 or s == 0:
         return out
     lib = _lib.load()
     if cu_seqlens is not None:
-        cu_seqlens = _boundaries(cu_seqlens, s, dev)
+        cu_seqlens = _boundaries(cu_seqlens, s, q.device)
     q, qf = _tma_readable(q)
     k, kf = _tma_readable(k)
     v, vf = _tma_readable(v)
     nbytes = _size(dev, "fmsa_prompt_workspace_bytes", b, s, hq, hkv, n_seqs)
-    ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+    ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=q.device)
     word = _Word(_KIND_PROMPT, dev)
     _call("fmsa_prompt_fwd", _size(dev, "fmsa_prompt_launches", b, s, hq, hkv, n_seqs), lib.fmsa_prompt_fwd, _PROMPT_ARGS.pack(
         *qf, *kf, *vf, 0 if cu_seqlens is None else cu_seqlens.data_ptr(), 0 if logits is None else logits.data_ptr(), out.data_ptr(),
