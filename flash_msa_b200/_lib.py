@@ -125,6 +125,8 @@ def _declare(lib):
     lib.fmsa_cache_attend_workspace_bytes.argtypes = [c_int32, c_int32, c_int32, c_int32]
     lib.fmsa_prompt_workspace_bytes.restype = c_int64
     lib.fmsa_prompt_workspace_bytes.argtypes = [c_int32, c_int32, c_int32, c_int32, c_int32]
+    lib.fmsa_cache_attend_launches.restype = c_int32
+    lib.fmsa_cache_attend_launches.argtypes = [c_int32] * 6
     lib.fmsa_prompt_launches.restype = c_int32
     lib.fmsa_prompt_launches.argtypes = [c_int32, c_int32, c_int32, c_int32, c_int32]
     lib.fmsa_boundaries.restype = c_int

@@ -39,6 +39,7 @@ struct AttendParams {
     int32_t Hq, n, group, rows, blocks, fp16, accumulate, grid;   // group: heads per KV head; rows = group * n; blocks of 8 * NT rows
     float scale_log2e;
     uint32_t magic;             // 1024, 1024 in fp16
+    int32_t spread;             // CTAs of a cluster, a power of two
 };
 
 // Nibbles as fp16: bits 3..6 of a half are q * 2^-21 (a denormal), bits 7..10 q * 2^-17 (from 8 on a normal number, which goes on where
@@ -79,6 +80,7 @@ struct AttendTeam {
     Queries<NT> q[2];
     float4 part[4][3][NT][2][32];    // [channels of a group, warp number][other warp][][row 2t, 2t + 1][lane]: what they have of these channels
     float2 ml[4][8 * NT];            // [warp][row]: (reference, sum)
+    float2 total[8 * NT];            // [row]: the team's (in a cluster)
     uint64_t full[kParts], empty[kParts], q_full[2], q_empty[2];
     int32_t first, rest, length;     // sequence in which the range begins, units of it before, its length
 };
@@ -121,19 +123,28 @@ __device__ __forceinline__ void scales_of(uint2 w, float (&s)[4]) {   // four bf
 // need to be free of bank conflicts.
 __device__ __forceinline__ int token_of_row(int r) { return r ^ ((r >> 1) & 1); }
 
-// Prepares 8 query rows (number nt of a block); all lanes of a warp.
+// What prepare_queries() works on: 8 query rows (number nt of a block), loaded by all lanes of a warp, which may do something else meanwhile.
+struct RawQueries {
+    uint4 x[4];
+    int limit;
+    __device__ __forceinline__ void load(const AttendParams& P, int seq, int kv, int row, int lane) {   // row: the eight's first
+        row += lane >> 2;
+        const bool real = row < P.rows;
+        const int hh = real ? row / P.n : 0, j = real ? row - hh * P.n : 0;
+        const uint16_t* from = P.q + seq * P.qs[0] + (static_cast<int64_t>(kv) * P.group + hh) * P.qs[1] + j * P.qs[2] + 8 * (lane & 3);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = real ? __ldg(reinterpret_cast<const uint4*>(from + 32 * i)) : make_uint4(0, 0, 0, 0);
+        limit = real ? 1 - P.n + j : -0x40000000;
+    }
+};
 template <int NT>
-__device__ __forceinline__ void prepare_queries(Queries<NT>& to, const AttendParams& P, int seq, int kv, int block, int nt, int lane) {
-    const int g = lane >> 2, t = lane & 3, row = (block * NT + nt) * 8 + g;
+__device__ __forceinline__ void prepare_queries(Queries<NT>& to, const AttendParams& P, const RawQueries& raw, int nt, int lane) {
+    const int t = lane & 3;
     float f[4][8];
     uint32_t top = 0;
-    const bool real = row < P.rows;
-    const int hh = real ? row / P.n : 0, j = real ? row - hh * P.n : 0;
-    const uint16_t* from = P.q + seq * P.qs[0] + (static_cast<int64_t>(kv) * P.group + hh) * P.qs[1] + j * P.qs[2] + 8 * t;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint4 x = real ? __ldg(reinterpret_cast<const uint4*>(from + 32 * i)) : make_uint4(0, 0, 0, 0);
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        const uint32_t w[4] = {raw.x[i].x, raw.x[i].y, raw.x[i].z, raw.x[i].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             f[i][2 * e] = P.fp16 ? act_lo<true>(w[e]) : act_lo<false>(w[e]);
@@ -167,7 +178,7 @@ __device__ __forceinline__ void prepare_queries(Queries<NT>& to, const AttendPar
     const float m0 = __bfloat162float(__float2bfloat16_rn(c0 - h0)), m1 = __bfloat162float(__float2bfloat16_rn(c1 - h1));
     to.corr[nt][lane] = make_uint2(t < 2 ? pack_bf16(h0, h1) : pack_bf16(m0, m1), t < 2 ? pack_bf16(c0 - h0 - m0, c1 - h1 - m1) : 0u);
     const float fac = __uint_as_float(static_cast<uint32_t>(127 + 21 - up) << 23) * P.scale_log2e;
-    const int lim = real ? 1 - P.n + j : -0x40000000;
+    const int lim = raw.limit;
     to.factor[nt][lane] = make_float2(__shfl_sync(0xffffffffu, fac, 8 * t), __shfl_sync(0xffffffffu, fac, 8 * t + 4));
     to.limit[nt][lane] = make_int2(__shfl_sync(0xffffffffu, lim, 8 * t), __shfl_sync(0xffffffffu, lim, 8 * t + 4));
 }
@@ -244,7 +255,30 @@ __device__ __forceinline__ uint32_t less_eight_high(uint32_t x, uint32_t magic) 
     return half2_bits(__hfma2(*reinterpret_cast<const __half2*>(&y), __float2half2_rn(0.0625f), __float2half2_rn(-72.f)));
 }
 
-template <int NT>
+// Cluster barrier, by every thread of every CTA of the cluster.
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// Address in CTA `rank` of the cluster of what this CTA has at `addr`, and reads there.
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float2 ld_cluster_v2(uint32_t addr) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
+// CLUSTER: for few pairs of sequence and KV head and not too many pages: `spread` CTAs, a cluster, share a pair's pages, and its parts meet
+// in their shared memory: one launch, and nothing but the result is written.
+template <int NT, bool CLUSTER>
 __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(const AttendParams P) {
     extern __shared__ uint8_t smem_raw[];
     constexpr int kRows = 8 * NT, kT = kTeams<NT>, kThreads = kAttendThreads<NT>;
@@ -266,69 +300,82 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
     }
     wait_for_previous_kernel();
 
-    // ---- the line of pages, and the teams' ranges of it (a unit is a page of a (sequence, KV head, block of rows)); ranges are numbered
-    // team by team, so that few units go to as many SMs
-    const int seqs = P.cache.seqs, per = P.cache.heads * P.blocks, cta = blockIdx.x;
-    int units = 0;
-    Ranges R = {};
-    // Pages of up to kThreads sequences, from c0 on: what(sequence, its first page, its length, sum so far) for the thread's own; returns the sum.
-    auto scan = [&](int c0, int before, auto&& what) {
-        const int b = c0 + tid, length = b < seqs ? P.cache.length(b) : 0, p = (length + kPage - 1) / kPage;
-        int sum = p;
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += v;
-        }
-        if (lane == 31) sm->sums[warp] = sum;
-        __syncthreads();
-        const int w = lane < kThreads / 32 ? sm->sums[lane] : 0;
-        const int ahead = __reduce_add_sync(0xffffffffu, lane < warp ? w : 0), all = __reduce_add_sync(0xffffffffu, w);
-        what(b, before + ahead + sum - p, length, before + all);
-        __syncthreads();
-        return before + all;
-    };
-    auto divide = [&](int pages) {
-        units = pages * per;
-        R = Ranges(units, P.grid * kT);
-    };
-    auto claim = [&](int b, int at, int length) {
-        const int p = (length + kPage - 1) / kPage;
-        if (b < seqs && cta == 0) P.prefix[b] = at;
-#pragma unroll
-        for (int i = 0; i < kT; ++i) {
-            const int u = R.begin(i * P.grid + cta);
-            if (at * per <= u && u < (at + p) * per) {
-                sm->team[i].first = b;
-                sm->team[i].rest = u - at * per;
-                sm->team[i].length = length;
-            }
-        }
-    };
-    int pages_all = 0;
-    if (seqs <= kThreads) {
-        pages_all = scan(0, 0, [&](int b, int at, int length, int all) { divide(all); claim(b, at, length); });
-    } else {
-        for (int c0 = 0; c0 < seqs; c0 += kThreads) pages_all = scan(c0, pages_all, [](int, int, int, int) {});
-        divide(pages_all);
-        int before = 0;
-        for (int c0 = 0; c0 < seqs; c0 += kThreads) before = scan(c0, before, [&](int b, int at, int length, int) { claim(b, at, length); });
-    }
-    if (cta == 0 && tid == 0) P.prefix[seqs] = pages_all;
-    if (R.begin(cta) == units) return;   // (nothing for any team)
-
     const bool loads = warp >= 4 * kT;
     const int team = loads ? warp - 4 * kT : warp >> 2;
     AttendTeam<NT>* tm = &sm->team[min(team, kT - 1)];
     const uint32_t ring = base + team * kParts * kPartBytes;
-    const int range = team * P.grid + cta;
-    int left = team < kT ? R.begin(range + 1) - R.begin(range) : 0;
+    const int per = P.cache.heads * P.blocks, cta = blockIdx.x;
+    int units = 0, range = 0, left = 0;
     int seq = 0, length = 0, pages = 1, item = 0, page = 0;   // item: KV head * blocks + block of rows
-    if (left > 0) {
-        seq = tm->first;
-        length = tm->length;
+    Ranges R = {};
+    if constexpr (CLUSTER) {
+        __syncthreads();   // (the barriers are there)
+        const int pair = cta / P.spread;
+        seq = pair / per;
+        item = pair - seq * per;
+        length = P.cache.length(seq);
         pages = (length + kPage - 1) / kPage;
-        item = tm->rest / pages;
-        page = tm->rest - item * pages;
+        R = Ranges(pages, P.spread * kT);
+        range = team * P.spread + cta % P.spread;
+        page = R.begin(range);
+        left = team < kT ? R.begin(range + 1) - page : 0;
+    } else {
+        // ---- the line of pages, and the teams' ranges of it (a unit is a page of a (sequence, KV head, block of rows)); ranges are numbered
+        // team by team, so that few units go to as many SMs
+        const int seqs = P.cache.seqs;
+        // Pages of up to kThreads sequences, from c0 on: what(sequence, its first page, its length, sum so far) for the thread's own; returns the sum.
+        auto scan = [&](int c0, int before, auto&& what) {
+            const int b = c0 + tid, length = b < seqs ? P.cache.length(b) : 0, p = (length + kPage - 1) / kPage;
+            int sum = p;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += v;
+            }
+            if (lane == 31) sm->sums[warp] = sum;
+            __syncthreads();
+            const int w = lane < kThreads / 32 ? sm->sums[lane] : 0;
+            const int ahead = __reduce_add_sync(0xffffffffu, lane < warp ? w : 0), all = __reduce_add_sync(0xffffffffu, w);
+            what(b, before + ahead + sum - p, length, before + all);
+            __syncthreads();
+            return before + all;
+        };
+        auto divide = [&](int pages) {
+            units = pages * per;
+            R = Ranges(units, P.grid * kT);
+        };
+        auto claim = [&](int b, int at, int length) {
+            const int p = (length + kPage - 1) / kPage;
+            if (b < seqs && cta == 0) P.prefix[b] = at;
+#pragma unroll
+            for (int i = 0; i < kT; ++i) {
+                const int u = R.begin(i * P.grid + cta);
+                if (at * per <= u && u < (at + p) * per) {
+                    sm->team[i].first = b;
+                    sm->team[i].rest = u - at * per;
+                    sm->team[i].length = length;
+                }
+            }
+        };
+        int pages_all = 0;
+        if (seqs <= kThreads) {
+            pages_all = scan(0, 0, [&](int b, int at, int length, int all) { divide(all); claim(b, at, length); });
+        } else {
+            for (int c0 = 0; c0 < seqs; c0 += kThreads) pages_all = scan(c0, pages_all, [](int, int, int, int) {});
+            divide(pages_all);
+            int before = 0;
+            for (int c0 = 0; c0 < seqs; c0 += kThreads) before = scan(c0, before, [&](int b, int at, int length, int) { claim(b, at, length); });
+        }
+        if (cta == 0 && tid == 0) P.prefix[seqs] = pages_all;
+        if (R.begin(cta) == units) return;   // (nothing for any team)
+        range = team * P.grid + cta;
+        left = team < kT ? R.begin(range + 1) - R.begin(range) : 0;
+        if (left > 0) {
+            seq = tm->first;
+            length = tm->length;
+            pages = (length + kPage - 1) / kPage;
+            item = tm->rest / pages;
+            page = tm->rest - item * pages;
+        }
     }
     uint32_t part = 0, phase = 0, pieces = 0;    // ring position of the next page's K (V's is one further); pieces so far
     bool bad = false;
@@ -355,6 +402,8 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
         reg_dec<kRegsLoad<NT>>();
         while (left > 0) {
             const int take = min(left, pages - page), head = item / P.blocks;
+            RawQueries raw;   // (the first eight rows, on their way while the pages are found; the others of a block when they are needed)
+            raw.load(P, seq, head, (item - head * P.blocks) * kRows, lane);
             int id = -1;
             for (int i = 0; i < take; ++i) {
                 if ((i & 31) == 0) id = i + lane < take ? P.cache.page(seq, page + i + lane) : -1;
@@ -384,16 +433,24 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
                     const uint32_t slot = pieces & 1;
                     if (pieces >= 2) wait(BAR(tm->q_empty[slot]), (pieces / 2 - 1) & 1);
 #pragma unroll 1
-                    for (int nt = 0; nt < NT; ++nt) prepare_queries<NT>(tm->q[slot], P, seq, head, item % P.blocks, nt, lane);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        if (nt) raw.load(P, seq, head, (item - head * P.blocks) * kRows + 8 * nt, lane);
+                        prepare_queries<NT>(tm->q[slot], P, raw, nt, lane);
+                    }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(BAR(tm->q_full[slot]));
                 }
             }
             next(take);
         }
+        if (CLUSTER) {
+            cluster_sync();
+            cluster_sync();
+        }
     } else {
         // =========================== products ===========================
         reg_inc<kRegsMath<NT>>();
+        if (CLUSTER && left == 0 && (warp & 3) == 0 && lane < kRows) tm->total[lane] = make_float2(-INFINITY, 0.f);
         const int g = lane >> 2, t = lane & 3, mine = warp & 3, tile = mine * 32;
         const int tok_a = tile + token_of_row(g), tok_v0 = tile + token_of_row(2 * t), tok_v1 = tile + token_of_row(2 * t + 1);
         const uint32_t k_at = tok_a * 64 + t * 16, s_at = kPartScales + tok_a * 8;
@@ -571,8 +628,8 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
                         else tm->part[i][(mine - i + 3) & 3][nt][c][lane] = x;   // (warp i + 1 + y, modulo 4, is number y)
                     }
             named_barrier_sync(1 + team, 128);
-            const bool whole = page == 0 && take == pages;
-            if (page == 0 && mine == 0 && lane == 0) {   // (the part that begins a pair says where its parts are)
+            const bool whole = !CLUSTER && page == 0 && take == pages;
+            if (!CLUSTER && page == 0 && mine == 0 && lane == 0) {   // (the part that begins a pair says where its parts are)
                 const int behind = R.begin(range + 1) - left + pages;   // the unit behind the pair's last
                 P.parts[static_cast<int64_t>(seq) * per + item] = make_int2(2 * range + (pieces ? 1 : 0), whole ? 0 : R.owner(behind - 1) - range + 1);
             }
@@ -596,7 +653,10 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
                     }
                     if (row >= P.rows) continue;
                     const int ch = 32 * mine + 4 * g;
-                    if (whole) {
+                    if (CLUSTER) {   // (where the team's pages were: all of them have been read)
+                        *reinterpret_cast<float4*>(smem_raw + (ring - smem_u32(smem_raw)) + (r * kHeadDim + ch) * 4) = acc;
+                        if (ch == 0) tm->total[r] = make_float2(top, l);
+                    } else if (whole) {
                         const int hh = row / P.n, j = row - hh * P.n, h = head * P.group + hh;
                         if (P.sinks) l += fast_exp2(P.sinks[h] * kLog2e - m);
                         const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -613,6 +673,47 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
                 }
             named_barrier_sync(1 + team, 128);
             next(take);
+        }
+        if (CLUSTER) {
+            cluster_sync();
+            const int head = item / P.blocks, block = item - head * P.blocks, parts = P.spread * kT;   // at most 32; team p / spread of CTA p % spread
+            const int shift = __ffs(P.spread) - 1, low = P.spread - 1;
+            const uint32_t all_rings = base, totals = smem_u32(sm->team[0].total);
+            for (int r = (cta & low) + (warp << shift); r < kRows; r += (4 * kT) << shift) {
+                const int row = block * kRows + r;
+                if (row >= P.rows) break;
+                float2 ml = make_float2(-INFINITY, 0.f);
+                if (lane < parts) ml = ld_cluster_v2(in_cta(totals + (lane >> shift) * static_cast<int>(sizeof(AttendTeam<NT>)) + r * 8, lane & low));
+                float top = ml.x;
+                for (int o2 = 16; o2; o2 >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o2));
+                const float m = top == -INFINITY ? 0.f : top, by = fast_exp2(ml.x - m);
+                float l = ml.y * by;
+                for (int o2 = 16; o2; o2 >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o2);
+                float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (uint32_t live = __ballot_sync(0xffffffffu, by != 0.f); live;) {   // the parts that have something, eight reads at once
+                    float f[8];
+                    float4 x[8];
+#pragma unroll
+                    for (int y = 0; y < 8; ++y) {
+                        const int p = live ? __ffs(live) - 1 : 0;
+                        f[y] = __shfl_sync(0xffffffffu, by, p);
+                        x[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (live) x[y] = ld_cluster_v4(in_cta(all_rings + (p >> shift) * (kParts * kPartBytes) + (r * kHeadDim + 4 * lane) * 4, p & low));
+                        else f[y] = 0.f;
+                        live &= live - 1;
+                    }
+#pragma unroll
+                    for (int y = 0; y < 8; ++y) acc = make_float4(fmaf(x[y].x, f[y], acc.x), fmaf(x[y].y, f[y], acc.y), fmaf(x[y].z, f[y], acc.z), fmaf(x[y].w, f[y], acc.w));
+                }
+                const int hh = row / P.n, j = row - hh * P.n, h = head * P.group + hh;
+                if (P.sinks) l += fast_exp2(P.sinks[h] * kLog2e - m);
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                uint2 y;
+                y.x = P.fp16 ? pack_act<true>(acc.x * inv, acc.y * inv) : pack_act<false>(acc.x * inv, acc.y * inv);
+                y.y = P.fp16 ? pack_act<true>(acc.z * inv, acc.w * inv) : pack_act<false>(acc.z * inv, acc.w * inv);
+                *reinterpret_cast<uint2*>(P.out + ((static_cast<int64_t>(seq) * P.n + j) * P.Hq + h) * kHeadDim + 4 * lane) = y;
+            }
+            cluster_sync();   // (no CTA leaves while another one reads from it)
         }
     }
     if (bad) {
@@ -736,7 +837,9 @@ __global__ void __launch_bounds__(kWeightWarps * 32, 2) cache_weights_kernel(con
                 const int n = min(held, P.blocks - lot);
                 __syncthreads();
                 for (int i = warp; i < n * NT; i += kWeightWarps) {
-                    prepare_queries<NT>(rows[i / NT].q, P, seq, head, lot + i / NT, i % NT, lane);
+                    RawQueries raw;
+                    raw.load(P, seq, head, (lot * NT + i) * 8, lane);
+                    prepare_queries<NT>(rows[i / NT].q, P, raw, i % NT, lane);
                     const int row = (lot * NT + i) * 8 + 2 * t;
                     const float* lse = P.lse + (static_cast<int64_t>(seq) * heads + head) * (P.blocks * NT * 8) + row;
                     rows[i / NT].lse[i % NT][lane] = make_float2(row < P.rows ? lse[0] : 0.f, row + 1 < P.rows ? lse[1] : 0.f);
@@ -826,11 +929,31 @@ AttendSpace carve_attend(int seqs, int Hq, int heads, int n, int grid) {
 
 constexpr int kWeightBlocks = 7;   // blocks of rows whose queries the weights kernel holds at once: 44 KB
 static_assert(kWeightBlocks * sizeof(WeightRows<2>) <= 48 * 1024, "more needs an attribute");
+// CTAs that share a pair of sequence and KV head (and block of rows) in a cluster, or 0. A power of two up to 8 that fits the GPU, where a
+// team's pages at the longest lengths the table can hold are at most one more than with all SMs' teams on all pages.  (The weights need
+// what the other form leaves in the workspace.)
+int cluster_spread(const fmsa_cache4& c, int64_t rows, bool weights, int sms) {
+    const int nt = tiles_for(rows), teams = nt == 1 ? kTeams<1> : kTeams<2>;
+    const int64_t pairs = static_cast<int64_t>(c.seqs) * c.heads * ((rows + 8 * nt - 1) / (8 * nt));
+    if (weights || pairs * 2 > sms) return 0;
+    int spread = 2;
+    while (spread < 8 && pairs * spread * 2 <= sms) spread *= 2;
+    auto rounds = [&](int64_t pages, int64_t by) { return (pages + by - 1) / by; };
+    return rounds(c.width, spread * teams) <= rounds(pairs * c.width, static_cast<int64_t>(sms) * teams) + 1 ? spread : 0;
+}
+
 template <int NT>
 int launch_attend(const AttendParams& P, cudaStream_t st) {
     const int sms = device_sm_count();
-    if (!ensure_smem_attr(reinterpret_cast<const void*>(cache_attend_kernel<NT>), kAttendSmem<NT>)) return FMSA_ERR_CUDA;
-    launch_chained(cache_attend_kernel<NT>, P.grid, kAttendThreads<NT>, kAttendSmem<NT>, st, P);
+    if (P.spread) {
+        const auto kernel = cache_attend_kernel<NT, true>;
+        if (!ensure_smem_attr(reinterpret_cast<const void*>(kernel), kAttendSmem<NT>)) return FMSA_ERR_CUDA;
+        launch_clusters(kernel, P.cache.seqs * P.cache.heads * P.blocks * P.spread, P.spread, kAttendThreads<NT>, kAttendSmem<NT>, st, P);
+        return check_launch();
+    }
+    const auto kernel = cache_attend_kernel<NT, false>;
+    if (!ensure_smem_attr(reinterpret_cast<const void*>(kernel), kAttendSmem<NT>)) return FMSA_ERR_CUDA;
+    launch_chained(kernel, P.grid, kAttendThreads<NT>, kAttendSmem<NT>, st, P);
     // A pair is cut into about ranges / pairs parts (+ 1): 16 warps a row where that is many.
     const int64_t pairs = static_cast<int64_t>(P.cache.seqs) * P.cache.heads * P.blocks;
     const int rows = P.rows < 8 * NT ? P.rows : 8 * NT;
@@ -851,6 +974,15 @@ extern "C" int64_t fmsa_cache_attend_workspace_bytes(int32_t seqs, int32_t Hq, i
     const int sms = device_sm_count();
     if (seqs <= 0 || heads <= 0 || Hq <= 0 || Hq % heads || n <= 0 || sms <= 0) return -1;
     return carve_attend(seqs, Hq, heads, n, sms).bytes;
+}
+
+extern "C" int32_t fmsa_cache_attend_launches(int32_t seqs, int32_t Hq, int32_t heads, int32_t n, int32_t width, int32_t weights) {
+    using namespace fmsa;
+    const int sms = device_sm_count();
+    if (seqs <= 0 || heads <= 0 || Hq <= 0 || Hq % heads || n <= 0 || width <= 0 || sms <= 0) return -1;
+    fmsa_cache4 c = {};
+    c.seqs = seqs; c.heads = heads; c.width = width;
+    return weights ? 3 : cluster_spread(c, static_cast<int64_t>(Hq / heads) * n, false, sms) ? 1 : 2;
 }
 
 extern "C" int fmsa_cache_attend(const fmsa_cache_attend_args* args, void* stream) {
@@ -891,6 +1023,7 @@ extern "C" int fmsa_cache_attend(const fmsa_cache_attend_args* args, void* strea
     P.fp16 = dtype == FMSA_DTYPE_FP16; P.accumulate = args->accumulate ? 1 : 0;
     P.scale_log2e = args->scale * kLog2e;
     P.magic = 0x64006400u;
+    P.spread = cluster_spread(*cache, rows, args->weights != nullptr, sms);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     return nt == 1 ? launch_attend<1>(P, st) : launch_attend<2>(P, st);
 }

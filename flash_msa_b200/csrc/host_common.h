@@ -36,6 +36,25 @@ inline void launch_chained(void (*kernel)(Params...), dim3 grid, dim3 block, siz
     cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);   // (check_launch reports what goes wrong)
 }
 
+// The same in clusters of `cluster` blocks.
+template <class... Params, class... Args>
+inline void launch_clusters(void (*kernel)(Params...), dim3 grid, unsigned cluster, dim3 block, size_t smem, cudaStream_t stream, Args&&... args) {
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Head-count relations every entry point relies on (the reference checks the same ones in

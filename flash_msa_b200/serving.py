@@ -274,7 +274,8 @@ def cache_attention(q, cache, block_table, lengths, scale: float, sinks=None, we
     q, qf = _readable(q)
     ws = cache.new_empty(max(nbytes, 1))
     word = _Word(_KIND_ATTEND, dev)
-    _call("fmsa_cache_attend", 2 if weights is None else 3, lib.fmsa_cache_attend, _ATTEND_ARGS.pack(
+    launches = _size(dev, "fmsa_cache_attend_launches", b, hq, hkv, n, fields[7], 0 if weights is None else 1)
+    _call("fmsa_cache_attend", launches, lib.fmsa_cache_attend, _ATTEND_ARGS.pack(
         *fields, *qf, 0 if logits is None else logits.data_ptr(), 0 if weights is None else weights.data_ptr(), out.data_ptr(), ws.data_ptr(),
         nbytes, word.ptr, hq, n, ops._dtype_code(q.dtype), 1 if accumulate else 0, scale, 0), dev)
     word.check()

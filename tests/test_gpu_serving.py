@@ -242,7 +242,29 @@ def test_attention_weights(fm, hq, hkv, n, lengths, sinks, accumulate):
     w = torch.rand(cache.shape[0], hkv, 128, generator=g, device="cuda")
     s = torch.randn(hq, generator=g, device="cuda") if sinks else None
     out = check_attend(fm, cache, table, ls, lengths, q, s, w, accumulate)
-    assert torch.equal(out, fm.flash_msa_cache_func(q, cache, table, ls, SCALE, sinks=s))
+    again = w.clone()
+    assert torch.equal(out, check_attend(fm, cache, table, ls, lengths, q, s, again, accumulate))
+    if not accumulate:
+        assert torch.equal(again, w)
+    check_attend(fm, cache, table, ls, lengths, q, s)     # (a call without weights may sum in another order)
+
+
+@pytest.mark.parametrize("hq,hkv,n,b,width", [(8, 2, 1, 1, 1), (8, 2, 1, 1, 9), (4, 4, 1, 4, 40), (12, 1, 2, 2, 64), (16, 8, 1, 9, 5), (8, 1, 1, 74, 3), (8, 1, 1, 75, 3),
+                                              (4, 4, 1, 40, 70), (24, 1, 1, 1, 300), (2, 1, 1, 700, 2)])
+def test_attention_at_every_number_of_launches(fm, hq, hkv, n, b, width):
+    """Few pairs of sequence and KV head go to clusters of 8, 4 or 2 blocks, the others to ranges that cut them: lengths up to what the table
+    holds, empty ones, and ones of which most blocks have nothing; and more sequences than a block has threads."""
+    from flash_msa_b200 import _lib
+    r = torch.Generator().manual_seed(b + width)
+    lengths = torch.randint(0, 128 * width + 1, (b,), generator=r).tolist()
+    lengths[0] = 128 * width
+    if b > 2:
+        lengths[1], lengths[2] = 0, 1
+    cache, table, ls, g = pool(fm, lengths, hkv, seed=b)
+    q = torch.randn(b, hq, n, 128, generator=g, device="cuda").to(torch.bfloat16)
+    check_attend(fm, cache, table, ls, lengths, q, torch.randn(hq, device="cuda"))
+    launches = _lib.load().fmsa_cache_attend_launches(b, hq, hkv, n, width, 0)
+    assert launches == (1 if (b, width) in ((1, 1), (1, 9), (4, 40), (9, 5), (74, 3)) else 2)
 
 
 def test_attention_repeats_and_follows_streams(fm):
