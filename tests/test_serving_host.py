@@ -97,6 +97,26 @@ def test_refusals(what, change, error):
         _call(what, **change)
 
 
+@pytest.mark.parametrize("what", ["append", "attend", "prompt"])
+def test_derivatives_and_traces_are_refused(what):
+    name = {"append": "k", "attend": "q", "prompt": "pq"}[what]
+    shape = (2, 4, 7, 128) if what == "prompt" else (3, 4, 1, 128) if what == "attend" else (3, 2, 1, 128)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(z(*shape), z(*shape))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            _call(what, **{name: dual})
+        with pytest.raises(RuntimeError, match="CUDA"):      # (a level without a tangent is not in the way)
+            _call(what)
+
+    def traced(t):
+        _call(what, **{name: t})
+        return t
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(traced, (z(*shape),))
+    with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+        _call(what, **{name: z(*shape).requires_grad_()})
+
+
 @pytest.mark.parametrize("cu", [[0, 3, 2], [1, 3], [0, 9], [0], [[[0, 1]]]])
 def test_boundaries_that_are_refused(cu):
     with pytest.raises(ValueError):
@@ -125,7 +145,7 @@ CACHE = (16, 16, 16, 2, 4, 2, 3, 2)
 ENTRIES = {"append": "fmsa_cache_append", "attend": "fmsa_cache_attend", "evict": "fmsa_cache_evict", "prompt": "fmsa_prompt_fwd"}
 C_REFUSALS = [
     ("append", dict(b=2), -1), ("append", dict(dtype=7), -1), ("append", dict(values=(16, 256, 128, 128, 0, 0, 0, 0)), -1), ("append", dict(k=ODD), -1),
-    ("append", dict(v=(0, 256, 128, 128)), -1), ("append", dict(v=(16, 256, 128, 12)), -1), ("append", dict(n=1 << 30), -2), ("append", dict(n=0), -1),
+    ("append", dict(v=(0, 256, 128, 128)), -1), ("append", dict(v=(16, 256, 128, 12)), -1), ("append", dict(n=1 << 30), -2), ("append", dict(cache=(16, 16, 16, 2, 1 << 23, 2, 3, 2)), -2), ("append", dict(n=0), -1),
     ("append", dict(status=0), -1), ("append", dict(cu=16), -1),
     ("attend", dict(hq=5), -1), ("attend", dict(q=ODD), -1), ("attend", dict(dtype=-1), -1), ("attend", dict(out=0), -1), ("attend", dict(ws=0), -1),
     ("evict", dict(keep=129, recent=0), -1), ("evict", dict(recent=101), -1), ("evict", dict(keep=0, recent=0), -1), ("evict", dict(weights=0), -1),
