@@ -197,7 +197,7 @@ def cache_append(cache, k, v, block_table, lengths, cu_seqlens=None, weights=Non
     """Stores new keys and values (B,Hkv,n,128) in the cache; `lengths` count them already.  Without `cu_seqlens` batch element i holds the
     last n tokens of sequence i (rows for which lengths[i] < n leaves no place are skipped: an empty place of a padded batch has length
     0).  With `cu_seqlens` ([sequences+1], as in `flash_msa_varlen_func`, but it may end before n) k and v have one batch element, and its
-    rows cu_seqlens[i] .. cu_seqlens[i+1]-1 are the last tokens of sequence i.
+    rows cu_seqlens[i] .. cu_seqlens[i+1]-1 are the last tokens of sequence i.  No two sequences may name a page that either appends to.
     `weights`: fp32 [pages, Hkv, 128] as `cache_attention` collects them; those of the stored tokens become zero.  Returns None, or with
     `return_values` (k, v) as the cache now holds them, in the inputs' type: what a prompt's own attention reads if it is to agree with
     the steps that follow (zeros for skipped rows).
@@ -208,7 +208,7 @@ def cache_append(cache, k, v, block_table, lengths, cu_seqlens=None, weights=Non
         raise ValueError("k and v must agree, and have the cache's KV heads")
     if v.dtype is not k.dtype:
         raise TypeError("k and v must have one dtype")
-    _no_gradients("flash_msa_cache_append", k, v)
+    _no_gradients("flash_msa_cache_append", k, v, weights)
     b, h, n, _ = shape
     fields, seqs, dev = _check_cache(cache, block_table, lengths, weights)
     if h != fields[5]:
@@ -223,15 +223,15 @@ def cache_append(cache, k, v, block_table, lengths, cu_seqlens=None, weights=Non
     elif tuple(cu_seqlens.shape if isinstance(cu_seqlens, torch.Tensor) else torch.as_tensor(cu_seqlens).shape) != (seqs + 1,):
         raise ValueError("cu_seqlens must hold one boundary more than block_table has rows")
     _require_cuda(dev)
+    k, kf = _readable(k)
+    v, vf = _readable(v)
     values, to = None, _NO_TENSOR + _NO_TENSOR
-    if return_values:
-        values = (ops._grad_like(k), ops._grad_like(v))
-        to = tuple(x for t in values for x in (t.data_ptr(), *t.stride()[:3]))
+    if return_values:   # (in the inputs' layout; what is readable has its channels innermost and strides of multiples of 8, and so have these)
+        ko, vo = values = torch.empty_like(k), torch.empty_like(v)
+        to = (ko.data_ptr(), *ko.stride()[:3], vo.data_ptr(), *vo.stride()[:3])
     if b and h and n:
         if cu_seqlens is not None:
             cu_seqlens = _boundaries(cu_seqlens, n, cache.device)
-        k, kf = _readable(k)
-        v, vf = _readable(v)
         word = _Word(_KIND_APPEND, dev)
         _call("fmsa_cache_append", 1, _lib.load().fmsa_cache_append, _APPEND_ARGS.pack(
             *fields, *kf, *vf, *to, 0 if cu_seqlens is None else cu_seqlens.data_ptr(), 0 if weights is None else weights.data_ptr(), word.ptr,
@@ -260,7 +260,7 @@ def cache_attention(q, cache, block_table, lengths, scale: float, sinks=None, we
     `flash_msa_func`.  `weights`: fp32 [pages, Hkv, 128]: the probability every token got from this call, summed over its KV head's query
     rows, is added, or written with `accumulate=False` (what `cache_evict` goes by).  With weights, no two sequences may name one page."""
     b, hq, n, _ = _activation("q", q)
-    _no_gradients("flash_msa_cache_func", q, sinks)
+    _no_gradients("flash_msa_cache_func", q, sinks, weights)
     fields, _, dev = _check_cache(cache, block_table, lengths, weights, b)
     if q.get_device() != dev:
         raise ValueError("q and the cache must be on one CUDA device")
@@ -294,6 +294,7 @@ def cache_evict(cache, weights, block_table, lengths, new_block_table, keep: int
     keep, recent = int(keep), int(recent)
     if weights is None:
         raise ValueError("weights must be a contiguous fp32 tensor [pages, KV heads, 128]")
+    _no_gradients("flash_msa_cache_evict", weights)
     fields, b, dev = _check_cache(cache, block_table, lengths, weights)
     (rows, width), stride = _check_table("new_block_table", new_block_table, dev)
     if rows != b:

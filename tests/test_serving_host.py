@@ -117,6 +117,15 @@ def test_derivatives_and_traces_are_refused(what):
         _call(what, **{name: z(*shape).requires_grad_()})
 
 
+@pytest.mark.parametrize("what", ["append", "attend", "evict"])
+def test_weights_that_want_a_gradient_are_refused(what):
+    weights = torch.zeros(4, 2, 128, requires_grad=True)     # (the calls write them in place)
+    with pytest.raises(RuntimeError, match="no backward"):
+        _call(what, weights=weights)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+        _call(what, weights=weights)
+
+
 @pytest.mark.parametrize("cu", [[0, 3, 2], [1, 3], [0, 9], [0], [[[0, 1]]]])
 def test_boundaries_that_are_refused(cu):
     with pytest.raises(ValueError):
