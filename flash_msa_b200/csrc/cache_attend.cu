@@ -22,37 +22,12 @@
 // B=32 Hq=32 Hkv=8, lengths to 8192 (158 MB): 38.4 us and 4.5 us for what was cut, 3.7 TB/s; without its products the first kernel takes
 // 32 us (6 us of them before the first page and behind the last), whatever the depth of the ring.  A tile of 16 tokens takes 300
 // instructions; at first, with one ring for 16 warps and the products' offsets as start values in registers, 505, and 66 + 10 us.
-#include "cache4.cuh"
+#include "cache_attend.cuh"
 #include "host_common.h"
 #include "sm100.cuh"
 
 namespace fmsa {
 namespace {
-
-struct AttendParams {
-    Cache4 cache;
-    const uint16_t* q;          // (seqs,Hq,n,128)
-    int64_t qs[3];
-    const float* sinks;         // [Hq] or null
-    uint16_t* out;              // [seqs][n][Hq*128]
-    float* weights;             // [pages][heads][128] or null
-    int32_t* prefix;            // [seqs + 1]: pages of the sequences before
-    int2* parts;                // [seqs][heads][blocks]: first slot of a pair that is cut and the number of its parts; 0 parts: not cut
-    float* o_part;              // [2 * ranges][rows of a block][128]
-    float2* ml_part;            // [2 * ranges][rows of a block]: (reference, sum), log2 domain
-    float* lse;                 // [seqs][heads][blocks * rows of a block], log2 domain
-    int32_t Hq, n, group, rows, blocks, fp16, accumulate, grid;   // group: heads per KV head; rows = group * n; blocks of 8 * NT rows
-    float scale_log2e;
-    uint32_t magic;             // 1024, 1024 in fp16
-    int32_t spread;             // CTAs of a cluster, a power of two
-};
-
-// Nibbles as fp16: bits 3..6 of a half are q * 2^-21 (a denormal), bits 7..10 q * 2^-17 (from 8 on a normal number, which goes on where
-// the denormals end).  Not lower in the half: the tensor core aligns its sums by the operands' exponent fields, so every leading zero of a
-// denormal costs a bit of the sum.  (With K and V at bits 0..3 and 4..7 a row over 900 tokens was 1.7 times further from 64 bits' than the
-// other roundings allow for.)
-constexpr uint32_t kLow = 0x00780078u, kHigh = 0x07800780u;
-constexpr float kUnitLow = 1.f / (1 << 21);
 
 template <bool V> struct Bool { static constexpr bool value = V; };
 
@@ -114,10 +89,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
-                 : "memory");
-}
 __device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ void scales_of(uint2 w, float (&s)[4]) {   // four bf16
     s[0] = __uint_as_float(w.x << 16);
@@ -129,20 +100,6 @@ __device__ __forceinline__ void scales_of(uint2 w, float (&s)[4]) {   // four bf
 // need to be free of bank conflicts.
 __device__ __forceinline__ int token_of_row(int r) { return r ^ ((r >> 1) & 1); }
 
-// What prepare_queries() works on: 8 query rows (number nt of a block), loaded by all lanes of a warp, which may do something else meanwhile.
-struct RawQueries {
-    uint4 x[4];
-    int limit;
-    __device__ __forceinline__ void load(const AttendParams& P, int seq, int kv, int row, int lane) {   // row: the eight's first
-        row += lane >> 2;
-        const bool real = row < P.rows;
-        const int hh = real ? row / P.n : 0, j = real ? row - hh * P.n : 0;
-        const uint16_t* from = P.q + seq * P.qs[0] + (static_cast<int64_t>(kv) * P.group + hh) * P.qs[1] + j * P.qs[2] + 8 * (lane & 3);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = real ? __ldg(reinterpret_cast<const uint4*>(from + 32 * i)) : make_uint4(0, 0, 0, 0);
-        limit = real ? 1 - P.n + j : -0x40000000;
-    }
-};
 template <int NT>
 __device__ __forceinline__ void prepare_queries(Queries<NT>& to, const AttendParams& P, const RawQueries& raw, int nt, int lane) {
     const int t = lane & 3;
@@ -226,32 +183,9 @@ __device__ __forceinline__ void logits(float (&s)[J][NT][4], const uint4 (&k)[J]
     }
 }
 
-// `units` pages in at most `most` ranges, the first ones one page longer: unit begin(r) is the first of range r (or `units` behind the last).
-struct Ranges {
-    int units, size, longer, n;
-    __device__ Ranges() {}
-    __device__ __forceinline__ Ranges(int all, int most) : units(all), n(min(all, most)) {
-        size = n ? all / n : 0;
-        longer = all - size * n;
-    }
-    __device__ __forceinline__ int begin(int r) const { return r < n ? size * r + min(r, longer) : units; }
-    __device__ __forceinline__ int owner(int u) const {
-        const int split = longer * (size + 1);
-        return u < split ? u / (size + 1) : longer + (u - split) / size;
-    }
-};
-
-// Logits (log2 domain) that a tile keeps below 2^kSlack times the reference before the reference is raised, and how far below the largest
-// (logit + log2 scale) the reference is set: fp16 holds p * s up to 2^(kSlack + kLift) and, at full precision, down to 2^-14.
-constexpr float kSlack = 8.f, kLift = 6.f;
 // Code q - 8 of nibbles 0 and 4 (bits 0..3 of each half) as fp16, and of nibbles 1 and 5 (bits 4..7): 1024 + q and 1024 + 16 q are what the
 // nibble gives under the exponent bits of `magic` (0x64006400: not a constant here, so that it stays in a register and both logical
 // operations are one instruction).
-__device__ __forceinline__ uint32_t masked_or(uint32_t x, uint32_t mask, uint32_t or_with) {
-    uint32_t y;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(or_with));
-    return y;
-}
 __device__ __forceinline__ uint32_t less_eight(uint32_t x, uint32_t magic) {
     const uint32_t y = masked_or(x, 0x000f000fu, magic);
     return half2_bits(__hadd2(*reinterpret_cast<const __half2*>(&y), __float2half2_rn(-1032.f)));
@@ -670,7 +604,7 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
                         y.x = P.fp16 ? pack_act<true>(acc.x * inv, acc.y * inv) : pack_act<false>(acc.x * inv, acc.y * inv);
                         y.y = P.fp16 ? pack_act<true>(acc.z * inv, acc.w * inv) : pack_act<false>(acc.z * inv, acc.w * inv);
                         *reinterpret_cast<uint2*>(P.out + ((static_cast<int64_t>(seq) * P.n + j) * P.Hq + h) * kHeadDim + ch) = y;
-                        if (ch == 0) P.lse[(static_cast<int64_t>(seq) * P.cache.heads + head) * (P.blocks * kRows) + row] = m + fast_log2(l);
+                        if (ch == 0) P.lse[(static_cast<int64_t>(seq) * P.cache.heads + head) * P.lse_rows + row] = m + fast_log2(l);
                     } else {
                         const int64_t slot = 2LL * range + (pieces ? 1 : 0);
                         *reinterpret_cast<float4*>(P.o_part + (slot * kRows + r) * kHeadDim + ch) = acc;
@@ -805,7 +739,7 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS) cache_combine_k
     y.x = P.fp16 ? pack_act<true>(acc.x * inv, acc.y * inv) : pack_act<false>(acc.x * inv, acc.y * inv);
     y.y = P.fp16 ? pack_act<true>(acc.z * inv, acc.w * inv) : pack_act<false>(acc.z * inv, acc.w * inv);
     *reinterpret_cast<uint2*>(P.out + ((static_cast<int64_t>(seq) * P.n + j) * P.Hq + h) * kHeadDim + 4 * lane) = y;
-    if (lane == 0) P.lse[(static_cast<int64_t>(seq) * P.cache.heads + head) * (P.blocks * kRows) + row] = m + fast_log2(l);
+    if (lane == 0) P.lse[(static_cast<int64_t>(seq) * P.cache.heads + head) * P.lse_rows + row] = m + fast_log2(l);
 }
 
 // The probabilities of every token, summed over the query rows of its KV head: the logits once more (half of the cache's bytes, most of
@@ -847,7 +781,7 @@ __global__ void __launch_bounds__(kWeightWarps * 32, 2) cache_weights_kernel(con
                     raw.load(P, seq, head, (lot * NT + i) * 8, lane);
                     prepare_queries<NT>(rows[i / NT].q, P, raw, i % NT, lane);
                     const int row = (lot * NT + i) * 8 + 2 * t;
-                    const float* lse = P.lse + (static_cast<int64_t>(seq) * heads + head) * (P.blocks * NT * 8) + row;
+                    const float* lse = P.lse + (static_cast<int64_t>(seq) * heads + head) * P.lse_rows + row;
                     rows[i / NT].lse[i % NT][lane] = make_float2(row < P.rows ? lse[0] : 0.f, row + 1 < P.rows ? lse[1] : 0.f);
                 }
                 __syncthreads();
@@ -913,7 +847,8 @@ __global__ void __launch_bounds__(kWeightWarps * 32, 2) cache_weights_kernel(con
 struct AttendSpace {
     int64_t prefix, parts, o_part, ml_part, lse, bytes;
 };
-int tiles_for(int64_t rows) { return rows <= 8 ? 1 : 2; }
+int tiles_for(int64_t rows) { return rows <= 8 ? 1 : rows < kRowsMin ? 2 : rows_of_block(rows) / 8; }   // eights of rows of a block
+int teams_for(int tiles) { return tiles == 1 ? kTeams<1> : tiles == 2 ? kTeams<2> : 1; }              // ranges of a CTA
 AttendSpace carve_attend(int seqs, int Hq, int heads, int n, int grid) {
     const int64_t rows = static_cast<int64_t>(Hq / heads) * n, block = 8 * tiles_for(rows);
     AttendSpace w;
@@ -925,7 +860,7 @@ AttendSpace carve_attend(int seqs, int Hq, int heads, int n, int grid) {
     };
     w.prefix = take(4LL * (seqs + 1));
     w.parts = take(8LL * seqs * heads * (round_up(rows, block) / block));
-    const int64_t ranges = static_cast<int64_t>(grid) * (block == 8 ? kTeams<1> : kTeams<2>);
+    const int64_t ranges = static_cast<int64_t>(grid) * teams_for(tiles_for(rows));
     w.o_part = take(2 * ranges * block * kHeadDim * 4);
     w.ml_part = take(2 * ranges * block * 8);
     w.lse = take(4LL * seqs * heads * round_up(rows, block));
@@ -939,9 +874,9 @@ static_assert(kWeightBlocks * sizeof(WeightRows<2>) <= 48 * 1024, "more needs an
 // team's pages at the longest lengths the table can hold are at most one more than with all SMs' teams on all pages.  (The weights need
 // what the other form leaves in the workspace.)
 int cluster_spread(const fmsa_cache4& c, int64_t rows, bool weights, int sms) {
-    const int nt = tiles_for(rows), teams = nt == 1 ? kTeams<1> : kTeams<2>;
+    const int nt = tiles_for(rows), teams = teams_for(nt);
     const int64_t pairs = static_cast<int64_t>(c.seqs) * c.heads * ((rows + 8 * nt - 1) / (8 * nt));
-    if (weights || pairs * 2 > sms) return 0;
+    if (weights || nt > 2 || pairs * 2 > sms) return 0;
     int spread = 2;
     while (spread < 8 && pairs * spread * 2 <= sms) spread *= 2;
     auto rounds = [&](int64_t pages, int64_t by) { return (pages + by - 1) / by; };
@@ -949,25 +884,56 @@ int cluster_spread(const fmsa_cache4& c, int64_t rows, bool weights, int sms) {
 }
 
 template <int NT>
-int launch_attend(const AttendParams& P, cudaStream_t st) {
-    const int sms = device_sm_count();
+bool launch_attend(const AttendParams& P, cudaStream_t st) {
     if (P.spread) {
         const auto kernel = cache_attend_kernel<NT, true>;
-        if (!ensure_smem_attr(reinterpret_cast<const void*>(kernel), kAttendSmem<NT>)) return FMSA_ERR_CUDA;
+        if (!ensure_smem_attr(reinterpret_cast<const void*>(kernel), kAttendSmem<NT>)) return false;
         launch_clusters(kernel, P.cache.seqs * P.cache.heads * P.blocks * P.spread, P.spread, kAttendThreads<NT>, kAttendSmem<NT>, st, P);
-        return check_launch();
+        return true;
     }
     const auto kernel = cache_attend_kernel<NT, false>;
-    if (!ensure_smem_attr(reinterpret_cast<const void*>(kernel), kAttendSmem<NT>)) return FMSA_ERR_CUDA;
+    if (!ensure_smem_attr(reinterpret_cast<const void*>(kernel), kAttendSmem<NT>)) return false;
     launch_chained(kernel, P.grid, kAttendThreads<NT>, kAttendSmem<NT>, st, P);
+    return true;
+}
+// Everything behind the first kernel.
+template <int NT>
+void launch_combine(const AttendParams& P, cudaStream_t st) {
     // A pair is cut into about ranges / pairs parts (+ 1): 16 warps a row where that is many.
     const int64_t pairs = static_cast<int64_t>(P.cache.seqs) * P.cache.heads * P.blocks;
     const int rows = P.rows < 8 * NT ? P.rows : 8 * NT;
-    if (pairs * 16 < P.grid * kTeams<NT>) launch_chained(cache_combine_kernel<NT, 16>, dim3(static_cast<unsigned>(pairs), rows), 512, 0, st, P);
+    if (pairs * 16 < P.grid * teams_for(NT)) launch_chained(cache_combine_kernel<NT, 16>, dim3(static_cast<unsigned>(pairs), rows), 512, 0, st, P);
     else launch_chained(cache_combine_kernel<NT, 1>, dim3(static_cast<unsigned>(pairs), (rows + 3) / 4), 128, 0, st, P);
+}
+template <int NT>
+void launch_weights(const AttendParams& P, cudaStream_t st) {
+    const int held = P.blocks < kWeightBlocks ? P.blocks : kWeightBlocks;
+    launch_chained(cache_weights_kernel<NT>, device_sm_count() * 2, kWeightWarps * 32, held * sizeof(WeightRows<NT>), st, P, held);
+}
+int launch_all(const AttendParams& P, int nt, cudaStream_t st) {
+    const bool fine = nt == 1 ? launch_attend<1>(P, st) : nt == 2 ? launch_attend<2>(P, st) : launch_attend_rows(P, st);
+    if (!fine) return FMSA_ERR_CUDA;
+    if (!P.spread) {
+        switch (nt) {
+            case 1: launch_combine<1>(P, st); break;
+            case 2: launch_combine<2>(P, st); break;
+            case 4: launch_combine<4>(P, st); break;
+            case 6: launch_combine<6>(P, st); break;
+            default: launch_combine<8>(P, st);
+        }
+    }
     if (P.weights) {
-        const int held = P.blocks < kWeightBlocks ? P.blocks : kWeightBlocks;
-        launch_chained(cache_weights_kernel<NT>, sms * 2, kWeightWarps * 32, held * sizeof(WeightRows<NT>), st, P, held);
+        if (nt == 1) {
+            launch_weights<1>(P, st);
+        } else if (nt == 2) {
+            launch_weights<2>(P, st);
+        } else if (P.blocks == 1) {
+            if (!launch_weights_rows(P, st)) return FMSA_ERR_CUDA;
+        } else {   // (a token's rows in several blocks: one kernel has to have them all)
+            AttendParams W = P;
+            W.blocks = (P.rows + 15) / 16;
+            launch_weights<2>(W, st);
+        }
     }
     return check_launch();
 }
@@ -1026,10 +992,11 @@ extern "C" int fmsa_cache_attend(const fmsa_cache_attend_args* args, void* strea
     P.ml_part = reinterpret_cast<float2*>(ws + w.ml_part);
     P.lse = reinterpret_cast<float*>(ws + w.lse);
     P.Hq = Hq; P.n = n; P.group = Hq / cache->heads; P.rows = static_cast<int32_t>(rows); P.blocks = static_cast<int32_t>(blocks);
+    P.lse_rows = P.blocks * 8 * nt;
     P.fp16 = dtype == FMSA_DTYPE_FP16; P.accumulate = args->accumulate ? 1 : 0;
     P.scale_log2e = args->scale * kLog2e;
     P.magic = 0x64006400u;
     P.spread = cluster_spread(*cache, rows, args->weights != nullptr, sms);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return nt == 1 ? launch_attend<1>(P, st) : launch_attend<2>(P, st);
+    return launch_all(P, nt, st);
 }

@@ -297,6 +297,112 @@ def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(fm):
     assert torch.equal(got[:2], want[:2]) and got[2].isnan().all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sinks", [False, True])
+@pytest.mark.parametrize("hq,hkv,n,lengths", [
+    (17, 1, 1, [1]), (32, 1, 1, [128, 0, 129]), (33, 1, 1, [5000]), (24, 2, 3, [700, 2, 64]), (48, 1, 1, [16] * 20), (64, 1, 1, [300, 40]),
+    (13, 1, 5, [4, 128, 1000]), (16, 1, 9, [600, 3]), (3, 1, 43, [40, 500]), (2, 1, 150, [149, 160, 1000]), (20, 1, 1, [30, 0, 200] * 250),
+    (40, 2, 1, [20000, 1]), (96, 4, 2, [900, 1300, 5])])
+def test_attention_of_many_rows(fm, hq, hkv, n, lengths, sinks, dtype):
+    """17 query rows to a KV head and more: blocks of 32, 48 and 64, several blocks, pieces of one page, whole and cut pairs."""
+    cache, table, ls, g = pool(fm, lengths, hkv, seed=hq + n)
+    q = torch.randn(len(lengths), hq, n, 128, generator=g, device="cuda").to(dtype)
+    s = torch.randn(hq, generator=g, device="cuda") if sinks else None
+    out = check_attend(fm, cache, table, ls, lengths, q, s)
+    w = torch.rand(cache.shape[0], hkv, 128, generator=g, device="cuda")
+    for accumulate in (True, False):
+        assert torch.equal(out, check_attend(fm, cache, table, ls, lengths, q, s, w, accumulate))
+
+
+@pytest.mark.parametrize("q_size,k_size,v_size", [(1e-4, 1, 1), (30, 1, 1), (1, 1, 1e-18), (1, 1, 1e18), (1e4, 1e-6, 3e4), (1, 30, 1e-7)])
+def test_attention_of_many_rows_of_other_magnitudes(fm, q_size, k_size, v_size):
+    lengths = [900, 77]
+    cache, table, ls, g = pool(fm, lengths, 1, seed=6, k_size=k_size, v_size=v_size)
+    q = (torch.randn(2, 24, 1, 128, generator=g, device="cuda") * q_size * torch.logspace(-3, 3, 24, device="cuda").view(1, 24, 1, 1)).to(torch.bfloat16)
+    check_attend(fm, cache, table, ls, lengths, q)
+
+
+def test_attention_of_many_rows_over_values_of_mixed_size(fm):
+    """Scales of V that differ by 2^60 from token to token, and by 2^16 within a token; tokens that hold zeros, and all of them."""
+    g = torch.Generator(device="cuda").manual_seed(8)
+    n = 700
+    k, v = (torch.randn(1, 1, n, 128, generator=g, device="cuda") for _ in range(2))
+    q = torch.randn(1, 24, 1, 128, generator=g, device="cuda").to(torch.bfloat16)
+    table = torch.arange(6, dtype=torch.int32, device="cuda")[None]
+    ls = torch.tensor([n], dtype=torch.int32, device="cuda")
+    cache = fm.flash_msa_cache_empty(6, 1)
+    groups = torch.exp2(torch.tensor([0.0, -16.0, -5.0, -11.0], device="cuda")).repeat_interleave(32)
+    zeros = v.clone()
+    zeros[:, :, ::2] = 0
+    for what in [v * torch.exp2(size).cuda().view(1, 1, n, 1) for size in (torch.linspace(-30, 30, n), torch.linspace(30, -30, n), torch.rand(n) * 60 - 30)] + [
+            v * groups, zeros, torch.zeros_like(v)]:
+        fm.flash_msa_cache_append(cache, k.to(torch.bfloat16), what.to(torch.bfloat16), table, ls)
+        check_attend(fm, cache, table, ls, [n], q)
+    # a group of channels far below the token's largest keeps its accuracy: against the same values with that group alone
+    fm.flash_msa_cache_append(cache, k.to(torch.bfloat16), (v * groups).to(torch.bfloat16), table, ls)
+    got = fm.flash_msa_cache_func(q, cache, table, ls, SCALE).view(24, 128)[:, 32:64].float()
+    fm.flash_msa_cache_append(cache, k.to(torch.bfloat16), v.to(torch.bfloat16), table, ls)
+    want = fm.flash_msa_cache_func(q, cache, table, ls, SCALE).view(24, 128)[:, 32:64].float() * 2.0 ** -16
+    # (both are sums of the same products, with probabilities rounded to fp16 at another place: 2^-11 of the sum of magnitudes, and bf16's step)
+    assert (got - want).abs().max() <= 2.0 ** -16 * (2.0 ** -10 * v[..., 32:64].abs().amax() + 2.0 ** -8 * want.abs().max() * 2.0 ** 16)
+
+
+@pytest.mark.parametrize("hq,n,length,at", [(24, 3, 260, 259), (24, 3, 257, 255), (2, 150, 300, 200), (2, 150, 400, 260), (40, 2, 1, 0)])
+def test_values_that_are_not_finite_stay_with_the_rows_that_see_them_of_many(fm, hq, n, length, at):
+    cache, table, ls, g = pool(fm, [length], 1, seed=4)
+    q = torch.randn(1, hq, n, 128, generator=g, device="cuda").to(torch.bfloat16)
+    want = fm.flash_msa_cache_func(q, cache, table, ls, SCALE).view(n, hq, 128)
+    k, v = (torch.randn(1, 1, 1, 128, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    v[..., 40] = math.inf
+    fm.flash_msa_cache_append(cache, k, v, table, torch.tensor([at + 1], dtype=torch.int32, device="cuda"))
+    first = max(0, at - (length - n))                     # the first query row that sees the token
+    got = fm.flash_msa_cache_func(q, cache, table, ls, SCALE).view(n, hq, 128)
+    assert torch.equal(got[:first], want[:first])
+    assert got[first:, :, 32:64].isnan().all() and torch.isfinite(got[first:, :, :32]).all() and torch.isfinite(got[first:, :, 64:]).all()
+    k[..., 3] = math.nan
+    fm.flash_msa_cache_append(cache, k, v, table, torch.tensor([at + 1], dtype=torch.int32, device="cuda"))
+    got = fm.flash_msa_cache_func(q, cache, table, ls, SCALE).view(n, hq, 128)
+    assert torch.equal(got[:first], want[:first]) and got[first:].isnan().all()
+
+
+def test_attention_of_many_rows_captured(fm):
+    """A captured call follows what its tensors hold at each replay; two graphs of the same shapes do not share anything."""
+    lengths = [700, 0, 130]
+    cache, table, ls, g = pool(fm, lengths, 2, seed=11)
+    qs = [torch.randn(3, 40, 1, 128, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2)]
+    want = [fm.flash_msa_cache_func(q, cache, table, ls, SCALE) for q in qs]
+    ws = [torch.zeros(cache.shape[0], 2, 128, device="cuda") for _ in range(2)]
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    from flash_msa_b200 import api
+    fm.flash_msa_cache_func(qs[0], cache, table, ls, SCALE, weights=ws[0].clone())
+    api.DEBUG_CHECK_STATUS = False
+    try:
+        fm.flash_msa_cache_func(qs[0], cache, table, ls, SCALE, weights=ws[0].clone())
+        for graph, q, w in zip(graphs, qs, ws):
+            with torch.cuda.graph(graph):
+                outs.append(fm.flash_msa_cache_func(q, cache, table, ls, SCALE, weights=w))
+    finally:
+        api.DEBUG_CHECK_STATUS = True
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        graphs[0].replay()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+    torch.cuda.synchronize()
+    for q, w, out, exp in zip(qs, ws, outs, want):
+        assert torch.equal(out, exp)
+        one = torch.zeros_like(w)
+        fm.flash_msa_cache_func(q, cache, table, ls, SCALE, weights=one, accumulate=False)
+        assert torch.equal(w, one + one + one)
+    ls.copy_(torch.tensor([1, 0, 129], dtype=torch.int32))
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    exp = fm.flash_msa_cache_func(qs[0], cache, table, ls, SCALE)
+    assert torch.equal(outs[0], exp)
+    fm.check_pending_status()
+
+
 def test_records_beyond_four_gigabytes(fm):
     lengths = [300]
     small, t_small, ls, g = pool(fm, lengths, 2, seed=11)
