@@ -122,7 +122,7 @@ def _declare(lib):
         getattr(lib, name).restype = c_int
         getattr(lib, name).argtypes = [P, P]
     lib.fmsa_cache_attend_workspace_bytes.restype = c_int64
-    lib.fmsa_cache_attend_workspace_bytes.argtypes = [c_int32, c_int32, c_int32, c_int32]
+    lib.fmsa_cache_attend_workspace_bytes.argtypes = [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]
     lib.fmsa_prompt_workspace_bytes.restype = c_int64
     lib.fmsa_prompt_workspace_bytes.argtypes = [c_int32, c_int32, c_int32, c_int32, c_int32]
     lib.fmsa_cache_attend_launches.restype = c_int32

@@ -941,13 +941,6 @@ int launch_all(const AttendParams& P, int nt, cudaStream_t st) {
 }  // namespace
 }  // namespace fmsa
 
-extern "C" int64_t fmsa_cache_attend_workspace_bytes(int32_t seqs, int32_t Hq, int32_t heads, int32_t n) {
-    using namespace fmsa;
-    const int sms = device_sm_count();
-    if (seqs <= 0 || heads <= 0 || Hq <= 0 || Hq % heads || n <= 0 || sms <= 0) return -1;
-    return carve_attend(seqs, Hq, heads, n, sms).bytes;
-}
-
 extern "C" int32_t fmsa_cache_attend_launches(int32_t seqs, int32_t Hq, int32_t heads, int32_t n, int32_t width, int32_t weights) {
     using namespace fmsa;
     const int sms = device_sm_count();
@@ -955,6 +948,12 @@ extern "C" int32_t fmsa_cache_attend_launches(int32_t seqs, int32_t Hq, int32_t 
     fmsa_cache4 c = {};
     c.seqs = seqs; c.heads = heads; c.width = width;
     return weights ? 3 : cluster_spread(c, static_cast<int64_t>(Hq / heads) * n, false, sms) ? 1 : 2;
+}
+
+extern "C" int64_t fmsa_cache_attend_workspace_bytes(int32_t seqs, int32_t Hq, int32_t heads, int32_t n, int32_t width, int32_t weights) {
+    using namespace fmsa;
+    const int32_t launches = fmsa_cache_attend_launches(seqs, Hq, heads, n, width, weights);
+    return launches <= 1 ? launches < 0 ? -1 : 0 : carve_attend(seqs, Hq, heads, n, device_sm_count()).bytes;
 }
 
 extern "C" int fmsa_cache_attend(const fmsa_cache_attend_args* args, void* stream) {
@@ -965,7 +964,7 @@ extern "C" int fmsa_cache_attend(const fmsa_cache_attend_args* args, void* strea
     const int32_t Hq = args->Hq, n = args->n, dtype = args->dtype;
     int32_t* status = args->status;
     void *out = args->out, *workspace = args->workspace;
-    FMSA_REQUIRE(cache4_ok(cache) && q->ptr && out && workspace && status && Hq > 0 && n > 0 && Hq % cache->heads == 0);
+    FMSA_REQUIRE(cache4_ok(cache) && q->ptr && out && status && Hq > 0 && n > 0 && Hq % cache->heads == 0);
     FMSA_REQUIRE(dtype == FMSA_DTYPE_BF16 || dtype == FMSA_DTYPE_FP16);
     FMSA_REQUIRE(aligned16(q->ptr) && q->stride_b % 8 == 0 && q->stride_h % 8 == 0 && q->stride_s % 8 == 0);
     const int64_t rows = static_cast<int64_t>(Hq / cache->heads) * n;
@@ -973,12 +972,16 @@ extern "C" int fmsa_cache_attend(const fmsa_cache_attend_args* args, void* strea
     const int64_t blocks = (rows + 8 * nt - 1) / (8 * nt), items = blocks * cache->heads * cache->seqs;
     if (items > 0x7fffffffLL || items * cache->width > 0x7fffffffLL) return FMSA_ERR_UNSUPPORTED;   // (units are counted in 32 bits)
     const int sms = device_sm_count();
-    if (sms <= 0) return FMSA_ERR_CUDA;
     AttendParams P = {};
     P.grid = sms;
-    const AttendSpace w = carve_attend(cache->seqs, Hq, cache->heads, n, P.grid);
-    if (args->workspace_bytes < w.bytes) return FMSA_ERR_WORKSPACE;
-    FMSA_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0);
+    P.spread = sms > 0 ? cluster_spread(*cache, rows, args->weights != nullptr, sms) : 0;
+    AttendSpace w = {};
+    if (!P.spread) {
+        FMSA_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0);
+        w = carve_attend(cache->seqs, Hq, cache->heads, n, sms > 0 ? sms : 1);
+        if (args->workspace_bytes < w.bytes) return FMSA_ERR_WORKSPACE;
+    }
+    if (sms <= 0) return FMSA_ERR_CUDA;
     char* ws = static_cast<char*>(workspace);
     P.cache = device_cache(cache, status);
     P.q = static_cast<const uint16_t*>(q->ptr);
@@ -996,7 +999,6 @@ extern "C" int fmsa_cache_attend(const fmsa_cache_attend_args* args, void* strea
     P.fp16 = dtype == FMSA_DTYPE_FP16; P.accumulate = args->accumulate ? 1 : 0;
     P.scale_log2e = args->scale * kLog2e;
     P.magic = 0x64006400u;
-    P.spread = cluster_spread(*cache, rows, args->weights != nullptr, sms);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     return launch_all(P, nt, st);
 }

@@ -720,7 +720,8 @@ extern "C" int32_t fmsa_prompt_launches(int32_t B, int32_t S, int32_t Hq, int32_
 
 extern "C" int64_t fmsa_prompt_workspace_bytes(int32_t B, int32_t S, int32_t Hq, int32_t Hkv, int32_t n_seqs) {
     fmsa::PromptSpace w;
-    return fmsa::prompt_space(B, S, Hq, Hkv, n_seqs, &w) ? w.bytes : -1;
+    if (!fmsa::prompt_space(B, S, Hq, Hkv, n_seqs, &w)) return -1;
+    return fmsa::prompt_direct(w, B, Hkv, n_seqs, fmsa::device_sm_count()) ? 0 : w.bytes;
 }
 
 extern "C" int fmsa_prompt_fwd(const fmsa_prompt_args* args, void* stream) {
@@ -734,13 +735,17 @@ extern "C" int fmsa_prompt_fwd(const fmsa_prompt_args* args, void* stream) {
     int32_t* status = args->status;
     if (!cu_seqlens) n_seqs = 1;
     PromptSpace w;
-    FMSA_REQUIRE(q->ptr && k->ptr && v->ptr && out && workspace && status && aligned16(out));
+    FMSA_REQUIRE(q->ptr && k->ptr && v->ptr && out && status && aligned16(out));
     FMSA_REQUIRE(B > 0 && S > 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && n_seqs > 0 && scale > 0.f);
     FMSA_REQUIRE(dtype == FMSA_DTYPE_BF16 || dtype == FMSA_DTYPE_FP16);
     if (!prompt_space(B, S, Hq, Hkv, n_seqs, &w)) return FMSA_ERR_UNSUPPORTED;
     if (S > (1 << 30) || w.cap * Hkv >= 0x7f000000LL || static_cast<int64_t>(B) * n_seqs >= 0x7f000000LL) return FMSA_ERR_UNSUPPORTED;
-    FMSA_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0);
-    if (args->workspace_bytes < w.bytes) return FMSA_ERR_WORKSPACE;
+    const int sms = device_sm_count();
+    const bool direct = prompt_direct(w, B, Hkv, n_seqs, sms);
+    if (!direct) {
+        FMSA_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0);
+        if (args->workspace_bytes < w.bytes) return FMSA_ERR_WORKSPACE;
+    }
     for (const fmsa_tensor* t : {q, k, v}) FMSA_REQUIRE(tma_compatible(t->ptr, t->stride_b, t->stride_h, t->stride_s));
     CUtensorMap tq, tk, tv;
     if (!make_tmap_heads(&tq, q->ptr, B, Hq, S, q->stride_b, q->stride_h, q->stride_s, w.group, w.tokens) ||
@@ -753,20 +758,21 @@ extern "C" int fmsa_prompt_fwd(const fmsa_prompt_args* args, void* stream) {
     P.v = static_cast<const __nv_bfloat16*>(v->ptr);
     P.vs[0] = v->stride_b; P.vs[1] = v->stride_h; P.vs[2] = v->stride_s;
     P.out = static_cast<__nv_bfloat16*>(out);
-    P.counter = static_cast<int32_t*>(workspace);
-    P.tiles = reinterpret_cast<int4*>(static_cast<char*>(workspace) + 256);
+    if (!direct) {
+        P.counter = static_cast<int32_t*>(workspace);
+        P.tiles = reinterpret_cast<int4*>(static_cast<char*>(workspace) + 256);
+    }
     P.status = status;
     P.B = B; P.S = S; P.Hq = Hq; P.Hkv = Hkv; P.group = w.group; P.tokens = w.tokens;
     P.n_seqs = n_seqs; P.per_batch = args->per_batch ? 1 : 0; P.cap = static_cast<int32_t>(w.cap);
     while (((S + kBlock - 1) / kBlock >> P.shift) >= kPlanBins) ++P.shift;
     P.scale_log2e = scale * kLog2e;
-    const int sms = device_sm_count();
     auto kernel = dtype == FMSA_DTYPE_FP16 ? prompt_fwd_kernel<true> : prompt_fwd_kernel<false>;
     if (sms <= 0 || !ensure_smem_attr(reinterpret_cast<const void*>(kernel), kPrSmemBytes)) return FMSA_ERR_CUDA;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int64_t items = w.cap * Hkv;
-    P.direct = prompt_direct(w, B, Hkv, n_seqs, sms);
-    if (!P.direct) launch_chained(prompt_plan_kernel, cu_seqlens ? 33 : 1, kPlanThreads, 0, st, P);
+    P.direct = direct;
+    if (!direct) launch_chained(prompt_plan_kernel, cu_seqlens ? 33 : 1, kPlanThreads, 0, st, P);
     launch_chained(kernel, static_cast<unsigned>(items < sms ? items : sms), kPrThreads, kPrSmemBytes, st, tq, tk, tv, P);
     return check_launch();
 }

@@ -240,17 +240,19 @@ def cache_append(cache, k, v, block_table, lengths, cu_seqlens=None, weights=Non
     return values
 
 
-_sizes = {}   # what the library says of (operator, sizes, device)
+_plans = {}   # what the library says of (operator, device, sizes)
 
 
-def _size(device, entry, *sizes):
+def _plan(device, entry, *sizes):
+    """(bytes of the workspace - none where one launch is all -, launches)."""
     key = (entry, device, *sizes)
-    got = _sizes.get(key)
+    got = _plans.get(key)
     if got is None:
-        if len(_sizes) >= 1024:
-            _sizes.clear()
+        if len(_plans) >= 1024:
+            _plans.clear()
+        lib = _lib.load()
         with torch.cuda.device(device):
-            got = _sizes[key] = getattr(_lib.load(), entry)(*sizes)
+            got = _plans[key] = max(getattr(lib, entry + "_workspace_bytes")(*sizes), 0), getattr(lib, entry + "_launches")(*sizes)
     return got
 
 
@@ -273,14 +275,13 @@ def cache_attention(q, cache, block_table, lengths, scale: float, sinks=None, we
     if b == 0 or n == 0:
         return out
     lib = _lib.load()
-    nbytes = _size(dev, "fmsa_cache_attend_workspace_bytes", b, hq, hkv, n)
+    nbytes, launches = _plan(dev, "fmsa_cache_attend", b, hq, hkv, n, fields[7], 0 if weights is None else 1)
     q, qf = _readable(q)
-    ws = cache.new_empty(max(nbytes, 1))
+    ws = cache.new_empty(nbytes) if nbytes else None
     word = _Word(_KIND_ATTEND, dev)
-    launches = _size(dev, "fmsa_cache_attend_launches", b, hq, hkv, n, fields[7], 0 if weights is None else 1)
     _call("fmsa_cache_attend", launches, lib.fmsa_cache_attend, _ATTEND_ARGS.pack(
-        *fields, *qf, 0 if logits is None else logits.data_ptr(), 0 if weights is None else weights.data_ptr(), out.data_ptr(), ws.data_ptr(),
-        nbytes, word.ptr, hq, n, ops._dtype_code(q.dtype), 1 if accumulate else 0, scale, 0), dev)
+        *fields, *qf, 0 if logits is None else logits.data_ptr(), 0 if weights is None else weights.data_ptr(), out.data_ptr(),
+        0 if ws is None else ws.data_ptr(), nbytes, word.ptr, hq, n, ops._dtype_code(q.dtype), 1 if accumulate else 0, scale, 0), dev)
     word.check()
     return out
 
@@ -354,11 +355,11 @@ def prompt_attention(q, k, v, cu_seqlens, scale: float, sinks=None):
     q, qf = _tma_readable(q)
     k, kf = _tma_readable(k)
     v, vf = _tma_readable(v)
-    nbytes = _size(dev, "fmsa_prompt_workspace_bytes", b, s, hq, hkv, n_seqs)
-    ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=q.device)
+    nbytes, launches = _plan(dev, "fmsa_prompt", b, s, hq, hkv, n_seqs)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     word = _Word(_KIND_PROMPT, dev)
-    _call("fmsa_prompt_fwd", _size(dev, "fmsa_prompt_launches", b, s, hq, hkv, n_seqs), lib.fmsa_prompt_fwd, _PROMPT_ARGS.pack(
+    _call("fmsa_prompt_fwd", launches, lib.fmsa_prompt_fwd, _PROMPT_ARGS.pack(
         *qf, *kf, *vf, 0 if cu_seqlens is None else cu_seqlens.data_ptr(), 0 if logits is None else logits.data_ptr(), out.data_ptr(),
-        ws.data_ptr(), nbytes, word.ptr, b, s, hq, hkv, n_seqs, per_batch, ops._dtype_code(q.dtype), scale), dev)
+        0 if ws is None else ws.data_ptr(), nbytes, word.ptr, b, s, hq, hkv, n_seqs, per_batch, ops._dtype_code(q.dtype), scale), dev)
     word.check()
     return out

@@ -374,7 +374,8 @@ int fmsa_cache_append(const fmsa_cache_append_args* args, void* stream);
 /* Attention of the last n tokens of every sequence over the cache: query j of q (seqs,Hq,n,128) sees the first lengths[i] - n + 1 + j
  * tokens; a row that sees none is zero.  out [seqs][n][Hq*128] contiguous.  sinks fp32 [Hq] or NULL, as in fmsa_forward_args.
  * weights fp32 [pages][heads][128] or NULL: for every token below lengths[i] the probability it got, summed over the rows of its KV
- * head, is added (accumulate = 1) or written (0).  workspace 256-byte aligned.  fmsa_cache_attend_launches() launches: one where few pairs
+ * head, is added (accumulate = 1) or written (0).  workspace 256-byte aligned (may be null where it
+ * takes no bytes, which is where one launch is all).  fmsa_cache_attend_launches() launches: one where few pairs
  * of sequence and KV head have few pages, two, or three with weights. */
 typedef struct {
     fmsa_cache4 cache;
@@ -388,7 +389,7 @@ typedef struct {
     float scale;
     int32_t reserved;
 } fmsa_cache_attend_args;
-int64_t fmsa_cache_attend_workspace_bytes(int32_t seqs, int32_t Hq, int32_t heads, int32_t n);
+int64_t fmsa_cache_attend_workspace_bytes(int32_t seqs, int32_t Hq, int32_t heads, int32_t n, int32_t width, int32_t weights);
 int32_t fmsa_cache_attend_launches(int32_t seqs, int32_t Hq, int32_t heads, int32_t n, int32_t width, int32_t weights);
 int fmsa_cache_attend(const fmsa_cache_attend_args* args, void* stream);
 

@@ -450,7 +450,8 @@ def test_pages_that_do_not_exist(fm):
 
 @pytest.mark.parametrize("kind", ["random", "ties", "zeros", "odd"])
 @pytest.mark.parametrize("lengths,hkv,keep,recent", [([1], 1, 1, 0), ([200], 2, 130, 0), ([200, 0, 129, 500], 3, 129, 129), ([700, 90], 1, 257, 60),
-                                                     ([1000], 2, 1, 1), ([3000, 2999], 1, 2998, 7), ([9000, 100], 1, 5000, 100), ([40000], 1, 5000, 100)])
+                                                     ([1000], 2, 1, 1), ([3000, 2999], 1, 2998, 7), ([9000, 100], 1, 5000, 100), ([40000], 1, 5000, 100),
+                                                     ([1100, 30, 0, 513], 2, 512, 64), ([8000, 1024, 1025], 1, 1024, 0), ([9000, 5], 1, 700, 3)])
 def test_evict(fm, lengths, hkv, keep, recent, kind):
     cache, table, ls, g = pool(fm, lengths, hkv, seed=keep, spare=len(lengths) * (-(-keep // 128)) + 2)
     own = len(lengths) * table.shape[1]

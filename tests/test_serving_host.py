@@ -175,8 +175,8 @@ def test_c_entries_refuse_before_they_touch_anything(kind, change, status):
 
 def test_other_c_entries():
     lib = _lib.load()
-    assert lib.fmsa_prompt_workspace_bytes(1, 100, 3, 2, 1) == -1 and lib.fmsa_prompt_workspace_bytes(2, 100, 4, 2, 3) > 0
-    assert lib.fmsa_cache_attend_workspace_bytes(1, 3, 2, 1) == -1
+    assert lib.fmsa_prompt_workspace_bytes(1, 100, 3, 2, 1) == -1 and lib.fmsa_prompt_workspace_bytes(2, 50000, 4, 2, 3) > 0
+    assert lib.fmsa_cache_attend_workspace_bytes(1, 3, 2, 1, 1, 0) == -1
     assert lib.fmsa_boundaries(None, 3, None, None) == -1
     assert lib.fmsa_boundaries((ctypes.c_int32 * 4)(), 897, 0x10, None) == -2
 
