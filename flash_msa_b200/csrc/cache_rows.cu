@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) cache_rows_kernel(const Atten
     // For those that are ahead: looks again after about `ns`.  (Warps that look all the time took half of the issue slots.)
     auto wait_idle = [&](uint32_t bar, uint32_t parity, uint32_t ns) {
         for (uint32_t n = 0; !bad && !__all_sync(0xffffffffu, mbar_try_wait(bar, parity)); ++n) {
-            bad = n > 2000000000u / ns;
+            bad = n > 1000000;   // (a try and a sleep take a microsecond or two)
             __nanosleep(ns);
         }
     };

@@ -117,28 +117,28 @@ struct PromptItem {
 };
 
 constexpr int kPrKvStages = 5, kPrBuffers = 3, kPrRing = 4;
-constexpr int kPrThreads = 3 * 128;
-// Registers per thread after the warpgroups re-divide the register file: 384 threads are launched with 168.
-constexpr int kPrRegsLaunch = 168, kPrRegsSoftmax = 208, kPrRegsMisc = 88;
-static_assert(2 * kPrRegsSoftmax + kPrRegsMisc <= 3 * kPrRegsLaunch, "register re-division must balance");
+constexpr int kPrThreads = 4 * 128;
+// Registers per thread after the warpgroups re-divide the register file: 512 threads are launched with 128.
+constexpr int kPrRegsLaunch = 128, kPrRegsSoftmax = 176, kPrRegsRows = 104, kPrRegsMisc = 56;
+static_assert(2 * kPrRegsSoftmax + kPrRegsRows + kPrRegsMisc <= 4 * kPrRegsLaunch, "register re-division must balance");
 static_assert(kPrRegsLaunch == (65536 / kPrThreads) / 8 * 8, "registers per thread at launch");
 
 struct PromptCtrl {
     uint64_t q_full, q_empty, kv_full[kPrKvStages], kv_empty[kPrKvStages];
     uint64_t s_full[kPrBuffers], p_full[kPrBuffers][2], pv_done[kPrBuffers];   // p_full: [half of the keys]
     uint64_t chain[2][4];                        // [group][quarter]
-    uint64_t sum_full[2], o_free;                // [group]
+    uint64_t sum_full[kPrRing], o_free;
     uint64_t item_full[kPrRing], item_empty[kPrRing];
     PromptItem items[kPrRing];
     uint32_t odd[kPrRing][2][4];                 // careful: keys of the item's first two blocks that hold a value that is not finite
     uint32_t again[kPrRing];                     // a result of the item is not finite
     float top[128];                              // running maximum of every row (log2 domain)
-    float2 part[2][128];                         // [group] (max, sum) at the end of an item
+    float2 part[kPrRing][2][128];                // [group] (max, sum) at the end of an item
     uint32_t tmem_slot;
 };
 constexpr size_t kPrTileBytes = static_cast<size_t>(1 + kPrKvStages) * kTileBytes;
-constexpr int kPrStaging = 32 * 64;              // of a softmax warp: 32 columns of its rows on their way out
-constexpr size_t kPrSmemBytes = kPrTileBytes + 8 * kPrStaging + 1024 + sizeof(PromptCtrl);
+constexpr int kPrStaging = 32 * 64;              // of a warp: 32 columns of its rows on their way out
+constexpr size_t kPrSmemBytes = kPrTileBytes + 4 * kPrStaging + 1024 + sizeof(PromptCtrl);
 static_assert(kPrSmemBytes <= 232448, "shared memory budget of one CTA");
 
 // As in tile_fwd.cu: rows whose maximum grows by less than this (log2) keep the old one; fp16 P are 2^7 times larger.
@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
     extern __shared__ uint8_t smem_raw[];
     const uint32_t tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t tile_q = tiles, tile_kv = tiles + kTileBytes;
-    PromptCtrl* sm = reinterpret_cast<PromptCtrl*>(smem_raw + (tiles - smem_u32(smem_raw)) + kPrTileBytes + 8 * kPrStaging);
+    PromptCtrl* sm = reinterpret_cast<PromptCtrl*>(smem_raw + (tiles - smem_u32(smem_raw)) + kPrTileBytes + 4 * kPrStaging);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
@@ -180,8 +180,6 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
     if (tid == 0) {
         mbar_init(BAR(sm->q_full), 1);
         mbar_init(BAR(sm->q_empty), 1);
-        mbar_init(BAR(sm->sum_full[0]), 4);
-        mbar_init(BAR(sm->sum_full[1]), 4);
         mbar_init(BAR(sm->o_free), 4);
         for (int i = 0; i < 8; ++i) mbar_init(BAR(sm->chain[i >> 2][i & 3]), 1);
         for (int i = 0; i < kPrBuffers; ++i) {
@@ -196,7 +194,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
         }
         for (int i = 0; i < kPrRing; ++i) {
             mbar_init(BAR(sm->item_full[i]), 1);
-            mbar_init(BAR(sm->item_empty[i]), 11);   // loads, issue (2), eight softmax warps
+            mbar_init(BAR(sm->item_empty[i]), 15);   // loads, issue (2), eight softmax warps, four that write rows
+            mbar_init(BAR(sm->sum_full[i]), 8);
         }
         fence_mbar_init();
         prefetch_tmap(&tmap_q);
@@ -234,9 +233,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
         __syncwarp();
         if (lane == 0) mbar_arrive(bar);
     };
-    if (warp >= 8) {
+    if (warp >= 12) {
         reg_dec<kPrRegsMisc>();
-        if (warp == 10) {
+        if (warp == 14) {
             // =========================== items ===========================
             uint32_t n_items = 0, draw = 0;
             int4 tile = make_int4(0, 0, 0, 0);   // direct: this CTA's
@@ -323,7 +322,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
             PromptItem none = {};
             none.steps = -1;
             if (!bad) publish(none);
-        } else if (warp == 8 && elect_one()) {
+        } else if (warp == 12 && elect_one()) {
             // =========================== tile loads ===========================
             uint32_t st = 0, ph = 1, items = 0;   // stage of the ring, phase bit of its kv_empty, items so far
             for (uint32_t draw = 0;; ++draw, ++items) {
@@ -356,9 +355,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
                 }
                 mbar_arrive(BAR(sm->item_empty[slot]));
             }
-        } else if ((warp == 9 || warp == 11) && elect_one()) {
-            // =========================== S (warp 9) and P V (warp 11) ===========================
-            const bool pv = warp == 11;
+        } else if ((warp == 13 || warp == 15) && elect_one()) {
+            // =========================== S (warp 13) and P V (warp 15) ===========================
+            const bool pv = warp == 15;
             uint32_t st0 = 0, ph0 = 0;       // ring position (stage, phase bit) of the item's first tile
             uint32_t buf = 0, bph = 0;       // S buffer and its phase bit
             for (uint32_t draw = 0;; ++draw) {
@@ -393,6 +392,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
                     } else {
                         wait1(BAR(sm->p_full[buf][0]), bph);
                         wait1(BAR(sm->kv_full[st]), ph);
+                        // the first product of an item overwrites O: the rows of the item before must have been read
+                        if (t == 0 && draw > 0) wait1(BAR(sm->o_free), (draw - 1) & 1);
                         if (bad) break;
                         tc_fence_after_sync();
                         // O += P V_j, of the first block the keys that are seen
@@ -421,6 +422,99 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
                 mbar_arrive(BAR(sm->item_empty[slot]));
             }
         }
+    } else if (warp >= 8) {
+        reg_dec<kPrRegsRows>();
+        // =========================== rows on their way out ===========================
+        const int tok = row / P.group, hh = row - tok * P.group;   // (rows behind the last whole token: tok >= P.tokens)
+        uint32_t done = 0;               // steps so far
+        for (uint32_t draw = 0;; ++draw) {
+            const uint32_t slot = draw % kPrRing;
+            wait(BAR(sm->item_full[slot]), (draw / kPrRing) & 1);
+            if (bad) break;
+            const PromptItem it = sm->items[slot];
+            if (it.steps < 0) break;
+            done += it.steps;
+            const int ahead = it.row0 - it.lo;
+            const bool careful = it.careful;
+            wait(BAR(sm->sum_full[slot]), (draw / kPrRing) & 1);
+            if (bad) break;
+            const float2 a = sm->part[slot][0][row], b = sm->part[slot][1][row];
+            const float m = fmaxf(a.x, b.x);   // (maxima only rise: the one of the group that had the last step)
+            float l = (a.x == -INFINITY ? 0.f : a.y * fast_exp2(a.x - m)) + (b.x == -INFINITY ? 0.f : b.y * fast_exp2(b.x - m));
+            const int head = it.head * P.group + hh;
+            const bool real = tok < it.count && tok < P.tokens;
+            if (P.sinks && real) l += fast_exp2(P.sinks[head] * kLog2e + (m == -INFINITY ? 0.f : kPrLiftP<FP16> - m));
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const float2 inv2 = make_float2(inv, inv);
+            wait(BAR(sm->pv_done[(done - 1) % kPrBuffers]), (done - 1) / kPrBuffers & 1);
+            if (bad) break;
+            tc_fence_after_sync();
+            __nv_bfloat16* to = P.out + (static_cast<int64_t>(it.b) * P.S + it.row0 + tok) * (static_cast<int64_t>(P.Hq) * kHeadDim) +
+                                static_cast<int64_t>(head) * kHeadDim;
+            // Rows leave through shared memory, 32 columns at a time, so that four lanes write 64 bytes of a row: a lane with a row of its
+            // own wrote 16 bytes here and there and took 4000 cycles a tile, 2600 this way.
+            const uint32_t staged = tiles + kPrTileBytes + quarter * kPrStaging;
+            int64_t out_of[4];               // where this lane's pieces of rows 8 i + lane / 4 go, or -1
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t at = real ? to - P.out : -1;
+                out_of[i] = __shfl_sync(0xffffffffu, at, 8 * i + (lane >> 2));
+            }
+            uint32_t finite = 0;             // 0 or NaN
+            uint32_t o[2][32];
+            tmem_ld32(tmem_addr(tmem_o, quarter, 0), o[0]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {    // (the columns after these are on their way meanwhile)
+                tmem_ld_wait();
+                if (c < 3) {
+                    tmem_ld32(tmem_addr(tmem_o, quarter, 32 * c + 32), o[(c + 1) & 1]);
+                } else {
+                    tc_fence_before_sync();
+                    warp_arrive(BAR(sm->o_free));
+                }
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    uint32_t pk[4];
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) {
+                        const float2 r = f2_mul(f2_from_bits(o[c & 1][8 * y + 2 * z], o[c & 1][8 * y + 2 * z + 1]), inv2);
+                        pk[z] = pack_act<FP16>(r.x, r.y);
+                        finite = times_zero<FP16>(pk[z], finite);
+                    }
+                    st_shared_v4(staged + lane * 64 + ((y ^ (lane >> 1 & 3)) << 4), pk[0], pk[1], pk[2], pk[3]);
+                }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = 8 * i + (lane >> 2);
+                    const uint4 x = ld_shared_v4(staged + r * 64 + (((lane & 3) ^ (r >> 1 & 3)) << 4));
+                    if (out_of[i] >= 0) *reinterpret_cast<uint4*>(P.out + out_of[i] + 32 * c + 8 * (lane & 3)) = x;
+                }
+                __syncwarp();
+            }
+            if (!careful && __any_sync(0xffffffffu, real && (finite & 0x7fff7fffu)) && lane == 0) sm->again[slot] = 1;
+            // values that are not finite, for the rows that see them (what they were multiplied with does not matter)
+#pragma unroll 1
+            for (int t = 0; careful && t < 2; ++t) {
+#pragma unroll 1
+                for (int w = 0; w < 4; ++w) {
+#pragma unroll 1
+                    for (uint32_t odd = sm->odd[slot][t][w]; odd; odd &= odd - 1) {
+                        const int key = (it.steps - 1 - t) * kBlock + 32 * w + __ffs(odd) - 1;
+                        if (!real || key > ahead + tok) continue;
+                        const __nv_bfloat16* from = P.v + it.b * P.vs[0] + it.head * P.vs[1] + (it.lo + key) * P.vs[2];
+#pragma unroll 1
+                        for (int c = 0; c < 128; c += 2) {
+                            const uint32_t x = *reinterpret_cast<const uint32_t*>(from + c), y = *reinterpret_cast<const uint32_t*>(to + c);
+                            const float x0 = act_lo<FP16>(x), x1 = act_hi<FP16>(x);
+                            const float y0 = act_lo<FP16>(y) + (isfinite(x0) ? 0.f : x0), y1 = act_hi<FP16>(y) + (isfinite(x1) ? 0.f : x1);
+                            *reinterpret_cast<uint32_t*>(to + c) = pack_act<FP16>(y0, y1);
+                        }
+                    }
+                }
+            }
+            warp_arrive(BAR(sm->item_empty[slot]));
+        }
     } else {
         reg_inc<kPrRegsSoftmax>();
         // =========================== softmax ===========================
@@ -430,10 +524,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
         const int g = warp >> 2;
         const uint32_t chain_in = BAR(sm->chain[g ^ 1][quarter]), chain_out = BAR(sm->chain[g][quarter]);
         const float2 sc2 = make_float2(P.scale_log2e, P.scale_log2e);
-        const int tok = row / P.group, hh = row - tok * P.group;   // (rows behind the last whole token: tok >= P.tokens)
+        const int tok = row / P.group;   // (rows behind the last whole token: tok >= P.tokens)
         uint32_t step = 0;               // steps so far
         uint32_t buf = 0, bph = 0;       // S buffer and its phase bit
-        uint32_t sums = 0;               // phase bits of sum_full
         uint32_t last = 0, last_ph = 0;  // S buffer of the step before, its phase bit
         uint32_t ring = 0;               // ring position (stage + 5 * phase bit) of the item's first tile
         for (uint32_t draw = 0;; ++draw) {
@@ -571,8 +664,6 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
                         tmem_st16(tmem_addr(ts, quarter, 16 * c), pk);
                         }
                         if (c & 1) {
-                            // the first product of an item overwrites O: the rows of the item before must have been read
-                            if (c == 1 && t == 0 && draw > 0) wait(BAR(sm->o_free), (draw - 1) & 1);
                             tmem_st_wait();
                             tc_fence_before_sync();
                             warp_arrive(BAR(sm->p_full[buf][c >> 1]));
@@ -589,94 +680,12 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
             }
             if (bad) break;
             ring = (ring + 2 * steps) % (2 * kPrKvStages);
-            // ---- the end of the item
-            const int other = step & 1;   // the group that did not have the last step
-            if (g == other) {
-                sm->part[g][row] = make_float2(m, l);
-                warp_arrive(BAR(sm->sum_full[g]));
-                warp_arrive(BAR(sm->item_empty[slot]));
-            } else {
-                const PromptItem it = sm->items[slot];
-                wait(BAR(sm->sum_full[other]), (sums >> other) & 1);
-                if (bad) break;
-                const float2 a = sm->part[other][row];
-                // (maxima only rise: this group's is the latest)
-                l += a.x == -INFINITY ? 0.f : a.y * fast_exp2(a.x - m);
-                const int head = it.head * P.group + hh;
-                const bool real = tok < it.count && tok < P.tokens;
-                if (P.sinks && real) l += fast_exp2(P.sinks[head] * kLog2e + (m == -INFINITY ? 0.f : kPrLiftP<FP16> - m));
-                const float inv = l == 0.f ? 0.f : 1.f / l;
-                const float2 inv2 = make_float2(inv, inv);
-                wait(BAR(sm->pv_done[last]), last_ph);
-                if (bad) break;
-                tc_fence_after_sync();
-                __nv_bfloat16* to = P.out + (static_cast<int64_t>(it.b) * P.S + it.row0 + tok) * (static_cast<int64_t>(P.Hq) * kHeadDim) +
-                                    static_cast<int64_t>(head) * kHeadDim;
-                // Rows leave through shared memory, 32 columns at a time, so that four lanes write 64 bytes of a row: a lane with a row of its
-                // own wrote 16 bytes here and there and took 4000 cycles a tile, 2600 this way.
-                const uint32_t staged = tiles + kPrTileBytes + warp * kPrStaging;
-                int64_t out_of[4];               // where this lane's pieces of rows 8 i + lane / 4 go, or -1
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int64_t at = real ? to - P.out : -1;
-                    out_of[i] = __shfl_sync(0xffffffffu, at, 8 * i + (lane >> 2));
-                }
-                uint32_t finite = 0;             // 0 or NaN
-                uint32_t o[2][32];
-                tmem_ld32(tmem_addr(tmem_o, quarter, 0), o[0]);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {    // (the columns after these are on their way meanwhile)
-                    tmem_ld_wait();
-                    if (c < 3) {
-                        tmem_ld32(tmem_addr(tmem_o, quarter, 32 * c + 32), o[(c + 1) & 1]);
-                    } else {
-                        tc_fence_before_sync();
-                        warp_arrive(BAR(sm->o_free));
-                    }
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) {
-                        uint32_t pk[4];
-#pragma unroll
-                        for (int z = 0; z < 4; ++z) {
-                            const float2 r = f2_mul(f2_from_bits(o[c & 1][8 * y + 2 * z], o[c & 1][8 * y + 2 * z + 1]), inv2);
-                            pk[z] = pack_act<FP16>(r.x, r.y);
-                            finite = times_zero<FP16>(pk[z], finite);
-                        }
-                        st_shared_v4(staged + lane * 64 + ((y ^ (lane >> 1 & 3)) << 4), pk[0], pk[1], pk[2], pk[3]);
-                    }
-                    __syncwarp();
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int r = 8 * i + (lane >> 2);
-                        const uint4 x = ld_shared_v4(staged + r * 64 + (((lane & 3) ^ (r >> 1 & 3)) << 4));
-                        if (out_of[i] >= 0) *reinterpret_cast<uint4*>(P.out + out_of[i] + 32 * c + 8 * (lane & 3)) = x;
-                    }
-                    __syncwarp();
-                }
-                if (!careful && __any_sync(0xffffffffu, real && (finite & 0x7fff7fffu)) && lane == 0) sm->again[slot] = 1;
-                // values that are not finite, for the rows that see them (what they were multiplied with does not matter)
-#pragma unroll 1
-                for (int t = 0; careful && t < 2; ++t) {
-#pragma unroll 1
-                    for (int w = 0; w < 4; ++w) {
-#pragma unroll 1
-                        for (uint32_t odd = sm->odd[slot][t][w]; odd; odd &= odd - 1) {
-                            const int key = (it.steps - 1 - t) * kBlock + 32 * w + __ffs(odd) - 1;
-                            if (!real || key > ahead + tok) continue;
-                            const __nv_bfloat16* from = P.v + it.b * P.vs[0] + it.head * P.vs[1] + (it.lo + key) * P.vs[2];
-#pragma unroll 1
-                            for (int c = 0; c < 128; c += 2) {
-                                const uint32_t x = *reinterpret_cast<const uint32_t*>(from + c), y = *reinterpret_cast<const uint32_t*>(to + c);
-                                const float x0 = act_lo<FP16>(x), x1 = act_hi<FP16>(x);
-                                const float y0 = act_lo<FP16>(y) + (isfinite(x0) ? 0.f : x0), y1 = act_hi<FP16>(y) + (isfinite(x1) ? 0.f : x1);
-                                *reinterpret_cast<uint32_t*>(to + c) = pack_act<FP16>(y0, y1);
-                            }
-                        }
-                    }
-                }
-                warp_arrive(BAR(sm->item_empty[slot]));
+            sm->part[slot][g][row] = make_float2(m, l);
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(BAR(sm->sum_full[slot]));
+                mbar_arrive(BAR(sm->item_empty[slot]));
             }
-            sums ^= 1u << other;
         }
     }
     if (bad) {
