@@ -10,7 +10,7 @@
 // 512 bytes come in and 144 leave per token and head (656 with the stored values); at first bound by instructions, so few are
 // spent: the maximum is taken on 16-bit pairs, the codes are the last bits of one fma each and join by multiply-adds.  16 lanes hold a row of
 // K, 16 the row of V, 8 channels a lane: a lane's K codes are one word of the record as it stands, two lanes exchange a halfword for V.
-// 32768 tokens of 8 heads with the stored values (307 MB): 63 us, 4.8 TB/s; with a division, four rows a warp and logical operations 103 us.
+// 32768 tokens of 8 heads with the stored values (307 MB): 61.5 us, 5.0 TB/s; with a division and logical operations 103 us.
 #include "cache4.cuh"
 #include "host_common.h"
 #include "sm100.cuh"
@@ -193,12 +193,13 @@ extern "C" int fmsa_cache_append(const fmsa_cache_append_args* args, void* strea
     P.cu = cu_seqlens;
     P.rows = static_cast<uint32_t>(rows);
     P.n = static_cast<uint32_t>(n);
-    // Eight rows a warp once they fill the GPU (64 warps an SM), one where latency is what counts.
+    // Four rows a warp once they fill the GPU (64 warps an SM; of 32768 tokens two rows took 74 us, four 61.5, eight 63.6, sixteen 74), one where
+    // latency is what counts.
     const int sms = device_sm_count();
     if (sms <= 0) return FMSA_ERR_CUDA;
-    const bool many = rows >= static_cast<int64_t>(sms) * 64 * 8, fp16 = dtype == FMSA_DTYPE_FP16;
-    const int64_t per_block = kAppendWarps * (many ? 8 : 1);
-    launch_chained(fp16 ? (many ? cache_append_kernel<true, 8> : cache_append_kernel<true, 1>) : (many ? cache_append_kernel<false, 8> : cache_append_kernel<false, 1>),
+    const bool many = rows >= static_cast<int64_t>(sms) * 64 * 4, fp16 = dtype == FMSA_DTYPE_FP16;
+    const int64_t per_block = kAppendWarps * (many ? 4 : 1);
+    launch_chained(fp16 ? (many ? cache_append_kernel<true, 4> : cache_append_kernel<true, 1>) : (many ? cache_append_kernel<false, 4> : cache_append_kernel<false, 1>),
                    static_cast<unsigned>((rows + per_block - 1) / per_block), kAppendWarps * 32, 0, static_cast<cudaStream_t>(stream), P);
     return check_launch();
 }

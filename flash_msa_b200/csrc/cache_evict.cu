@@ -4,12 +4,12 @@
 // next time.)
 //
 // First kernel, a block per (sequence, KV head): the weight of rank keep - recent among the weights as ordered whole numbers by up to three
-// passes of a radix selection (11 + 11 + 10 bits, one histogram in shared memory), then the list of kept tokens in order.  Up to kHeld * 512
-// tokens the numbers stay in registers, a selection ends with the digit whose keys are just those still needed, and the list comes from one
-// scan of (larger, equal) counts.  (32 sequences of up to 8192 tokens, 8 heads: 14.9 us; bit by bit, one
-// count over the block each, 22.7.)  Of longer sequences kKeysHeld numbers
-// are held in shared memory and more come from L2 again; every warp counts and writes a run of tokens.
-// Second kernel, a block per page that is written: 144 + 4 bytes per token, 44.7 us there: at the memory rate (6.2 TB/s of what passes HBM).
+// histograms of 2048 bins in shared memory, then the list of kept tokens in order.  Up to kHeld * 512 tokens the numbers stay in registers, bins
+// divide the range that is still open, the search ends with the bin whose keys are just those still needed, and the list comes from one
+// scan of (larger, equal) counts.  (32 sequences of up to 8192 tokens, 8 heads: 13.7 us, most of it waiting: lengths, table, weights, and the
+// block's barriers; bins of the keys' upper bits 14.9, bit by bit with one count over the block each 22.7.)  Of longer sequences kKeysHeld numbers
+// are held in shared memory and more come from L2 again, by radix selection (11 + 11 + 10 bits); every warp counts and writes a run of tokens.
+// Second kernel, a block per page that is written: 144 + 4 bytes per token, 44.5 us there: at the memory rate (6.2 TB/s of what passes HBM).
 #include "cache4.cuh"
 #include "host_common.h"
 #include "sm100.cuh"
@@ -55,7 +55,7 @@ template <int HELD>
 __global__ void __launch_bounds__(kHeldThreads, HELD <= 16 ? 2 : 1) cache_select_held_kernel(const EvictParams P) {
     constexpr int kWarps = kHeldThreads / 32;
     __shared__ uint32_t bins[kBins], sums[kWarps], counts[HELD * kWarps];
-    __shared__ uint3 digit;   // the wanted one, keys of larger ones, its own keys
+    __shared__ uint3 digit;   // the wanted bin, keys of larger ones, its own keys
     wait_for_previous_kernel();
     const int seq = blockIdx.x / P.cache.heads, head = blockIdx.x % P.cache.heads, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int length = P.cache.length(seq);
@@ -80,17 +80,33 @@ __global__ void __launch_bounds__(kHeldThreads, HELD <= 16 ? 2 : 1) cache_select
 #pragma unroll
     for (int j = 0; j < HELD; ++j) key[j] = j * kHeldThreads + tid < others ? ordered(__uint_as_float(key[j])) : 0u;
     if (bad) atomicMax(P.cache.status, kStatusBadIndex);
-    // the largest number that `need` keys reach: digit by digit, until a digit's keys are just the ones that are still needed
-    uint32_t rank = need ? 0u : 0xffffffffu, mask = 0, rest = need;
-    for (int pass = 0; pass < 3 && need; ++pass) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+    // the largest number that `need` keys reach.  Bins divide the range of the keys that are there (weights lie in a few octaves: under the
+    // keys' upper 11 bits most atomics of a warp would meet in the same bins), then the range of one bin, until that holds just the keys that
+    // are still needed, or one number.
+    uint32_t rank = 0xffffffffu, rest = need, lo = 0xffffffffu, width = 0;   // of keys from lo to lo + width - 1
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) {
+        lo = min(lo, key[j] - 1);    // (0 is none, and goes round)
+        width = max(width, key[j]);
+    }
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    width = __reduce_max_sync(0xffffffffu, width);
+    if (lane == 0) {
+        sums[warp] = lo;
+        counts[warp] = width;
+    }
+    __syncthreads();
+    lo = __reduce_min_sync(0xffffffffu, sums[lane % kWarps]) + 1;
+    width = __reduce_max_sync(0xffffffffu, counts[lane % kWarps]) - lo + 1;
+    while (rest) {                   // at most three times: 11 bits of the range each
+        const int shift = max(21 - __clz(width - 1), 0);
         for (int i = tid; i < kBins; i += kHeldThreads) bins[i] = 0;
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < HELD; ++j)
-            if (key[j] && (key[j] & mask) == rank) atomicAdd(&bins[(key[j] >> shift) & ((1u << bits) - 1)], 1u);
+            if (key[j] - lo < width) atomicAdd(&bins[(key[j] - lo) >> shift], 1u);
         __syncthreads();
-        // from the largest digit down: a thread has kRun bins
+        // from the largest bin down: a thread has kRun
         constexpr int kRun = kBins / kHeldThreads;
         uint32_t n[kRun], sum = 0;
 #pragma unroll
@@ -103,7 +119,7 @@ __global__ void __launch_bounds__(kHeldThreads, HELD <= 16 ? 2 : 1) cache_select
         if (lane == 31) sums[warp] = at;
         __syncthreads();
         const uint32_t w = lane < kWarps ? sums[lane] : 0;
-        at += __reduce_add_sync(0xffffffffu, lane < warp ? w : 0) - sum;   // keys of larger digits
+        at += __reduce_add_sync(0xffffffffu, lane < warp ? w : 0) - sum;   // keys of larger bins
 #pragma unroll
         for (int y = 0; y < kRun; ++y) {
             if (at < rest && rest <= at + n[y]) digit = make_uint3(kBins - 1 - kRun * tid - y, at, n[y]);
@@ -111,13 +127,15 @@ __global__ void __launch_bounds__(kHeldThreads, HELD <= 16 ? 2 : 1) cache_select
         }
         __syncthreads();
         const uint3 d = digit;
-        rank |= d.x << shift;
-        mask |= ((1u << bits) - 1) << shift;
+        lo += d.x << shift;
+        rank = lo;
         rest -= d.y;
         if (rest == d.z) {
-            --rank;       // (all keys from here on: none is equal to the number below)
+            --rank;       // (all keys from here on: none is equal to the number below, but for some that there is no room for)
             break;
         }
+        if (shift == 0) break;
+        width = 1u << shift;
     }
     // Kept: keys above `rank`, the first ones equal to it as far as there is room, and the last tokens.  Counts of both in one word.
     uint32_t mine[HELD];       // before this token, in its row of 32
