@@ -444,6 +444,34 @@ def test_pages_that_do_not_exist(fm):
     assert torch.isfinite(out.float()).all()
 
 
+def test_pages_that_do_not_exist_for_many_rows(fm):
+    cache, table, ls, g = pool(fm, [300, 300], 1, seed=12)
+    q = torch.randn(2, 40, 1, 128, generator=g, device="cuda").to(torch.bfloat16)
+    want = fm.flash_msa_cache_func(q, cache, table, ls, SCALE)
+    before = cache.clone()
+    for bad in (-1, cache.shape[0], 2 ** 31 - 1):
+        t = table.clone()
+        t[1, 1] = bad
+        w = torch.zeros(cache.shape[0], 1, 128, device="cuda")
+        for weights in (None, w):
+            with pytest.raises(RuntimeError):
+                fm.flash_msa_cache_func(q, cache, t, ls, SCALE, weights=weights)
+        unused = [p for p in range(cache.shape[0]) if p not in t.flatten().tolist()]
+        assert (w[unused] == 0).all()
+    assert torch.equal(cache, before) and torch.equal(fm.flash_msa_cache_func(q, cache, table, ls, SCALE), want)
+
+
+@pytest.mark.parametrize("hq", [4, 12, 24])
+def test_lengths_outside_the_table(fm, hq):
+    """Below zero is zero; beyond what the table can hold is that."""
+    cache, table, ls, g = pool(fm, [256, 256, 256], 1, seed=14)
+    q = torch.randn(3, hq, 1, 128, generator=g, device="cuda").to(torch.bfloat16)
+    odd = torch.tensor([-(2 ** 31), 2 ** 31 - 1, 257], dtype=torch.int32, device="cuda")
+    got = fm.flash_msa_cache_func(q, cache, table, odd, SCALE)
+    assert torch.equal(got, fm.flash_msa_cache_func(q, cache, table, torch.tensor([0, 256, 256], dtype=torch.int32, device="cuda"), SCALE))
+    assert (got[0] == 0).all()
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # eviction
 # ---------------------------------------------------------------------------------------------------------------------
