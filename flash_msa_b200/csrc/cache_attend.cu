@@ -1,4 +1,5 @@
-// Attention over the cache held in 4 bits: the last few tokens of every sequence, their heads sharing KV heads.
+// Attention over the cache held in 4 bits: the last few tokens of every sequence, their heads sharing KV heads.  Here up to 16 query rows to a
+// KV head, and the merging of what is cut; cache_rows.cu has the others (form_of() chooses).
 //
 // 144 bytes per token and KV head are read once, whatever the number of query rows (heads of the group x new tokens); beside HBM it is
 // bound by the instructions per nibble.  So:
@@ -847,10 +848,14 @@ __global__ void __launch_bounds__(kWeightWarps * 32, 2) cache_weights_kernel(con
 struct AttendSpace {
     int64_t prefix, parts, o_part, ml_part, lse, bytes;
 };
-int tiles_for(int64_t rows) { return rows <= 8 ? 1 : rows < kRowsMin ? 2 : rows_of_block(rows) / 8; }   // eights of rows of a block
-int teams_for(int tiles) { return tiles == 1 ? kTeams<1> : tiles == 2 ? kTeams<2> : 1; }              // ranges of a CTA
-AttendSpace carve_attend(int seqs, int Hq, int heads, int n, int grid) {
-    const int64_t rows = static_cast<int64_t>(Hq / heads) * n, block = 8 * tiles_for(rows);
+// How a call is done: eights of rows of a block; whether a page is unpacked into shared memory (cache_rows.cu); ranges of a CTA; CTAs of a
+// cluster that shares a pair of sequence and KV head (0: none).
+struct Form {
+    int nt, by_rows, teams, spread;
+};
+Form form_of(const fmsa_cache4& c, int64_t rows, bool weights, int sms);
+AttendSpace carve_attend(const Form& form, int seqs, int heads, int64_t rows, int grid) {
+    const int64_t block = 8 * form.nt;
     AttendSpace w;
     int64_t off = 0;
     auto take = [&](int64_t bytes) {
@@ -860,7 +865,7 @@ AttendSpace carve_attend(int seqs, int Hq, int heads, int n, int grid) {
     };
     w.prefix = take(4LL * (seqs + 1));
     w.parts = take(8LL * seqs * heads * (round_up(rows, block) / block));
-    const int64_t ranges = static_cast<int64_t>(grid) * teams_for(tiles_for(rows));
+    const int64_t ranges = static_cast<int64_t>(grid) * form.teams;
     w.o_part = take(2 * ranges * block * kHeadDim * 4);
     w.ml_part = take(2 * ranges * block * 8);
     w.lse = take(4LL * seqs * heads * round_up(rows, block));
@@ -870,17 +875,22 @@ AttendSpace carve_attend(int seqs, int Hq, int heads, int n, int grid) {
 
 constexpr int kWeightBlocks = 7;   // blocks of rows whose queries the weights kernel holds at once: 44 KB
 static_assert(kWeightBlocks * sizeof(WeightRows<2>) <= 48 * 1024, "more needs an attribute");
-// CTAs that share a pair of sequence and KV head (and block of rows) in a cluster, or 0. A power of two up to 8 that fits the GPU, where a
-// team's pages at the longest lengths the table can hold are at most one more than with all SMs' teams on all pages.  (The weights need
-// what the other form leaves in the workspace.)
-int cluster_spread(const fmsa_cache4& c, int64_t rows, bool weights, int sms) {
-    const int nt = tiles_for(rows), teams = teams_for(nt);
-    const int64_t pairs = static_cast<int64_t>(c.seqs) * c.heads * ((rows + 8 * nt - 1) / (8 * nt));
-    if (weights || nt > 2 || pairs * 2 > sms) return 0;
+Form form_of(const fmsa_cache4& c, int64_t rows, bool weights, int sms) {
+    const int64_t pairs = static_cast<int64_t>(c.seqs) * c.heads, pages = pairs * c.width;   // (at the longest lengths that the table can hold)
+    // Nine to sixteen rows: unpacking into shared memory costs less where a CTA has few pages, and with weights, whose second pass it shortens;
+    // over many pages a tile's shorter way through registers counts.  (Through registers -> this way, 16 rows, 2 heads: one sequence of 4K
+    // 13.0 -> 9.5 us, 32 of 8K 32.8 -> 36.3, with weights 59.0 -> 58.1; 12 rows, 1 head: one of 64K (6.9 pages an SM) 18.1 -> 16.7, 32 of 8K
+    // (13.8) 21.7 -> 24.0, with weights 39.9 -> 36.9.  20 rows, 4 heads, 32 of 8K: 92.5 -> 71.2, with weights 153 -> 111.)
+    if (rows > 16 || (rows > 8 && (weights || pages <= 8LL * sms))) return {rows_of_block(rows) / 8, 1, 1, 0};
+    // Clusters: a power of two up to 8 that fits the GPU, where a team's pages are at most one more than with all SMs' teams on all pages.
+    // (The weights need what the other form leaves in the workspace.)
+    Form f = {rows > 8 ? 2 : 1, 0, rows > 8 ? kTeams<2> : kTeams<1>, 0};
+    if (weights || pairs * 2 > sms) return f;
     int spread = 2;
     while (spread < 8 && pairs * spread * 2 <= sms) spread *= 2;
-    auto rounds = [&](int64_t pages, int64_t by) { return (pages + by - 1) / by; };
-    return rounds(c.width, spread * teams) <= rounds(pairs * c.width, static_cast<int64_t>(sms) * teams) + 1 ? spread : 0;
+    auto rounds = [](int64_t pages, int64_t by) { return (pages + by - 1) / by; };
+    if (rounds(c.width, spread * f.teams) <= rounds(pages, static_cast<int64_t>(sms) * f.teams) + 1) f.spread = spread;
+    return f;
 }
 
 template <int NT>
@@ -888,7 +898,7 @@ bool launch_attend(const AttendParams& P, cudaStream_t st) {
     if (P.spread) {
         const auto kernel = cache_attend_kernel<NT, true>;
         if (!ensure_smem_attr(reinterpret_cast<const void*>(kernel), kAttendSmem<NT>)) return false;
-        launch_clusters(kernel, P.cache.seqs * P.cache.heads * P.blocks * P.spread, P.spread, kAttendThreads<NT>, kAttendSmem<NT>, st, P);
+        launch_clusters(kernel, P.cache.seqs * P.cache.heads * P.spread, P.spread, kAttendThreads<NT>, kAttendSmem<NT>, st, P);
         return true;
     }
     const auto kernel = cache_attend_kernel<NT, false>;
@@ -898,11 +908,11 @@ bool launch_attend(const AttendParams& P, cudaStream_t st) {
 }
 // Everything behind the first kernel.
 template <int NT>
-void launch_combine(const AttendParams& P, cudaStream_t st) {
+void launch_combine(const AttendParams& P, int teams, cudaStream_t st) {
     // A pair is cut into about ranges / pairs parts (+ 1): 16 warps a row where that is many.
     const int64_t pairs = static_cast<int64_t>(P.cache.seqs) * P.cache.heads * P.blocks;
     const int rows = P.rows < 8 * NT ? P.rows : 8 * NT;
-    if (pairs * 16 < P.grid * teams_for(NT)) launch_chained(cache_combine_kernel<NT, 16>, dim3(static_cast<unsigned>(pairs), rows), 512, 0, st, P);
+    if (pairs * 16 < P.grid * teams) launch_chained(cache_combine_kernel<NT, 16>, dim3(static_cast<unsigned>(pairs), rows), 512, 0, st, P);
     else launch_chained(cache_combine_kernel<NT, 1>, dim3(static_cast<unsigned>(pairs), (rows + 3) / 4), 128, 0, st, P);
 }
 template <int NT>
@@ -910,23 +920,20 @@ void launch_weights(const AttendParams& P, cudaStream_t st) {
     const int held = P.blocks < kWeightBlocks ? P.blocks : kWeightBlocks;
     launch_chained(cache_weights_kernel<NT>, device_sm_count() * 2, kWeightWarps * 32, held * sizeof(WeightRows<NT>), st, P, held);
 }
-int launch_all(const AttendParams& P, int nt, cudaStream_t st) {
-    const bool fine = nt == 1 ? launch_attend<1>(P, st) : nt == 2 ? launch_attend<2>(P, st) : launch_attend_rows(P, st);
-    if (!fine) return FMSA_ERR_CUDA;
+int launch_all(const AttendParams& P, const Form& form, cudaStream_t st) {
+    if (!(form.by_rows ? launch_attend_rows(P, st) : form.nt == 1 ? launch_attend<1>(P, st) : launch_attend<2>(P, st))) return FMSA_ERR_CUDA;
     if (!P.spread) {
-        switch (nt) {
-            case 1: launch_combine<1>(P, st); break;
-            case 2: launch_combine<2>(P, st); break;
-            case 4: launch_combine<4>(P, st); break;
-            case 6: launch_combine<6>(P, st); break;
-            default: launch_combine<8>(P, st);
+        switch (form.nt) {
+            case 1: launch_combine<1>(P, form.teams, st); break;
+            case 2: launch_combine<2>(P, form.teams, st); break;
+            case 4: launch_combine<4>(P, form.teams, st); break;
+            case 6: launch_combine<6>(P, form.teams, st); break;
+            default: launch_combine<8>(P, form.teams, st);
         }
     }
     if (P.weights) {
-        if (nt == 1) {
+        if (!form.by_rows) {
             launch_weights<1>(P, st);
-        } else if (nt == 2) {
-            launch_weights<2>(P, st);
         } else if (P.blocks == 1) {
             if (!launch_weights_rows(P, st)) return FMSA_ERR_CUDA;
         } else {   // (a token's rows in several blocks: one kernel has to have them all)
@@ -947,13 +954,18 @@ extern "C" int32_t fmsa_cache_attend_launches(int32_t seqs, int32_t Hq, int32_t 
     if (seqs <= 0 || heads <= 0 || Hq <= 0 || Hq % heads || n <= 0 || width <= 0 || sms <= 0) return -1;
     fmsa_cache4 c = {};
     c.seqs = seqs; c.heads = heads; c.width = width;
-    return weights ? 3 : cluster_spread(c, static_cast<int64_t>(Hq / heads) * n, false, sms) ? 1 : 2;
+    return weights ? 3 : form_of(c, static_cast<int64_t>(Hq / heads) * n, false, sms).spread ? 1 : 2;
 }
 
 extern "C" int64_t fmsa_cache_attend_workspace_bytes(int32_t seqs, int32_t Hq, int32_t heads, int32_t n, int32_t width, int32_t weights) {
     using namespace fmsa;
-    const int32_t launches = fmsa_cache_attend_launches(seqs, Hq, heads, n, width, weights);
-    return launches <= 1 ? launches < 0 ? -1 : 0 : carve_attend(seqs, Hq, heads, n, device_sm_count()).bytes;
+    const int sms = device_sm_count();
+    if (seqs <= 0 || heads <= 0 || Hq <= 0 || Hq % heads || n <= 0 || width <= 0 || sms <= 0) return -1;
+    fmsa_cache4 c = {};
+    c.seqs = seqs; c.heads = heads; c.width = width;
+    const int64_t rows = static_cast<int64_t>(Hq / heads) * n;
+    const Form form = form_of(c, rows, weights != 0, sms);
+    return form.spread ? 0 : carve_attend(form, seqs, heads, rows, sms).bytes;
 }
 
 extern "C" int fmsa_cache_attend(const fmsa_cache_attend_args* args, void* stream) {
@@ -968,17 +980,17 @@ extern "C" int fmsa_cache_attend(const fmsa_cache_attend_args* args, void* strea
     FMSA_REQUIRE(dtype == FMSA_DTYPE_BF16 || dtype == FMSA_DTYPE_FP16);
     FMSA_REQUIRE(aligned16(q->ptr) && q->stride_b % 8 == 0 && q->stride_h % 8 == 0 && q->stride_s % 8 == 0);
     const int64_t rows = static_cast<int64_t>(Hq / cache->heads) * n;
-    const int nt = tiles_for(rows);
-    const int64_t blocks = (rows + 8 * nt - 1) / (8 * nt), items = blocks * cache->heads * cache->seqs;
-    if (items > 0x7fffffffLL || items * cache->width > 0x7fffffffLL) return FMSA_ERR_UNSUPPORTED;   // (units are counted in 32 bits)
     const int sms = device_sm_count();
+    const Form form = form_of(*cache, rows, args->weights != nullptr, sms);
+    const int64_t block = 8 * form.nt, blocks = (rows + block - 1) / block, items = blocks * cache->heads * cache->seqs;
+    if (items > 0x7fffffffLL || items * cache->width > 0x7fffffffLL) return FMSA_ERR_UNSUPPORTED;   // (units are counted in 32 bits)
     AttendParams P = {};
     P.grid = sms;
-    P.spread = sms > 0 ? cluster_spread(*cache, rows, args->weights != nullptr, sms) : 0;
+    P.spread = form.spread;
     AttendSpace w = {};
     if (!P.spread) {
         FMSA_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0);
-        w = carve_attend(cache->seqs, Hq, cache->heads, n, sms > 0 ? sms : 1);
+        w = carve_attend(form, cache->seqs, cache->heads, rows, sms);
         if (args->workspace_bytes < w.bytes) return FMSA_ERR_WORKSPACE;
     }
     if (sms <= 0) return FMSA_ERR_CUDA;
@@ -995,10 +1007,10 @@ extern "C" int fmsa_cache_attend(const fmsa_cache_attend_args* args, void* strea
     P.ml_part = reinterpret_cast<float2*>(ws + w.ml_part);
     P.lse = reinterpret_cast<float*>(ws + w.lse);
     P.Hq = Hq; P.n = n; P.group = Hq / cache->heads; P.rows = static_cast<int32_t>(rows); P.blocks = static_cast<int32_t>(blocks);
-    P.lse_rows = P.blocks * 8 * nt;
+    P.lse_rows = static_cast<int32_t>(blocks * block);
     P.fp16 = dtype == FMSA_DTYPE_FP16; P.accumulate = args->accumulate ? 1 : 0;
     P.scale_log2e = args->scale * kLog2e;
     P.magic = 0x64006400u;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return launch_all(P, nt, st);
+    return launch_all(P, form, st);
 }

@@ -79,10 +79,10 @@ struct Ranges {
 constexpr float kSlack = 8.f, kLift = 6.f;
 
 // cache_rows.cu: pairs of sequence and KV head with many query rows.
-constexpr int kRowsMin = 17, kRowsMost = 64;   // rows that it is for; of a block
-inline int rows_of_block(int64_t rows) {       // blocks of equal size, whole sixteens, at least 32
-    const int64_t blocks = (rows + kRowsMost - 1) / kRowsMost, some = ((rows + blocks - 1) / blocks + 15) / 16 * 16;
-    return some < 32 ? 32 : static_cast<int>(some);
+constexpr int kRowsMost = 64;                  // rows of a block
+inline int rows_of_block(int64_t rows) {       // blocks of equal size, whole sixteens
+    const int64_t blocks = (rows + kRowsMost - 1) / kRowsMost;
+    return static_cast<int>(((rows + blocks - 1) / blocks + 15) / 16 * 16);
 }
 bool launch_attend_rows(const AttendParams& P, cudaStream_t st);    // everything but the merging
 bool launch_weights_rows(const AttendParams& P, cudaStream_t st);   // one block of rows

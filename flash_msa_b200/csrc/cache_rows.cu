@@ -1,7 +1,8 @@
-// Attention over the cache held in 4 bits where many query rows share a KV head (17 and more; cache_attend.cu has the others).
+// Attention over the cache held in 4 bits where many query rows share a KV head (17 and more, or 9 and more over few pages or with weights:
+// form_of() in cache_attend.cu, which has the others).
 //
 // There the instructions per row, not those per nibble, are what counts: scaling sums and probabilities of 16 tokens x 8 rows in registers for
-// mma.sync takes 140 of them.  Here a page is unpacked once, with its scales, into fp16 tiles in shared memory, and tcgen05 has both
+// mma.sync takes 140 of them, and blocks of 16 rows unpack the cache again and again.  Here a page is unpacked once, with its scales, into fp16 tiles in shared memory, and tcgen05 has both
 // operands from there:
 //   S^T = K Q^T     M: the page's 128 tokens, N: the rows (a multiple of 16, up to 64 a block), so that a thread has one token, and what
 //                   belongs to a token - the power of two that its scales were divided by - is one factor of the thread's;
@@ -13,7 +14,13 @@
 //
 // A CTA has a range of the line of pages (of all pairs of sequence and KV head, and blocks of rows); what is cut goes to the workspace as in
 // cache_attend.cu.  One warp loads halves of records, four unpack K, four V, eight have a token and half of the rows a thread, one issues the
-// products, two prepare queries.  WEIGHTS: the probabilities of every token summed over the rows, relative to the log-sum-exps that the first kernel left.
+// products, two prepare queries.  WEIGHTS: the probabilities of every token summed over the rows, relative to the log-sum-exps that the first kernel left (K alone; two
+// groups of four warps have every other page).
+//
+// B=16 Hq=48 Hkv=4 n=4 (48 rows), lengths to 6001 (41 MB): 30.4 us, 3.8 for what was cut, and 17.0 for the weights; in blocks of 16 rows
+// through registers 46 + 4 + 24.  Bound by latency: a page takes 2600 cycles in the warps that have tokens (500 for S out of tensor memory, 550
+// for the common decision on the reference, 780 for probabilities, the rest barriers and fences) and 2200 in those that unpack (950 for
+// the codes), at a third of the issue rate; 8000 cycles go by before the first page is multiplied and 3000 at the end.
 #include "cache_attend.cuh"
 #include "host_common.h"
 #include "sm100.cuh"
@@ -31,12 +38,12 @@ static_assert(kKScales == 8192 && kVCodes == kRawBytes && kVScales == kRawBytes 
 
 template <int N>
 struct RowsCtrl {
-    uint64_t raw_full[kRawParts], raw_empty[kRawParts], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], s_empty[2], p_full[2], pv_done[2], q_full[2], q_empty[2], o_free[2];
+    uint64_t raw_full[kRawParts], raw_empty[kRawParts], k_full[2], v_full[2], v_empty[2], s_full[2], s_empty[2], p_full[2], pv_done[2], q_full[2], q_empty[2], o_free[2];
     float4 scale[2][N / 2];          // [slot of queries][two rows]: product -> logit of either row, -reference (WEIGHTS: -log-sum-exp) of either
     float2 alpha[N / 2], delta[N / 2];   // of a raise: the factor for what there is, and by how much
     float part[4][N];                // [warp]: maxima or sums
     float inv[N];
-    float k_factor[2][kPage], v_factor[2][kPage];   // [stage][token]
+    float k_factor[4][kPage], v_factor[4][kPage];   // [page, modulo 4][token]: read before S of the page after the next one is made
     int32_t limit[2][N];             // tokens the row sees, less the sequence's length
     uint32_t odd[kOddSlots];         // a piece has V that is not finite in tokens that some rows do not see
     int32_t first, rest, length;     // sequence in which the range begins, units of it before, its length
@@ -155,9 +162,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1) cache_rows_kernel(const Atten
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(BAR(sm->k_full[i]), 4);
-            mbar_init(BAR(sm->k_empty[i]), 1 + kReaders);   // the product, the warps that have read the factors
             mbar_init(BAR(sm->v_full[i]), 4);
-            mbar_init(BAR(sm->v_empty[i]), 1 + 8);
+            mbar_init(BAR(sm->v_empty[i]), 1);
             mbar_init(BAR(sm->s_full[i]), 1 + (WEIGHTS ? 4 : 8));   // the product, the warps that have written the factors
             mbar_init(BAR(sm->s_empty[i]), kReaders);
             mbar_init(BAR(sm->p_full[i]), 8);
@@ -335,18 +341,14 @@ __global__ void __launch_bounds__(kRowsThreads, 1) cache_rows_kernel(const Atten
                     const bool there = page >= 0 && place < 0;
                     const float old = there && P.accumulate ? *weight : 0.f;
                     wait(BAR(sm->s_full[st]), ph);
-                    const float factor = sm->k_factor[st][token];
+                    const float factor = sm->k_factor[it & 3][token];
                     tc_fence_after_sync();
                     uint32_t s[N / 8][8];
 #pragma unroll
                     for (int i = 0; i < N / 8; ++i) tmem_ld8(tmem_addr(tmem + 64 * st, quarter, 8 * i), s[i]);
                     tmem_ld_wait();
                     tc_fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) {
-                        mbar_arrive(BAR(sm->s_empty[st]));
-                        mbar_arrive(BAR(sm->k_empty[st]));
-                    }
+                    warp_arrive(BAR(sm->s_empty[st]));
                     const float2 f2 = make_float2(factor, factor);
                     float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
@@ -368,7 +370,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) cache_rows_kernel(const Atten
                 }
             } else {
                 wait(BAR(sm->s_full[st]), ph);
-                const float factor_k = sm->k_factor[st][token], factor_v = sm->v_factor[st][token];
+                const float factor_k = sm->k_factor[it & 3][token], factor_v = sm->v_factor[it & 3][token];
                 tc_fence_after_sync();
                 float2 y[H / 2];   // logits less the reference, log2 domain
                 {
@@ -377,12 +379,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) cache_rows_kernel(const Atten
                     for (int i = 0; i < H / 8; ++i) tmem_ld8(tmem_addr(tmem + 64 * st, quarter, low + 8 * i), s[i]);
                     tmem_ld_wait();
                     tc_fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) {
-                        mbar_arrive(BAR(sm->s_empty[st]));
-                        mbar_arrive(BAR(sm->k_empty[st]));
-                        mbar_arrive(BAR(sm->v_empty[st]));
-                    }
+                    warp_arrive(BAR(sm->s_empty[st]));
                     const float2 f2 = make_float2(factor_k, factor_k);
 #pragma unroll
                     for (int c = 0; c < H / 2; ++c) {
@@ -571,10 +568,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) cache_rows_kernel(const Atten
         auto unpack = [&](auto which) {
             constexpr bool is_v = decltype(which)::value;
             uint32_t pieces = 0, n = is_v || (WEIGHTS && group) ? 1 : 0;   // n: parts so far, of either kind
-            if (WEIGHTS && group && at.left > 0) {   // (K of even pages, and of odd ones)
-                pieces += at.last();
-                at.advance(P);
-            }
+            if (WEIGHTS && group && at.left > 0) at.advance(P);   // (K of even pages, and of odd ones)
             for (uint32_t it = WEIGHTS ? group : 0; at.left > 0; it += WEIGHTS ? 2 : 1, n += 2) {
                 const uint32_t st = it & 1, ph = it >> 1 & 1, part = n % kRawParts;
                 wait(BAR(sm->raw_full[part]), n / kRawParts & 1);
@@ -598,9 +592,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1) cache_rows_kernel(const Atten
                 const float factor = token_scales(w, s);
                 const __half2 s01 = __floats2half2_rn(s[0], s[1]), s23 = __floats2half2_rn(s[2], s[3]);
                 const __half2 b01 = __hmul2(s01, __float2half2_rn(-24.f)), b23 = __hmul2(s23, __float2half2_rn(-24.f));
-                wait_idle(BAR((is_v ? sm->v_empty : sm->k_empty)[st]), ph ^ 1, kIdleNs);   // (the first round finds both stages free)
+                // (K goes when S of the page two before is complete, factors and all: nobody arrives there twice.  The first round finds both free)
+                wait_idle(BAR((is_v ? sm->v_empty : sm->s_full)[st]), ph ^ 1, kIdleNs);
                 if (bad) break;
-                (is_v ? sm->v_factor : sm->k_factor)[st][row] = factor;
+                (is_v ? sm->v_factor : sm->k_factor)[it & 3][row] = factor;
                 const uint32_t tile = (is_v ? tile_v : tile_k) + st * kTileBytes + tile_row;
 #pragma unroll 2
                 for (int k = 0; k < 4; ++k) {
@@ -629,12 +624,9 @@ __global__ void __launch_bounds__(kRowsThreads, 1) cache_rows_kernel(const Atten
                     mbar_arrive(BAR(sm->s_full[st]));
                     mbar_arrive(BAR(sm->raw_empty[part]));
                 }
-                pieces += at.last();
+                if (is_v) pieces += at.last();
                 at.advance(P);
-                if (WEIGHTS && at.left > 0) {
-                    pieces += at.last();
-                    at.advance(P);
-                }
+                if (WEIGHTS && at.left > 0) at.advance(P);
             }
         };
         if (!WEIGHTS && group) unpack(IsV<true>());
@@ -668,7 +660,6 @@ __global__ void __launch_bounds__(kRowsThreads, 1) cache_rows_kernel(const Atten
                     tc_fence_after_sync();
                     umma_ss<N, 8, false, false, true>(tmem + 64 * st, tile_k + st * kTileBytes, tile_q + slot * (kPanelBytes / 2), false);   // S^T = K Q^T
                     umma_commit(BAR(sm->s_full[st]));
-                    umma_commit(BAR(sm->k_empty[st]));
                     const bool first = at.begin, last = at.last();
                     if (last) umma_commit(BAR(sm->q_empty[slot]));
                     if (!WEIGHTS) {
@@ -757,6 +748,7 @@ bool launch(const AttendParams& P, cudaStream_t st) {
 template <bool WEIGHTS>
 bool launch(const AttendParams& P, cudaStream_t st) {
     switch (rows_of_block(P.rows)) {
+        case 16: return launch<16, WEIGHTS>(P, st);
         case 32: return launch<32, WEIGHTS>(P, st);
         case 48: return launch<48, WEIGHTS>(P, st);
         default: return launch<64, WEIGHTS>(P, st);

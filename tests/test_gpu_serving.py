@@ -188,7 +188,7 @@ def check_attend(fm, cache, table, ls, lengths, q, sinks=None, weights=None, acc
 @pytest.mark.parametrize("hq,hkv,n,lengths", [
     (1, 1, 1, [1]), (2, 2, 1, [16]), (8, 1, 1, [127, 128, 129]), (4, 2, 1, [0, 5, 0, 1000]), (16, 2, 1, [1000]), (9, 1, 1, [300, 40]),
     (16, 1, 1, [17, 500]), (17, 1, 1, [260]), (6, 3, 2, [2, 130, 1, 0]), (12, 1, 4, [3, 257, 900]), (5, 1, 5, [4, 128, 131]), (40, 2, 3, [333]),
-    (8, 8, 1, [700] * 30), (4, 1, 1, [6001]), (1, 1, 1, [40000])])
+    (8, 8, 1, [700] * 30), (4, 1, 1, [6001]), (1, 1, 1, [40000]), (12, 1, 1, [1500, 0, 1537, 64] * 30), (32, 2, 1, [1300] * 60), (4, 1, 3, [9000])])
 def test_attention(fm, hq, hkv, n, lengths, dtype):
     cache, table, ls, g = pool(fm, lengths, hkv, seed=hq + n)
     q = torch.randn(len(lengths), hq, n, 128, generator=g, device="cuda").to(dtype)
@@ -250,7 +250,8 @@ def test_attention_weights(fm, hq, hkv, n, lengths, sinks, accumulate):
 
 
 @pytest.mark.parametrize("hq,hkv,n,b,width", [(8, 2, 1, 1, 1), (8, 2, 1, 1, 9), (4, 4, 1, 4, 40), (12, 1, 2, 2, 64), (16, 8, 1, 9, 5), (8, 1, 1, 74, 3), (8, 1, 1, 75, 3),
-                                              (4, 4, 1, 40, 70), (24, 1, 1, 1, 300), (2, 1, 1, 700, 2)])
+                                              (4, 4, 1, 40, 70), (24, 1, 1, 1, 300), (2, 1, 1, 700, 2), (12, 1, 1, 32, 40), (32, 2, 1, 37, 17),
+                                              (32, 2, 1, 9, 70)])
 def test_attention_at_every_number_of_launches(fm, hq, hkv, n, b, width):
     """Few pairs of sequence and KV head go to clusters of 8, 4 or 2 blocks, the others to ranges that cut them: lengths up to what the table
     holds, empty ones, and ones of which most blocks have nothing; and more sequences than a block has threads."""
@@ -264,7 +265,7 @@ def test_attention_at_every_number_of_launches(fm, hq, hkv, n, b, width):
     q = torch.randn(b, hq, n, 128, generator=g, device="cuda").to(torch.bfloat16)
     check_attend(fm, cache, table, ls, lengths, q, torch.randn(hq, device="cuda"))
     launches = _lib.load().fmsa_cache_attend_launches(b, hq, hkv, n, width, 0)
-    assert launches == (1 if (b, width) in ((1, 1), (1, 9), (4, 40), (9, 5), (74, 3)) else 2)
+    assert launches == (1 if (b, width) in ((1, 1), (1, 9), (4, 40), (9, 5), (74, 3), (32, 40), (37, 17), (9, 70)) else 2)
 
 
 def test_attention_repeats_and_follows_streams(fm):
