@@ -2,8 +2,8 @@
 // form_of() in cache_attend.cu, which has the others).
 //
 // There the instructions per row, not those per nibble, are what counts: scaling sums and probabilities of 16 tokens x 8 rows in registers for
-// mma.sync takes 140 of them, and blocks of 16 rows unpack the cache again and again.  Here a page is unpacked once, with its scales, into fp16 tiles in shared memory, and tcgen05 has both
-// operands from there:
+// mma.sync takes 140 of them, and blocks of 16 rows unpack the cache again and again.  Here a page is unpacked once, with its scales, into
+// fp16 tiles in shared memory, and tcgen05 has both operands from there:
 //   S^T = K Q^T     M: the page's 128 tokens, N: the rows (a multiple of 16, up to 64 a block), so that a thread has one token, and what
 //                   belongs to a token - the power of two that its scales were divided by - is one factor of the thread's;
 //   O^T += V^T P^T  M: the channels, N: the rows; P goes through shared memory, [token][row] as the threads have it.
@@ -14,8 +14,8 @@
 //
 // A CTA has a range of the line of pages (of all pairs of sequence and KV head, and blocks of rows); what is cut goes to the workspace as in
 // cache_attend.cu.  One warp loads halves of records, four unpack K, four V, eight have a token and half of the rows a thread, one issues the
-// products, two prepare queries.  WEIGHTS: the probabilities of every token summed over the rows, relative to the log-sum-exps that the first kernel left (K alone; two
-// groups of four warps have every other page).
+// products, two prepare queries.  WEIGHTS: the probabilities of every token summed over the rows, relative to the log-sum-exps that the
+// first kernel left (K alone; two groups of four warps have every other page).
 //
 // B=16 Hq=48 Hkv=4 n=4 (48 rows), lengths to 6001 (41 MB): 30.4 us, 3.8 for what was cut, and 17.0 for the weights; in blocks of 16 rows
 // through registers 46 + 4 + 24.  Bound by latency: a page takes 2600 cycles in the warps that have tokens (500 for S out of tensor memory, 550
@@ -33,12 +33,15 @@ constexpr int kRegsTokens = 120, kRegsUnpack = 80, kRegsRest = 80;   // 96 each 
 static_assert(2 * kRegsTokens + 2 * kRegsUnpack + kRegsRest <= 5 * 96, "register re-division must balance");
 constexpr int kOddSlots = 4;
 constexpr uint32_t kIdleNs = 200;
-constexpr int kRawParts = 4, kRawBytes = kRecordBytes / 2;   // halves of a record on their way: K or V, codes and scales (each part always the same warps': a barrier's parity tells two phases apart, not four)
+// Halves of a record on their way, K or V, codes and scales.  (Each part is always the same warps': a barrier's parity tells two phases apart, not
+// four, so everyone who waits for a part has to see each of its phases.)
+constexpr int kRawParts = 4, kRawBytes = kRecordBytes / 2;
 static_assert(kKScales == 8192 && kVCodes == kRawBytes && kVScales == kRawBytes + 8192, "the halves look alike");
 
 template <int N>
 struct RowsCtrl {
-    uint64_t raw_full[kRawParts], raw_empty[kRawParts], k_full[2], v_full[2], v_empty[2], s_full[2], s_empty[2], p_full[2], pv_done[2], q_full[2], q_empty[2], o_free[2];
+    uint64_t raw_full[kRawParts], raw_empty[kRawParts], k_full[2], v_full[2], v_empty[2], s_full[2], s_empty[2];
+    uint64_t p_full[2], pv_done[2], q_full[2], q_empty[2], o_free[2];
     float4 scale[2][N / 2];          // [slot of queries][two rows]: product -> logit of either row, -reference (WEIGHTS: -log-sum-exp) of either
     float2 alpha[N / 2], delta[N / 2];   // of a raise: the factor for what there is, and by how much
     float part[4][N];                // [warp]: maxima or sums

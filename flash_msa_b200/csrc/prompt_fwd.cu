@@ -12,6 +12,12 @@
 // carefully: where the causal edge crosses a block, the group that turns its scores into probabilities first clears V's rows behind the
 // tile's last token in shared memory, sets values that are not finite to zero in the others, and they are added, after the last block, to
 // the rows that do see them.  (Every tile done carefully: B=1 S=8100 Hq=20 Hkv=4 as eleven sequences 72 us, first like this 65.)
+//
+// Two groups of softmax warps pass an item's key blocks to one another; four more warps write its rows while the groups are at the next item
+// (one of the groups did before: 56 us for those eleven sequences, 53.3 now, 660 TFLOP/s).  S=8192 Hq=32 Hkv=8: 440 us alone, 1.25 PFLOP/s, 504 back to
+// back at 1.57 GHz (power); 333 tokens as five sequences 9.4 us, one launch.  Bound by exponentials and issue beside them (a block of
+// 128 keys takes a group about 2900 cycles: 400 for the maximum, 400 to 500 for the hand-over, 1600 to 2250 for exponentials and stores), and, with
+// few key blocks to an item, by the first block of the next item.
 #include "host_common.h"
 #include "sm100.cuh"
 #include "tma_host.h"
@@ -519,8 +525,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
         reg_inc<kPrRegsSoftmax>();
         // =========================== softmax ===========================
         // Thread = row.  The running maximum of a row is handed from group to group, step by step; either group sums the P of its own
-        // steps.  At the end of an item the group that did not have its last step leaves its sum to the other one, which writes the
-        // rows while this one is at the next item's first step.
+        // steps.  At the end of an item both leave their sums to the warps that write its rows.
         const int g = warp >> 2;
         const uint32_t chain_in = BAR(sm->chain[g ^ 1][quarter]), chain_out = BAR(sm->chain[g][quarter]);
         const float2 sc2 = make_float2(P.scale_log2e, P.scale_log2e);
