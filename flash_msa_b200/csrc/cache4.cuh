@@ -12,6 +12,7 @@
 #include <stdint.h>
 
 #include "host_common.h"
+#include "sm100.cuh"
 
 namespace fmsa {
 
@@ -19,7 +20,7 @@ constexpr int kPage = 128;
 constexpr int kKCodes = 0, kKScales = 8192, kVCodes = 9216, kVScales = 17408, kRecordBytes = 18432;
 constexpr int kGroup = 32;   // channels that share a scale
 
-// The cache as its kernels see it; `length` of a sequence is bounded by what its row of the block table can hold.
+// The cache as its kernels see it; `length` of a sequence is bounded by what its row of the block table can hold (and the status word says so).
 struct Cache4 {
     uint8_t* records;         // [pages][heads][kRecordBytes]
     const int32_t* table;     // [seqs][table_stride]
@@ -27,12 +28,16 @@ struct Cache4 {
     int32_t* status;
     int32_t pages, heads, seqs, width, table_stride;
 
-    __device__ __forceinline__ int length(int seq) const { return min(max(lengths[seq], 0), width * kPage); }
+    __device__ __forceinline__ int length(int seq) const {
+        const int n = lengths[seq], most = width * kPage;
+        if (n > most) atomicMax(status, kStatusBadIndex);
+        return min(max(n, 0), most);
+    }
     // Page of a place of a sequence, or -1 (and the status word) where the table does not name one.  0 <= place < width * kPage.
     __device__ __forceinline__ int page(int seq, int at) const {
         const int p = table[static_cast<int64_t>(seq) * table_stride + at];
         if (p >= 0 && p < pages) return p;
-        atomicMax(status, 2);
+        atomicMax(status, kStatusBadIndex);
         return -1;
     }
     __device__ __forceinline__ uint8_t* record(int page, int head) const {

@@ -464,13 +464,20 @@ def test_pages_that_do_not_exist_for_many_rows(fm):
 
 @pytest.mark.parametrize("hq", [4, 12, 24])
 def test_lengths_outside_the_table(fm, hq):
-    """Below zero is zero; beyond what the table can hold is that."""
-    cache, table, ls, g = pool(fm, [256, 256, 256], 1, seed=14)
+    """Below zero is zero; beyond what the table can hold is reported."""
+    cache, table, ls, g = pool(fm, [256, 256, 256], 1, seed=14, spare=3)
     q = torch.randn(3, hq, 1, 128, generator=g, device="cuda").to(torch.bfloat16)
-    odd = torch.tensor([-(2 ** 31), 2 ** 31 - 1, 257], dtype=torch.int32, device="cuda")
-    got = fm.flash_msa_cache_func(q, cache, table, odd, SCALE)
-    assert torch.equal(got, fm.flash_msa_cache_func(q, cache, table, torch.tensor([0, 256, 256], dtype=torch.int32, device="cuda"), SCALE))
-    assert (got[0] == 0).all()
+    w = torch.rand(cache.shape[0], 1, 128, device="cuda")
+    to = table.numel() + torch.arange(3, dtype=torch.int32, device="cuda").view(3, 1)
+    for odd in ([256, 2 ** 31 - 1, 0], [257, 0, 0]):
+        ls = torch.tensor(odd, dtype=torch.int32, device="cuda")
+        for call in (lambda: fm.flash_msa_cache_func(q, cache, table, ls, SCALE), lambda: fm.flash_msa_cache_func(q, cache, table, ls, SCALE, weights=w),
+                     lambda: fm.flash_msa_cache_evict(cache, w, table, ls, to, 100, 5)):
+            with pytest.raises(RuntimeError):
+                call()
+    got = fm.flash_msa_cache_func(q, cache, table, torch.tensor([-(2 ** 31), 256, -1], dtype=torch.int32, device="cuda"), SCALE)
+    assert torch.equal(got, fm.flash_msa_cache_func(q, cache, table, torch.tensor([0, 256, 0], dtype=torch.int32, device="cuda"), SCALE))
+    assert (got[0] == 0).all() and (got[2] == 0).all()
 
 
 # ---------------------------------------------------------------------------------------------------------------------
