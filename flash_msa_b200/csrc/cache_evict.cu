@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(kHeldThreads, HELD <= 16 ? 2 : 1) cache_select
             break;
         }
         if (shift == 0) break;
-        width = 1u << shift;
+        width = min(1u << shift, 0u - lo);   // (not past the largest number, which is NaN's: the 0 of threads without a token would be in it)
     }
     // Kept: keys above `rank`, the first ones equal to it as far as there is room, and the last tokens.  Counts of both in one word.
     uint32_t mine[HELD];       // before this token, in its row of 32
@@ -177,8 +177,8 @@ __global__ void __launch_bounds__(kHeldThreads, HELD <= 16 ? 2 : 1) cache_select
     for (int j = 0; j < HELD; ++j) {
         const int i = j * kHeldThreads + tid;
         const bool more = i < length && (i >= others || key[j] > rank), equal = i < others && key[j] == rank;
-        const uint32_t at = counts[j * kWarps + warp] + mine[j], equals = at >> 16;
-        if (more || (equal && equals < room)) kept[(at & 0xffffu) + min(equals, room)] = i;
+        const uint32_t at = counts[j * kWarps + warp] + mine[j], equals = at >> 16, to = (at & 0xffffu) + min(equals, room);
+        if ((more || (equal && equals < room)) && to < static_cast<uint32_t>(P.keep)) kept[to] = i;
     }
 }
 
@@ -267,7 +267,8 @@ __global__ void __launch_bounds__(kSelectThreads) cache_select_kernel(const Evic
         classify(i0 + lane, more, equal);
         const uint32_t m = __ballot_sync(0xffffffffu, more), e = __ballot_sync(0xffffffffu, equal);
         const uint32_t my_more = c_more + __popc(m & before_lane), my_equal = c_equal + __popc(e & before_lane);
-        if (more || (equal && my_equal < need)) kept[my_more + min(my_equal, need)] = i0 + lane;
+        const uint32_t to = my_more + min(my_equal, need);   // (below keep, unless the weights change meanwhile)
+        if ((more || (equal && my_equal < need)) && to < static_cast<uint32_t>(P.keep)) kept[to] = i0 + lane;
         c_more += __popc(m);
         c_equal += __popc(e);
     }
