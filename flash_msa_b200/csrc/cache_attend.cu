@@ -57,6 +57,8 @@ struct Queries {
     int2 limit[NT][32];      // tokens the row sees, less the sequence's length
 };
 
+constexpr int kNowhere = 0x7fffff80;   // behind every length
+
 template <int NT>
 struct AttendTeam {
     Queries<NT> q[2];
@@ -64,6 +66,7 @@ struct AttendTeam {
     float2 ml[4][8 * NT];            // [warp][row]: (reference, sum)
     float2 total[8 * NT];            // [row]: the team's (in a cluster)
     uint64_t full[kParts], empty[kParts], q_full[2], q_empty[2];
+    int32_t from[kParts / 2];        // first token of the page whose halves are parts 2 i and 2 i + 1; kNowhere if it does not exist: nothing was loaded
     int32_t first, rest, length;     // sequence in which the range begins, units of it before, its length
 };
 template <int NT>
@@ -354,6 +357,7 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
                     const uint32_t bar = BAR(tm->full[part + v]), to = ring + (part + v) * kPartBytes;
                     wait(BAR(tm->empty[part + v]), phase ^ 1);   // (the first round finds all parts free)
                     if (!bad && lane == 0) {                     // (after a wait that ran out nothing is asked for; the others give up too)
+                        if (v == 0) tm->from[part >> 1] = pg < 0 ? kNowhere : (page + i) * kPage;
                         if (pg < 0) {
                             mbar_arrive(bar);
                         } else {
@@ -531,7 +535,7 @@ __global__ void __launch_bounds__(kAttendThreads<NT>, 1) cache_attend_kernel(con
 #pragma unroll 1
             for (int i = 0; i < take; ++i) {
                 wait(BAR(tm->full[part]), phase);
-                const int first = (page + i) * kPage;   // first token of the page
+                const int first = tm->from[part >> 1];   // first token of the page
                 if (!bad && first + tile < length) {
                     const uint8_t* at = smem_raw + (ring - smem_u32(smem_raw)) + part * kPartBytes;
                     if (first + kPage > length - P.n + 1) two_tiles(Bool<true>(), at, first);

@@ -48,6 +48,8 @@ struct RowsCtrl {
     float inv[N];
     float k_factor[4][kPage], v_factor[4][kPage];   // [page, modulo 4][token]: read before S of the page after the next one is made
     int32_t limit[2][N];             // tokens the row sees, less the sequence's length
+    // A page that does not exist: nothing was loaded.  Its tokens' K factors are zero, which no other token's is, and nobody sees them.
+    uint32_t gone[kRawParts];
     uint32_t odd[kOddSlots];         // a piece has V that is not finite in tokens that some rows do not see
     int32_t first, rest, length;     // sequence in which the range begins, units of it before, its length
     int32_t sums[kRowsThreads / 32];
@@ -319,6 +321,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) cache_rows_kernel(const Atten
         float2 l[H / 2];
         uint32_t pieces = 0;
         int begun = 0;            // first page of the piece
+        bool fresh = true;        // no page of the piece so far
         int ids = -1, from = 0;   // pages from `from` on, a lane each
         for (uint32_t it = 0; at.left > 0; ++it, at.advance(P)) {
             const uint32_t st = it & 1, ph = it >> 1 & 1, slot = pieces & 1;
@@ -326,6 +329,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) cache_rows_kernel(const Atten
             const bool edge = (at.page + 1) * kPage > at.length - P.n + 1;   // (some tokens are not seen by some row, or are not there)
             if (at.begin) {
                 begun = at.page;
+                fresh = true;
                 wait(BAR(sm->q_full[slot]), pieces >> 1 & 1);
                 if (!WEIGHTS && at.page == 0 && tid == 0) {   // (the part that begins a pair says where its parts are)
                     const int behind = R.begin(cta + 1) - at.left + at.pages;   // the unit behind the pair's last
@@ -390,12 +394,13 @@ __global__ void __launch_bounds__(kRowsThreads, 1) cache_rows_kernel(const Atten
                         y[c] = f2_fma(f2_mul(f2_from_bits(s[c >> 2][2 * (c & 3)], s[c >> 2][2 * (c & 3) + 1]), f2), make_float2(sc.x, sc.y), make_float2(sc.z, sc.w));
                     }
                 }
-                if (edge) {
+                const bool gone = factor_k == 0.f;   // (of all 128 tokens or of none)
+                if (edge || gone) {
 #pragma unroll
                     for (int c = 0; c < H / 2; ++c) {
                         const int2 lim = *reinterpret_cast<const int2*>(&sm->limit[slot][low + 2 * c]);
-                        if (place >= lim.x) y[c].x = -INFINITY;
-                        if (place >= lim.y) y[c].y = -INFINITY;
+                        if (gone || place >= lim.x) y[c].x = -INFINITY;
+                        if (gone || place >= lim.y) y[c].y = -INFINITY;
                     }
                 }
                 const float lg = static_cast<float>(static_cast<int>(__float_as_uint(factor_v) >> 23) - 127);
@@ -405,8 +410,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1) cache_rows_kernel(const Atten
                     m0 = fmax3(m0, y[c].x, y[c].y);
                     m1 = fmax3(m1, y[c + 1].x, y[c + 1].y);
                 }
-                if (at.begin || any_of_half(half, fmaxf(m0, m1) + lg > kLift + kSlack)) {
-                    // the references: set at a piece's begin, else raised, for every row by what it needs
+                if (fresh || any_of_half(half, fmaxf(m0, m1) + lg > kLift + kSlack)) {
+                    // the references: set by a piece's first page, else raised, for every row by what it needs
                     float v[H];
 #pragma unroll
                     for (int c = 0; c < H; ++c) v[c] = (c & 1 ? y[c >> 1].y : y[c >> 1].x) + lg;
@@ -418,7 +423,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) cache_rows_kernel(const Atten
                     if (token < H) {
                         const int c = low + token;
                         const float top = fmaxf(fmaxf(sm->part[0][c], sm->part[1][c]), fmaxf(sm->part[2][c], sm->part[3][c])) - kLift;
-                        const float by = top < INFINITY && (at.begin ? top > -INFINITY : top > 0.f) ? top : 0.f;
+                        const float by = top < INFINITY && (fresh ? top > -INFINITY : top > 0.f) ? top : 0.f;
                         reinterpret_cast<float*>(sm->delta)[c] = by;
                         reinterpret_cast<float*>(sm->alpha)[c] = fast_exp2(-by);
                         reinterpret_cast<float*>(&sm->scale[slot][c >> 1])[2 + (c & 1)] -= by;
@@ -429,7 +434,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) cache_rows_kernel(const Atten
                         const float2 by = sm->delta[low / 2 + c];
                         y[c] = f2_add(y[c], make_float2(-by.x, -by.y));
                     }
-                    if (at.begin) {
+                    if (fresh) {             // (O is not there yet, or zero)
 #pragma unroll
                         for (int c = 0; c < H / 2; ++c) l[c] = make_float2(0.f, 0.f);
                     } else {
@@ -454,6 +459,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) cache_rows_kernel(const Atten
                         tmem_st_wait();
                     }
                     named_barrier_sync(1 + half, 128);   // (part, alpha and delta may be written again)
+                    fresh &= gone;
                 }
                 if (it >= 1) wait(BAR(sm->pv_done[st ^ 1]), (it - 1) >> 1 & 1);   // (P of the page before has been read)
                 const uint32_t p_at = tile_p + token * 128;
@@ -578,9 +584,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1) cache_rows_kernel(const Atten
                 if (bad) break;
                 const uint32_t raw = smem_u32(raw_at) + part * kRawBytes;
                 uint2 w = ld_shared_v2(raw + 8192 + row * 8);
+                const bool gone = sm->gone[part];
                 if (is_v) {
                     const int place = at.page * kPage + row - at.length;
-                    if (place >= 0) {
+                    if (place >= 0 || gone) {
                         w = make_uint2(0, 0);     // not there
                     } else if (place > -P.n) {    // not seen by all rows: 0 * NaN must not reach the others
                         const uint2 old = w;
@@ -598,7 +605,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) cache_rows_kernel(const Atten
                 // (K goes when S of the page two before is complete, factors and all: nobody arrives there twice.  The first round finds both free)
                 wait_idle(BAR((is_v ? sm->v_empty : sm->s_full)[st]), ph ^ 1, kIdleNs);
                 if (bad) break;
-                (is_v ? sm->v_factor : sm->k_factor)[it & 3][row] = factor;
+                (is_v ? sm->v_factor : sm->k_factor)[it & 3][row] = !is_v && gone ? 0.f : factor;
                 const uint32_t tile = (is_v ? tile_v : tile_k) + st * kTileBytes + tile_row;
 #pragma unroll 2
                 for (int k = 0; k < 4; ++k) {
@@ -689,6 +696,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) cache_rows_kernel(const Atten
                     const uint32_t part = n % kRawParts, bar = BAR(sm->raw_full[part]), to = smem_u32(raw_at) + part * kRawBytes;
                     wait_idle(BAR(sm->raw_empty[part]), (n / kRawParts & 1) ^ 1, kIdleNs);   // (the first round finds all parts free)
                     if (bad || lane) continue;
+                    sm->gone[part] = page < 0;
                     if (page < 0) {
                         mbar_arrive(bar);
                         continue;

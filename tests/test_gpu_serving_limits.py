@@ -10,6 +10,72 @@ from tests.test_gpu_serving import SCALE, fm, pool  # noqa: F401
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture
+def late(fm):  # noqa: F811
+    """Calls that return what they computed; what they met is reported by `check_pending_status()`."""
+    from flash_msa_b200 import api
+    fm.check_pending_status()
+    api.DEBUG_CHECK_STATUS = False
+    yield fm
+    api.DEBUG_CHECK_STATUS = True
+
+
+def reported(fm):
+    with pytest.raises(RuntimeError, match="out-of-range"):
+        fm.check_pending_status()
+    fm.check_pending_status()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# pages that do not exist
+# ---------------------------------------------------------------------------------------------------------------------
+
+def without(table, lengths, gone):
+    """The table and the lengths of the same sequences without their pages gone[i] (None: all of them)."""
+    rows, left = [], []
+    for row, length, p in zip(table.tolist(), lengths, gone):
+        rows.append(row if p is None else row[:p] + row[p + 1:] + [0])
+        left.append(length if p is None else length - min(128, length - 128 * p))
+    return torch.tensor(rows, dtype=torch.int32, device="cuda"), left
+
+
+# The last page only where one row of queries sees every token of it.  Forms: a cluster of either size, ranges of either size, rows of either count.
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("hq,hkv,n,lengths,gone", [
+    (4, 1, 1, [1000, 300], [0, 2]), (4, 1, 2, [1000, 40, 900], [7 - 1, None, 0]), (8, 8, 1, [700] * 30, [i % 6 for i in range(30)]),
+    (12, 1, 1, [4000, 5120] + [5000] * 30, [0, 39, None] + [i for i in range(29)]), (24, 2, 1, [1280] * 60, [i % 10 for i in range(60)]),
+    (24, 1, 1, [700, 100, 1], [0, 0, 0]), (24, 1, 3, [700, 300], [0, 1]), (48, 1, 1, [4000] * 3, [0, 15, 31]), (100, 1, 1, [900, 300], [0, 2]),
+    (1, 1, 1, [40000], [100])])
+def test_tokens_of_pages_that_do_not_exist_are_hidden(late, hq, hkv, n, lengths, gone, weights):
+    """The result is the one without those tokens, whatever the kernels have loaded before: the values that there are lie far below logits of
+    zero (which is what nothing looks like), and everything that was not appended is NaN."""
+    fm = late  # noqa: F811
+    cache, table, ls, g = pool(fm, lengths, hkv, seed=3 * hq + n)
+    mean = torch.stack([R.rows_of(cache, table[0], lengths[0], h, "k").mean(0) for h in range(hkv)]).float()
+    q = torch.randn(len(lengths), hq, n, 128, generator=g, device="cuda")
+    q[:, ::2] -= 20 * mean.repeat_interleave(hq // hkv, 0)[::2].view(1, -1, 1, 128)
+    q = q.to(torch.bfloat16)
+    t2, l2 = without(table, lengths, gone)
+    want, tol, new = R.attend(q, cache, t2, l2, SCALE)
+    for bad in (-1, cache.shape[0], 2 ** 31 - 1):
+        t = table.clone()
+        for i, p in enumerate(gone):
+            if p is not None:
+                t[i, p] = bad
+        w = torch.rand(cache.shape[0], hkv, 128, generator=g, device="cuda") if weights else None
+        before = None if w is None else w.double()
+        out = fm.flash_msa_cache_func(q, cache, t, ls, SCALE, weights=w)
+        reported(fm)
+        assert ((out.view(len(lengths), n, hq, 128).double() - want).abs() <= tol).all()
+        if weights:
+            slack = before.abs() * 2.0 ** -23
+            for (i, h), (x, e) in new.items():
+                at = torch.arange(len(x), device="cuda")
+                before[t2[i].long()[at // 128], h, at % 128] += x
+                slack[t2[i].long()[at // 128], h, at % 128] += e + x * 2.0 ** -20
+            assert ((w.double() - before).abs() <= slack).all()
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # eviction
 # ---------------------------------------------------------------------------------------------------------------------
