@@ -20,7 +20,8 @@ constexpr int kPage = 128;
 constexpr int kKCodes = 0, kKScales = 8192, kVCodes = 9216, kVScales = 17408, kRecordBytes = 18432;
 constexpr int kGroup = 32;   // channels that share a scale
 
-// The cache as its kernels see it; `length` of a sequence is bounded by what its row of the block table can hold (and the status word says so).
+// The cache as its kernels see it.  A sequence whose length is beyond what its row of the block table can hold counts as empty (and the status
+// word says so): where its last tokens are is not known, so nothing of it is read or written.
 struct Cache4 {
     uint8_t* records;         // [pages][heads][kRecordBytes]
     const int32_t* table;     // [seqs][table_stride]
@@ -29,9 +30,12 @@ struct Cache4 {
     int32_t pages, heads, seqs, width, table_stride;
 
     __device__ __forceinline__ int length(int seq) const {
-        const int n = lengths[seq], most = width * kPage;
-        if (n > most) atomicMax(status, kStatusBadIndex);
-        return min(max(n, 0), most);
+        const int n = lengths[seq];
+        if (n > width * kPage) {
+            atomicMax(status, kStatusBadIndex);
+            return 0;
+        }
+        return max(n, 0);
     }
     // Page of a place of a sequence, or -1 (and the status word) where the table does not name one.  0 <= place < width * kPage.
     __device__ __forceinline__ int page(int seq, int at) const {

@@ -78,14 +78,10 @@ __global__ void __launch_bounds__(kAppendWarps * 32) cache_append_kernel(const A
             const int end = P.cu[seq + 1];
             behind = static_cast<int>(j) >= P.cu[seq] && static_cast<int>(j) < end ? end - static_cast<int>(j) : 0;
         }
-        const int64_t at = static_cast<int64_t>(P.cache.lengths[seq]) - behind;
+        const int at = P.cache.length(seq) - behind;
         if (behind > 0 && at >= 0) {
-            if (at < static_cast<int64_t>(P.cache.width) * kPage) {
-                const int page = P.cache.page(seq, static_cast<int>(at / kPage));
-                if (page >= 0) place = (page * P.cache.heads + static_cast<int>(h)) * kPage + static_cast<int>(at % kPage);
-            } else {
-                atomicMax(P.cache.status, kStatusBadIndex);
-            }
+            const int page = P.cache.page(seq, at / kPage);
+            if (page >= 0) place = (page * P.cache.heads + static_cast<int>(h)) * kPage + at % kPage;
         }
     }
     const uint16_t* from = (is_v ? P.v : P.k) + 8 * l;

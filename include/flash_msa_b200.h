@@ -345,8 +345,8 @@ int fmsa_doc_start(const int32_t* boundaries, int32_t n, int32_t per_batch, int3
  * The cache is a pool of pages of FMSA_CACHE_PAGE tokens, records[pages][heads][FMSA_CACHE_RECORD_BYTES]: per KV head K codes
  * [128][64 bytes], K scales bf16 [128][4], V codes [128][64 bytes], V scales bf16 [128][4]; a value is (nibble - 8) * the scale of its
  * token and group of 32 channels (order of the nibbles inside a row: csrc/cache4.cuh).  Sequence i holds lengths[i] tokens, token j in page
- * block_table[i][j / 128] at slot j % 128.  Table and lengths are device memory: nothing waits for the device.  Lengths beyond
- * width * 128 count as that; a page outside 0 .. pages-1 is not touched, no query sees its tokens, and status becomes 2. */
+ * block_table[i][j / 128] at slot j % 128.  Table and lengths are device memory: nothing waits for the device.  A sequence whose length is
+ * beyond width * 128 counts as empty; a page outside 0 .. pages-1 is not touched and no query sees its tokens; for either status becomes 2. */
 #define FMSA_CACHE_PAGE 128
 #define FMSA_CACHE_RECORD_BYTES 18432
 typedef struct {

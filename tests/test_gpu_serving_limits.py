@@ -77,6 +77,55 @@ def test_tokens_of_pages_that_do_not_exist_are_hidden(late, hq, hkv, n, lengths,
 
 
 # ---------------------------------------------------------------------------------------------------------------------
+# lengths beyond the table
+# ---------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("hq", [4, 12, 24, 100])
+@pytest.mark.parametrize("far", [257, 300, 2 ** 31 - 1])
+def test_sequences_longer_than_their_row_of_the_table_count_as_empty(late, hq, far):
+    """In every call: nothing of them is read, weighed, stored or copied, and the calls say so; the others are what they are."""
+    fm = late  # noqa: F811
+    cache, table, ls, g = pool(fm, [256, 256, 40, 256], 1, seed=14, spare=8)
+    lengths = [256, 0, 40, 0]
+    odd = torch.tensor([256, far, 40, far], dtype=torch.int32, device="cuda")
+    q = torch.randn(4, hq, 1, 128, generator=g, device="cuda").to(torch.bfloat16)
+    want, tol, new = R.attend(q, cache, table, lengths, SCALE)
+    for accumulate in (None, False, True):
+        w = None if accumulate is None else torch.rand(cache.shape[0], 1, 128, generator=g, device="cuda")
+        before = None if w is None else w.clone()
+        out = fm.flash_msa_cache_func(q, cache, table, odd, SCALE, weights=w, accumulate=bool(accumulate))
+        reported(fm)
+        assert ((out.view(4, 1, hq, 128).double() - want).abs() <= tol).all() and (out[1] == 0).all() and (out[3] == 0).all()
+        if w is not None:
+            touched = torch.zeros(w.shape, dtype=torch.bool, device="cuda")
+            for (i, h), (x, _) in new.items():
+                at = torch.arange(len(x), device="cuda")
+                touched[table[i].long()[at // 128], h, at % 128] = True
+            assert torch.equal(w[~touched], before[~touched])
+    # eviction
+    w = torch.rand(cache.shape[0], 1, 128, generator=g, device="cuda")
+    old, old_w = cache.clone(), w.clone()
+    to = table.numel() + torch.arange(4, dtype=torch.int32, device="cuda").view(4, 1)
+    new_lengths, kept = fm.flash_msa_cache_evict(cache, w, table, odd, to, 100, 7)
+    reported(fm)
+    assert new_lengths.tolist() == [100, 0, 40, 0] and (kept[1] == -1).all() and (kept[3] == -1).all()
+    rest = [p for p in range(cache.shape[0]) if p not in (int(to[0]), int(to[2]))]
+    assert torch.equal(cache[rest], old[rest]) and torch.equal(w[rest], old_w[rest])
+    # new tokens: as many as the first sequences have room for, and packed ones
+    cache.copy_(old)
+    k, v = (torch.randn(4, 1, 3, 128, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    for args in (dict(), dict(cu_seqlens=[0, 3, 6, 9, 12])):
+        kk, vv = (t.transpose(0, 1).reshape(1, 1, 12, 128) for t in (k, v)) if args else (k, v)
+        got = fm.flash_msa_cache_append(cache, kk, vv, table, odd, weights=w, return_values=True, **args)
+        reported(fm)
+        assert all((x.view(4, 3, 128)[1::2] == 0).all() and (x.view(4, 3, 128)[::2] != 0).any() for x in got)
+        pages = [int(table[i, p]) for i in (1, 3) for p in range(2)]
+        assert torch.equal(cache[pages], old[pages]) and torch.equal(w[pages], old_w[pages])
+        assert not torch.equal(cache[table[0, 1].long()], old[table[0, 1].long()])
+        cache.copy_(old)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
 # eviction
 # ---------------------------------------------------------------------------------------------------------------------
 
