@@ -35,7 +35,7 @@ __device__ __forceinline__ uint32_t ordered(float w) {
     return w != w ? 0xffffffffu : v;
 }
 
-// Weights of the first `others` tokens of a sequence, as ordered numbers (all of them above 0).
+// Weights of the first `others` tokens of a sequence, as ordered numbers (all of them above 0; tokens of pages that do not exist below all others).
 __device__ __forceinline__ uint32_t weight_of(const EvictParams& P, int seq, int head, int i) {
     const int p = P.cache.page(seq, i / kPage);
     return p < 0 ? 1u : ordered(P.weights[(static_cast<int64_t>(p) * P.cache.heads + head) * kPage + i % kPage]);
@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(kHeldThreads, HELD <= 16 ? 2 : 1) cache_select
     const uint32_t need = P.keep - P.recent; // of these
     uint32_t key[HELD];                      // of token kHeldThreads * j + tid; 0 behind the last
     // (all pages, then all weights, then what they are: with a branch between two loads each would wait for the one before, 16000 cycles
-    // instead of 2000 for 8192 tokens.  A page that does not exist is page 0 until it is found out.)
+    // instead of 2000 for 8192 tokens.  A page that does not exist is page 0 until then.)
     const int32_t* table = P.cache.table + static_cast<int64_t>(seq) * P.cache.table_stride;
     bool bad = false;
 #pragma unroll
@@ -79,7 +79,13 @@ __global__ void __launch_bounds__(kHeldThreads, HELD <= 16 ? 2 : 1) cache_select
     }
 #pragma unroll
     for (int j = 0; j < HELD; ++j) key[j] = j * kHeldThreads + tid < others ? ordered(__uint_as_float(key[j])) : 0u;
-    if (bad) atomicMax(P.cache.status, kStatusBadIndex);
+    if (bad) {   // (here, out of the way of the loads)
+#pragma unroll
+        for (int j = 0; j < HELD; ++j) {
+            const int i = j * kHeldThreads + tid;
+            if (i < others && P.cache.page(seq, i / kPage) < 0) key[j] = 1u;
+        }
+    }
     // the largest number that `need` keys reach.  Bins divide the range of the keys that are there (weights lie in a few octaves: under the
     // keys' upper 11 bits most atomics of a warp would meet in the same bins), then the range of one bin, until that holds just the keys that
     // are still needed, or one number.
@@ -177,8 +183,8 @@ __global__ void __launch_bounds__(kHeldThreads, HELD <= 16 ? 2 : 1) cache_select
     for (int j = 0; j < HELD; ++j) {
         const int i = j * kHeldThreads + tid;
         const bool more = i < length && (i >= others || key[j] > rank), equal = i < others && key[j] == rank;
-        const uint32_t at = counts[j * kWarps + warp] + mine[j], equals = at >> 16, to = (at & 0xffffu) + min(equals, room);
-        if ((more || (equal && equals < room)) && to < static_cast<uint32_t>(P.keep)) kept[to] = i;
+        const uint32_t at = counts[j * kWarps + warp] + mine[j], equals = at >> 16;
+        if (more || (equal && equals < room)) kept[(at & 0xffffu) + min(equals, room)] = i;
     }
 }
 
@@ -275,7 +281,7 @@ __global__ void __launch_bounds__(kSelectThreads) cache_select_kernel(const Evic
 }
 
 __global__ void __launch_bounds__(256) cache_move_kernel(const EvictParams P) {
-    __shared__ int64_t from[kPage];      // record index * 128 + slot, or -1
+    __shared__ int64_t from[kPage];      // record index * 128 + slot; -1 behind the last token, -2 (zeros) if its page does not exist
     wait_for_previous_kernel();
     const int tid = threadIdx.x, head = blockIdx.y, seq = blockIdx.z, first = blockIdx.x * kPage;
     const int page = P.to[static_cast<int64_t>(seq) * P.to_stride + blockIdx.x];
@@ -284,9 +290,9 @@ __global__ void __launch_bounds__(256) cache_move_kernel(const EvictParams P) {
         int64_t f = -1;
         const int at = first + tid < P.keep ? P.kept[(static_cast<int64_t>(seq) * P.cache.heads + head) * P.keep + first + tid] : -1;
         const int p = at >= 0 ? P.cache.page(seq, at / kPage) : -1;
-        if (p >= 0) f = (static_cast<int64_t>(p) * P.cache.heads + head) * kPage + at % kPage;
+        if (at >= 0) f = p < 0 ? -2 : (static_cast<int64_t>(p) * P.cache.heads + head) * kPage + at % kPage;
         from[tid] = f;
-        some = f >= 0;
+        some = f != -1;
     }
     if (!__syncthreads_or(some)) return;
     if (page < 0 || page >= P.cache.pages) {
@@ -318,8 +324,13 @@ __global__ void __launch_bounds__(256) cache_move_kernel(const EvictParams P) {
         const int token = (tid >> 3) + 32 * i;
         if (from[token] >= 0) *reinterpret_cast<uint4*>(to + token * 64 + (part < 4 ? kKCodes + part * 16 : kVCodes + (part & 3) * 16)) = x[i];
     }
-    if (fs >= 0) {
-        *reinterpret_cast<uint2*>(to + (tid < kPage ? kKScales : kVScales) + (tid & 127) * 8) = sc;
+    uint8_t* half = to + (tid < kPage ? kKCodes : kVCodes);
+    if (fs == -2) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) reinterpret_cast<uint4*>(half + (tid & 127) * 64)[c] = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
+    }
+    if (fs != -1) {
+        *reinterpret_cast<uint2*>(half + kKScales + (tid & 127) * 8) = sc;
         if (tid < kPage) P.weights[(static_cast<int64_t>(page) * P.cache.heads + head) * kPage + tid] = w;
     }
 }

@@ -292,7 +292,8 @@ def cache_evict(cache, weights, block_table, lengths, new_block_table, keep: int
     """Cuts every sequence to `keep` tokens per KV head: the last `recent` ones, and the others of the largest `weights` (ties: the earlier
     one; NaN counts as the largest).  What stays is copied, in its order and with its weights, to the pages that `new_block_table` (int32
     [sequences, at least keep/128 pages]) names; a sequence of at most `keep` tokens is copied whole.  Those pages must be named by no
-    other row of either table; the old ones are only read, so pages that sequences share stay what they are.
+    other row of either table; the old ones are only read, so pages that sequences share stay what they are.  (Tokens of pages that do not exist,
+    which is reported, count less than any weight and are copied as zeros.)
     Returns (new lengths int32 [B], kept int32 [B, Hkv, keep]: the places the tokens had, -1 behind the last)."""
     keep, recent = int(keep), int(recent)
     if weights is None:

@@ -395,7 +395,8 @@ int fmsa_cache_attend(const fmsa_cache_attend_args* args, void* stream);
 
 /* Eviction by accumulated attention weight: of every sequence and KV head min(lengths[i], keep) tokens stay, the last `recent` ones and
  * the others of largest weight (of equal ones the first, NaN above everything), in their order; they are copied, weights with them, to
- * new_table [seqs][new_width] (pages that no row of block_table names; new_width * 128 >= keep).  new_lengths [seqs];
+ * new_table [seqs][new_width] (pages that no row of block_table names; new_width * 128 >= keep).  Tokens of pages that do not exist stay last,
+ * and are copied as zeros.  new_lengths [seqs];
  * kept int32 [seqs][heads][keep]: where they were, -1 behind the last.  Two launches. */
 typedef struct {
     fmsa_cache4 cache;

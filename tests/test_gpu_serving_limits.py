@@ -166,3 +166,38 @@ def test_evict_with_more_nan_than_room(fm, lengths, hkv, keep, recent, share):
     """Weights that are NaN for more tokens than stay (a query row that is not finite leaves them), and finite positive ones: the first of the
     NaN ones stay, and nothing is written behind a list."""
     evict_and_check(fm, lengths, hkv, keep, recent, some_nan(share), seed=41)
+
+
+@pytest.mark.parametrize("keep", [130, 1000])
+@pytest.mark.parametrize("length,width", [(1100, 9), (1100, 40), (1100, 200), (1100, 300), (40000, 313)])
+def test_evict_takes_tokens_of_pages_that_do_not_exist_last(late, length, width, keep):
+    """Whichever kernel the width of the table asks for, and whatever the first page of the pool holds.  What has to stay all the same is copied
+    as zeros."""
+    fm = late  # noqa: F811
+    recent, gone = 30, [0, 3, 4]
+    if length > 2000:
+        gone = list(range(2, 270))      # (five thousand others)
+    cache, table, ls, g = pool(fm, [length], 2, seed=51, spare=8)
+    to = (cache.shape[0] - 8 + torch.arange(8, dtype=torch.int32, device="cuda")).view(1, 8)
+    w = torch.randn(cache.shape[0], 2, 128, generator=g, device="cuda")
+    w[0] += 10
+    ref = w.clone()
+    t = torch.full((1, width), -1, dtype=torch.int32, device="cuda")
+    t[:, :table.shape[1]] = table
+    for p, bad in zip(gone, (-1, 2 ** 31 - 1, cache.shape[0]) * len(gone)):
+        ref[table[0, p].long()] = -math.inf
+        t[0, p] = bad
+    want = R.evict(ref, table, [length], keep, recent)
+    old, old_w = cache.clone(), w.clone()
+    cache[to[0].long()] = 0xFF
+    new_lengths, kept = fm.flash_msa_cache_evict(cache, w, t, ls, to, keep, recent)
+    reported(fm)
+    assert new_lengths.tolist() == [keep] and all(kept[0, h].tolist() == want[0, h] for h in range(2))
+    for h in range(2):
+        at, j = torch.tensor(want[0, h], device="cuda"), torch.arange(keep, device="cuda")
+        there = torch.tensor([x // 128 not in gone for x in want[0, h]], device="cuda")
+        assert there.all() == (keep == 130 or length > 2000)
+        for which in "kv":
+            rows = R.rows_of(cache, to[0], keep, h, which)
+            assert torch.equal(rows, R.rows_of(old, table[0], length, h, which)[at] * there.view(-1, 1).double())
+        assert torch.equal(w[to[0].long()[j // 128], h, j % 128], old_w[table[0].long()[at // 128], h, at % 128] * there)
