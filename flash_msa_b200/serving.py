@@ -155,7 +155,7 @@ def _require_cuda(device):
 
 
 def _boundaries(cu_seqlens, total, device):
-    """Sequence boundaries int32 [n+1] (or [B, n+1]) on the device.  Those in host memory are checked and travel with a kernel launch; those
+    """Sequence boundaries int32 [n+1] (or [B, n+1]) on the device.  Those in host memory are checked and travel with kernel launches; those
     in device memory are taken as they are: nothing waits for them, and whatever they hold, no kernel leaves its tensors for it."""
     if isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.device.type == "cuda":
         if cu_seqlens.device != device:
@@ -169,12 +169,18 @@ def _boundaries(cu_seqlens, total, device):
     if (cu[..., 0] != 0).any() or (cu[..., -1] > total).any() or (cu[..., 1:] < cu[..., :-1]).any():
         raise ValueError("cu_seqlens must rise from 0 to at most the sequence length")
     cu = np.ascontiguousarray(cu, dtype=np.int32)
-    if cu.size > ops.MAX_HOST_BOUNDARIES:
-        return torch.from_numpy(cu).to(device)
     out = torch.empty(cu.shape, dtype=torch.int32, device=device)
     with torch.cuda.device(device):
-        ops._launch("fmsa_boundaries", 1, _lib.load().fmsa_boundaries(cu.ctypes.data, cu.size, out.data_ptr(), ops._stream(device)), device)
+        _send_boundaries(cu.ctypes.data, cu.size, out.data_ptr(), ops._stream(device), device)
     return out
+
+
+def _send_boundaries(src, n, dst, stream, device):
+    """`n` boundaries from host to device memory, as parameters of as many launches as that takes (a copy from memory that is not pinned would
+    wait for the device, and could not be captured)."""
+    for at in range(0, n, ops.MAX_HOST_BOUNDARIES):
+        count = min(n - at, ops.MAX_HOST_BOUNDARIES)
+        ops._launch("fmsa_boundaries", 1, _lib.load().fmsa_boundaries(src + 4 * at, count, dst + 4 * at, stream), device)
 
 
 def cache_empty(n_pages: int, n_kv_heads: int, device="cuda") -> torch.Tensor:

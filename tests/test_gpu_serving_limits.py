@@ -126,6 +126,41 @@ def test_sequences_longer_than_their_row_of_the_table_count_as_empty(late, hq, f
 
 
 # ---------------------------------------------------------------------------------------------------------------------
+# boundaries
+# ---------------------------------------------------------------------------------------------------------------------
+
+def test_many_boundaries_in_host_memory_are_captured(late):
+    """More of them than one launch takes: the calls do not wait for the device, and can be captured."""
+    fm = late  # noqa: F811
+    g = torch.Generator(device="cuda").manual_seed(61)
+    cu = [0] + torch.randint(0, 5, (2000,), generator=torch.Generator().manual_seed(1)).cumsum(0).tolist()
+    n = cu[-1]
+    q, k, v = (torch.randn(1, h, n, 128, generator=g, device="cuda").to(torch.bfloat16) for h in (4, 2, 2))
+    cache = fm.flash_msa_cache_empty(2000, 2)
+    table = torch.arange(2000, dtype=torch.int32, device="cuda").view(2000, 1)
+    ls = torch.tensor([b - a for a, b in zip(cu, cu[1:])], dtype=torch.int32, device="cuda")
+
+    def call():
+        fm.flash_msa_cache_append(cache, k, v, table, ls, cu_seqlens=cu)
+        return fm.flash_msa_prompt_func(q, k, v, cu, SCALE)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    cache.zero_()
+    out.zero_()
+    graph.replay()
+    fm.check_pending_status()
+    want, tol = R.prompt(q, k, v, [cu], SCALE)
+    assert ((out.view(1, n, 4, 128).double() - want).abs() <= tol).all()
+    for i in (0, 1, 895, 896, 897, 1999):
+        for h in range(2):
+            codes, scales = R.quantize(k[0, h, cu[i]:cu[i + 1]])
+            assert torch.equal(R.rows_of(cache, table[i], cu[i + 1] - cu[i], h, "k"), (codes.unflatten(-1, (4, 32)) * scales.unsqueeze(-1)).flatten(-2))
+
+
+# ---------------------------------------------------------------------------------------------------------------------
 # eviction
 # ---------------------------------------------------------------------------------------------------------------------
 

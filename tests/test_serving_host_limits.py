@@ -27,3 +27,27 @@ def test_made_up_addresses_are_kept_from_a_gpu(monkeypatch, there):
     monkeypatch.setattr(torch.cuda, "is_available", lambda: there)
     conftest.pytest_collection_modifyitems(items)
     assert [i.markers for i in items] == [["skip"] if there else [], []]
+
+
+@pytest.mark.parametrize("n", [1, 895, 896, 897, 1792, 5000])
+def test_boundaries_go_in_parts_that_a_launch_holds(monkeypatch, n):
+    """However many there are: every one once, in its place."""
+    import ctypes
+
+    from flash_msa_b200 import ops, serving
+
+    class Library:
+        sent = []
+
+        def fmsa_boundaries(self, src, count, dst, stream):
+            assert 0 < count <= ops.MAX_HOST_BOUNDARIES and stream == 7
+            ctypes.memmove(dst, src, 4 * count)
+            self.sent.append(count)
+            return 0
+    lib = Library()
+    monkeypatch.setattr(_lib, "load", lambda: lib)
+    src, dst = torch.arange(n, dtype=torch.int32), torch.full((n + 2,), -7, dtype=torch.int32)
+    before = ops.LAUNCHES
+    serving._send_boundaries(src.data_ptr(), n, dst.data_ptr() + 4, 7, None)
+    assert torch.equal(dst[1:-1], src) and dst[0] == dst[-1] == -7
+    assert sum(lib.sent) == n and ops.LAUNCHES - before == len(lib.sent) == -(-n // 896)
