@@ -26,7 +26,7 @@ struct AppendParams {
     int64_t kos[3], vos[3];
     float* weights;                            // [pages][heads][128] or null
     const int32_t* cu;                         // [seqs + 1] or null: sequence i is batch row i
-    uint32_t rows, n;
+    uint32_t rows, n, blocks;                  // blocks: that have rows
 };
 
 constexpr int kAppendWarps = 8;
@@ -53,6 +53,11 @@ __device__ __forceinline__ float reciprocal(float x) {   // to 2^-23
 template <bool FP16, int ROWS>
 __global__ void __launch_bounds__(kAppendWarps * 32) cache_append_kernel(const AppendParams P) {
     wait_for_previous_kernel();
+    if (P.cu && blockIdx.x == P.blocks) {   // with boundaries there is a block behind the rows, which looks whether they rise
+        for (int i = threadIdx.x; i < P.cache.seqs; i += kAppendWarps * 32)
+            if (bad_boundaries(P.cu, i, static_cast<int>(P.n))) atomicMax(P.cache.status, kStatusBadIndex);
+        return;
+    }
     const int lane = threadIdx.x & 31;
     const uint32_t row0 = (blockIdx.x * kAppendWarps + (threadIdx.x >> 5)) * ROWS;
     if (row0 >= P.rows) return;
@@ -195,7 +200,8 @@ extern "C" int fmsa_cache_append(const fmsa_cache_append_args* args, void* strea
     if (sms <= 0) return FMSA_ERR_CUDA;
     const bool many = rows >= static_cast<int64_t>(sms) * 64 * 4, fp16 = dtype == FMSA_DTYPE_FP16;
     const int64_t per_block = kAppendWarps * (many ? 4 : 1);
+    P.blocks = static_cast<uint32_t>((rows + per_block - 1) / per_block);
     launch_chained(fp16 ? (many ? cache_append_kernel<true, 4> : cache_append_kernel<true, 1>) : (many ? cache_append_kernel<false, 4> : cache_append_kernel<false, 1>),
-                   static_cast<unsigned>((rows + per_block - 1) / per_block), kAppendWarps * 32, 0, static_cast<cudaStream_t>(stream), P);
+                   P.blocks + (cu_seqlens ? 1 : 0), kAppendWarps * 32, 0, static_cast<cudaStream_t>(stream), P);
     return check_launch();
 }

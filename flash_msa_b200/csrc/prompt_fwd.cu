@@ -51,6 +51,13 @@ __device__ __forceinline__ void sequence_of(const PromptParams& P, int b, int i,
     }
 }
 
+// Whether boundaries rise (where they do not, rows can be nobody's or two sequences'): thread `at` of `threads`.
+__device__ __forceinline__ void check_boundaries(const PromptParams& P, int at, int threads) {
+    for (int b = 0; b < (P.per_batch ? P.B : 1); ++b)
+        for (int i = at; i < P.n_seqs; i += threads)
+            if (bad_boundaries(P.cu + static_cast<int64_t>(b) * (P.n_seqs + 1), i, P.S)) atomicMax(P.status, kStatusBadIndex);
+}
+
 // Sets the rows behind the last sequences to zero: thread `at` of `threads`.
 __device__ __forceinline__ void clear_tails(const PromptParams& P, int64_t at, int64_t threads) {
     for (int b = 0; b < P.B; ++b) {
@@ -68,7 +75,9 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const PromptP
     wait_for_previous_kernel();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (blockIdx.x > 0) {
-        clear_tails(P, static_cast<int64_t>(blockIdx.x - 1) * kPlanThreads + tid, static_cast<int64_t>(gridDim.x - 1) * kPlanThreads);
+        const int at = (blockIdx.x - 1) * kPlanThreads + tid, threads = (gridDim.x - 1) * kPlanThreads;
+        clear_tails(P, at, threads);
+        check_boundaries(P, at, threads);
         return;
     }
     for (int i = tid; i < kPlanBins; i += kPlanThreads) bins[i] = 0;
@@ -102,7 +111,7 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const PromptP
     bins[kPlanBins - 2 - 2 * tid] = before + b0;
     if (tid == kPlanThreads - 1) {
         const uint32_t all = before + b0 + b1;
-        if (all > static_cast<uint32_t>(P.cap)) atomicMax(P.status, kStatusBadIndex);   // (boundaries that fall)
+        // (more than `cap` where boundaries fall, which the other blocks report)
         P.counter[0] = 0;
         P.counter[1] = static_cast<int32_t>(min(all, static_cast<uint32_t>(P.cap)));
     }
@@ -328,6 +337,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_fwd_kernel(const __grid_
             PromptItem none = {};
             none.steps = -1;
             if (!bad) publish(none);
+            if (P.direct && P.cu) check_boundaries(P, blockIdx.x * 32 + lane, gridDim.x * 32);
         } else if (warp == 12 && elect_one()) {
             // =========================== tile loads ===========================
             uint32_t st = 0, ph = 1, items = 0;   // stage of the ring, phase bit of its kv_empty, items so far

@@ -32,6 +32,12 @@ constexpr int kStatusWaitTimeout = 1;    // a bounded mbarrier wait gave up
 constexpr int kStatusBadSmem = 3;        // shared or tensor memory does not start where a kernel needs it to
 constexpr int kStatusBadIndex = 2;       // an index read from metadata was out of range
 
+// Boundaries of sequences rise from 0 to at most `rows`: true if those of sequence i do not.
+__device__ __forceinline__ bool bad_boundaries(const int32_t* cu, int i, int rows) {
+    const int lo = cu[i], hi = cu[i + 1];
+    return lo > hi || hi > rows || (i == 0 && lo != 0);
+}
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }

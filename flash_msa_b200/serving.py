@@ -156,7 +156,8 @@ def _require_cuda(device):
 
 def _boundaries(cu_seqlens, total, device):
     """Sequence boundaries int32 [n+1] (or [B, n+1]) on the device.  Those in host memory are checked and travel with kernel launches; those
-    in device memory are taken as they are: nothing waits for them, and whatever they hold, no kernel leaves its tensors for it."""
+    in device memory are not waited for: the kernels report what does not rise from 0 to at most the rows there are, and leave their tensors for
+    nothing."""
     if isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.device.type == "cuda":
         if cu_seqlens.device != device:
             raise ValueError("cu_seqlens must be on the inputs' device")
@@ -328,7 +329,8 @@ def prompt_attention(q, k, v, cu_seqlens, scale: float, sinks=None):
     Returns [B, S, Hq*128].  `cu_seqlens` None: every batch element is one sequence.  Otherwise [n+1], or [B,n+1] for a packing per batch
     element: the rows cu_seqlens[i] .. cu_seqlens[i+1]-1 are sequence i, a row sees the rows of its own sequence up to itself; it starts
     at 0 and may end before S (rows behind the last sequence come back zero, whatever they hold).  Boundaries in host memory are checked;
-    those in device memory are not waited for, and have to rise from 0 to at most S.  `sinks` as in `flash_msa_func`; scale > 0.
+    those in device memory are not waited for, and have to rise from 0 to at most S (which is reported like the status of other calls, and what
+    came back then undefined).  `sinks` as in `flash_msa_func`; scale > 0.
     For serving: it keeps nothing for a backward (training: `flash_msa_func`, `flash_msa_warmup_func`)."""
     b, hq, s, _ = _activation("q", q)
     shape = _activation("k", k)

@@ -358,7 +358,8 @@ typedef struct {
 
 /* Stores new keys and values (B,heads,n,128).  `lengths` count them already.  cu_seqlens NULL: the n rows of batch element i are the last
  * n tokens of sequence i (B = seqs); rows for which a sequence has no place (lengths[i] < n) are left out.  cu_seqlens [seqs+1] (B = 1):
- * rows cu_seqlens[i] .. cu_seqlens[i+1]-1 are the last tokens of sequence i; rows in no sequence are left out.
+ * rows cu_seqlens[i] .. cu_seqlens[i+1]-1 are the last tokens of sequence i; rows in no sequence are left out.  Boundaries that do not rise from
+ * 0 to at most n set status to 2; which rows are stored is then undefined.
  * weights fp32 [pages][heads][128] or NULL: set to zero for the stored tokens.  k_values, v_values: views (B,heads,n,128) that receive the
  * values the cache now holds (zero for rows left out), or with null pointers.  One launch. */
 typedef struct {
@@ -410,7 +411,8 @@ int fmsa_cache_evict(const fmsa_cache_evict_args* args, void* stream);
 
 /* Causal attention over whole prompts of any length, grouped heads: q (B,Hq,S,128), k, v (B,Hkv,S,128); out [B][S][Hq*128] contiguous.
  * cu_seqlens NULL: every batch element is one sequence; else int32 [n_seqs+1] on the device (per_batch = 1: [B][n_seqs+1]), rising from
- * 0: rows cu[i] .. cu[i+1]-1 are sequence i, rows behind the last one are set to zero.  Hq/Hkv <= 128.  fmsa_prompt_launches() launches. */
+ * 0 to at most S (others set status to 2, and rows of `out` are then undefined): rows cu[i] .. cu[i+1]-1 are sequence i, rows behind the last one
+ * are set to zero.  Hq/Hkv <= 128.  fmsa_prompt_launches() launches. */
 typedef struct {
     fmsa_tensor q, k, v;
     const int32_t* cu_seqlens;

@@ -160,6 +160,40 @@ def test_many_boundaries_in_host_memory_are_captured(late):
             assert torch.equal(R.rows_of(cache, table[i], cu[i + 1] - cu[i], h, "k"), (codes.unflatten(-1, (4, 32)) * scales.unsqueeze(-1)).flatten(-2))
 
 
+WRONG = [[0, 400, 100, 499], [1, 100, 200, 499], [0, 100, 200, 501], [-5, 0, 200, 499], [0, 2 ** 31 - 1, -2 ** 31, 499], [0, 499, 498, 498], [600, 700, 800, 900]]
+RIGHT = [[0, 100, 200, 499], [0, 0, 0, 0], [0, 500, 500, 500], [0, 0, 0, 500], [0, 1, 2, 3]]
+
+
+@pytest.mark.parametrize("hq,hkv,size", [(4, 2, 1), (8, 8, 20), (4, 2, 2000)])
+@pytest.mark.parametrize("cu,wrong", [(c, True) for c in WRONG] + [(c, False) for c in RIGHT])
+def test_boundaries_in_device_memory_that_do_not_rise_are_reported(late, cu, wrong, hq, hkv, size):
+    """By prompts of few tiles (without a list of them) and of many, for each batch element that has its own, and by packed appends; those that do
+    rise are not."""
+    fm = late  # noqa: F811
+    g = torch.Generator(device="cuda").manual_seed(71)
+    n = 500 * size if size < 1000 else 500
+    scaled = [max(-2 ** 31, min(2 ** 31 - 1, x * (n // 500))) for x in cu]
+    if size == 2000:   # many sequences: what is wrong comes last, or first
+        scaled = ([0] * 1200 + scaled) if cu[0] == 0 else scaled + [scaled[-1]] * 1200
+    at = torch.tensor(scaled, dtype=torch.int32, device="cuda")
+    q, k, v = (torch.randn(2, h, n, 128, generator=g, device="cuda").to(torch.bfloat16) for h in (hq, hkv, hkv))
+    good = torch.zeros_like(at)
+    for given, bad in ((at, wrong), (torch.stack([good, at]), wrong), (torch.stack([at, good]), wrong), (good, False)):
+        fm.flash_msa_prompt_func(q, k, v, given, SCALE)
+        if bad:
+            reported(fm)
+        else:
+            fm.check_pending_status()
+    seqs = len(scaled) - 1
+    cache = fm.flash_msa_cache_empty(200, hkv)
+    table = torch.zeros(seqs, 200, dtype=torch.int32, device="cuda")      # (what goes where does not matter here)
+    fm.flash_msa_cache_append(cache, k[:1], v[:1], table, torch.full((seqs,), 25000, dtype=torch.int32, device="cuda"), cu_seqlens=at)
+    if wrong:
+        reported(fm)
+    else:
+        fm.check_pending_status()
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # eviction
 # ---------------------------------------------------------------------------------------------------------------------
