@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from tests import serving_ref as R
-from tests.test_gpu_serving import SCALE, fm, pool  # noqa: F401
+from tests.test_gpu_serving import SCALE, append_reference, check_attend, fm, layout, pool  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -74,6 +74,174 @@ def test_tokens_of_pages_that_do_not_exist_are_hidden(late, hq, hkv, n, lengths,
                 before[t2[i].long()[at // 128], h, at % 128] += x
                 slack[t2[i].long()[at // 128], h, at % 128] += e + x * 2.0 ** -20
             assert ((w.double() - before).abs() <= slack).all()
+
+
+@pytest.mark.parametrize("hq", [4, 24])
+def test_calls_with_pages_that_do_not_exist_write_nothing_else(late, hq):
+    """The pool and the weights, byte by byte, and the next call on the same pool."""
+    fm = late  # noqa: F811
+    lengths = [300, 300]
+    cache, table, ls, g = pool(fm, lengths, 1, seed=12, spare=4)
+    q = torch.randn(2, hq, 1, 128, generator=g, device="cuda").to(torch.bfloat16)
+    k, v = (torch.randn(2, 1, 200, 128, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    weights = torch.rand(cache.shape[0], 1, 128, generator=g, device="cuda")
+    for bad in (-1, cache.shape[0], 2 ** 31 - 1):
+        t = table.clone()
+        t[1, 1] = bad
+        old, w = cache.clone(), weights.clone()
+        fm.flash_msa_cache_func(q, cache, t, ls, SCALE, weights=w)
+        reported(fm)
+        named = [int(x) for x in t.flatten() if 0 <= int(x) < cache.shape[0]]
+        others = [p for p in range(cache.shape[0]) if p not in named]
+        assert torch.equal(cache, old) and torch.equal(w[others], weights[others])
+        # (a list that leads nowhere: nothing is moved)
+        w = weights.clone()
+        nowhere = torch.tensor([[bad], [bad]], dtype=torch.int32, device="cuda")
+        fm.flash_msa_cache_evict(cache, w, table, ls, nowhere, 100, 5)
+        reported(fm)
+        assert torch.equal(cache, old) and torch.equal(w, weights)
+        # (tokens 100 .. 299 of both sequences, of which those on the page that there is not are left out)
+        got = fm.flash_msa_cache_append(cache, k, v, t, ls, weights=w, return_values=True)
+        reported(fm)
+        want, vals = append_reference(old, k, v, t, lengths, lambda i, j: None if i == 1 and (100 + j) // 128 == 1 else (i, 100 + j))
+        assert torch.equal(cache.cpu(), want)
+        for x, val in zip(got, vals):
+            assert torch.equal(x.cpu(), val.to(torch.float32).to(x.dtype))
+        for i in range(2):
+            for j in range(100, 300):
+                if (i, j // 128) != (1, 1):
+                    assert w[t[i, j // 128].long(), 0, j % 128] == 0
+        assert int((w != weights).sum()) <= 400 - 128
+        check_attend(fm, cache, table, ls, lengths, q)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# queries and values, in every form
+# ---------------------------------------------------------------------------------------------------------------------
+
+# clusters and ranges of eight and of sixteen rows, rows through shared memory in one and in several blocks
+FORMS = {"cluster8": (6, 2, 2, [200, 0, 1]), "range8": (16, 8, 2, [130, 700, 0, 1, 257] * 6), "cluster16": (4, 1, 3, [5120] + [300, 0, 3] * 10),
+         "range16": (8, 2, 3, [1280, 131, 2, 600] * 15), "rows": (24, 2, 2, [200, 0, 1, 700]), "blocks": (50, 1, 3, [200, 2, 0, 900])}
+
+
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("form", list(FORMS))
+def test_query_layouts_in_every_form(fm, form, weights):  # noqa: F811
+    hq, hkv, n, lengths = FORMS[form]
+    cache, table, ls, g = pool(fm, lengths, hkv, seed=81)
+    for dtype in (torch.bfloat16, torch.float16):
+        q = torch.randn(len(lengths), hq, n, 128, generator=g, device="cuda").to(dtype)
+        sinks = torch.randn(hq, generator=g, device="cuda")
+        for x in (layout(q, "bshd"), layout(q, "odd"), layout(q, "wide"), q[:1].expand(q.shape), q[:, :1].expand(q.shape), q[:, :, :1].expand(q.shape)):
+            w = torch.rand(cache.shape[0], hkv, 128, generator=g, device="cuda") if weights else None
+            check_attend(fm, cache, table, ls, lengths, x, sinks, w)
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+def test_values_that_are_not_finite_in_every_form(fm, form):  # noqa: F811
+    """The last token, which only the last query of its sequence sees, and one that all see: other sequences and heads stay what they are bit for
+    bit, and other rows but for their rounding; of V only the group of channels that holds the value shows it, K shows it in all of a row, and so
+    do the weights."""
+    hq, hkv, n, lengths = FORMS[form]
+    cache, table, ls, g = pool(fm, lengths, hkv, seed=82)
+    b, group = len(lengths), hq // hkv
+    q = torch.randn(b, hq, n, 128, generator=g, device="cuda").to(torch.bfloat16)
+    call = lambda w=None: fm.flash_msa_cache_func(q, cache, table, ls, SCALE, weights=w).view(b, n, hkv, group, 128)
+    want = call()
+    seq = max(range(b), key=lambda i: (lengths[i] < 1000, lengths[i]))
+    clean = cache.clone()
+    for at in (lengths[seq] - 1, 5):
+        rows = slice(n - 1, n) if at > 5 else slice(0, n)                 # of the sequence that see the token
+        pairs = torch.ones(b, hkv, dtype=torch.bool, device="cuda")
+        pairs[seq, 0] = False
+
+        def alike(a, b):   # two sums of the same products: both within half a step, and 2^-11 of the values (below 8) for each probability
+            return ((a - b).abs() <= 2.0 ** -7 * b.abs() + 2.0 ** -10 * 8).all()
+        for which in ("v", "k"):
+            cache.copy_(clean)
+            record = cache[table[seq, at // 128].long(), 0]
+            lo = (17408 if which == "v" else 8192) + at % 128 * 8 + 2     # the scale of the token's second group
+            record[lo:lo + 2] = torch.tensor([0xFF, 0x7F], dtype=torch.uint8, device="cuda")
+            got = call()
+            assert torch.equal(got.transpose(1, 2)[pairs], want.transpose(1, 2)[pairs])
+            assert alike(got[seq, :rows.start, 0].float(), want[seq, :rows.start, 0].float())
+            seen = got[seq, rows, 0].float()
+            if which == "k":
+                assert seen.isnan().all()
+            else:
+                assert seen[..., 32:64].isnan().all()
+                left = want[seq, rows, 0].float()
+                for c in (slice(0, 32), slice(64, 128)):
+                    assert alike(seen[..., c], left[..., c])
+            w = torch.zeros(cache.shape[0], hkv, 128, device="cuda")
+            call(w)
+            page = table[seq, :-(-lengths[seq] // 128)].long()
+            mine = w[page, 0].reshape(-1)[:lengths[seq]]
+            assert (mine.isnan().all() if which == "k" and at == 5 else mine.isfinite().all() if which == "v" else mine.isnan().any())
+            w[page, 0] = 0
+            assert w.isfinite().all()
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+def test_groups_of_channels_far_below_the_tokens_largest(fm, form):  # noqa: F811
+    """A group 2^16 below the token's largest keeps its accuracy: as the same values with nothing larger beside them."""
+    hq, hkv, n, lengths = FORMS[form]
+    group = hq // hkv
+    g = torch.Generator(device="cuda").manual_seed(83)
+    total, b = sum(lengths), len(lengths)
+    width = -(-max(lengths) // 128)
+    k, v = (torch.randn(1, hkv, total, 128, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    size = torch.exp2(torch.tensor([0.0, -16.0, -5.0, -11.0], device="cuda")).repeat_interleave(32)
+    cu = torch.tensor([0] + lengths).cumsum(0).tolist()
+    table = torch.arange(b * width, dtype=torch.int32, device="cuda").view(b, width)
+    ls = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    q = torch.randn(b, hq, n, 128, generator=g, device="cuda").to(torch.bfloat16)
+    outs = []
+    for x in (v * size.to(torch.bfloat16), v):
+        cache = fm.flash_msa_cache_empty(b * width, hkv)
+        fm.flash_msa_cache_append(cache, k, x, table, ls, cu_seqlens=cu)
+        outs.append(fm.flash_msa_cache_func(q, cache, table, ls, SCALE).view(b, n, hq, 128)[..., 32:64].float())
+    got, want, top = outs[0] * 2.0 ** 16, outs[1], torch.zeros(b, n, hq, 1, device="cuda")
+    for i, length in enumerate(lengths):          # every row's largest probability
+        for h in range(hkv if length else 0):
+            x = q[i, h * group:(h + 1) * group].double().reshape(group * n, 128)
+            seen = torch.arange(length, device="cuda") < (length - n + 1 + torch.arange(n, device="cuda").repeat(group)).view(-1, 1)
+            p = R.softmax((x @ R.rows_of(cache, table[i], length, h, "k").T * SCALE).masked_fill(~seen, -math.inf))
+            top[i, :, h * group:(h + 1) * group] = p.amax(-1).view(group, n).T.unsqueeze(-1).float()
+    # Both are sums of the same products, exact powers of two apart: half a step each, and the rounding of every probability times V's scale to fp16,
+    # 2^-11 of the sum of magnitudes each.  What that loses below fp16's normal numbers is at most 2^-25 a token where the token's largest scale
+    # makes 2^6 of the row's largest probability: here 2^-31 * 2^16 of a largest value for each token.
+    size = v.float().abs().amax()
+    assert ((got - want).abs() <= 2.0 ** -10 * size + 2.0 ** -7 * want.abs() + max(lengths) * 2.0 ** -15 * top * size).all()
+    assert top.amax() > 0 and want.abs().amax() > 0.1
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_prefill_and_steps_against_what_the_cache_holds(fm, dtype):  # noqa: F811
+    """A prompt attended to on the values that the cache gives back, then steps over the cache: each against 64 bits within its own tolerance, which
+    a result of zeros is not."""
+    g = torch.Generator(device="cuda").manual_seed(23)
+    s, new, hq, hkv = 300, 5, 8, 2
+    q, k, v = (torch.randn(1, h, s + new, 128, generator=g, device="cuda").to(dtype) for h in (hq, hkv, hkv))
+    cache = fm.flash_msa_cache_empty(3, hkv)
+    table = torch.tensor([[2, 0, 1]], dtype=torch.int32, device="cuda")
+    at = lambda n: torch.tensor([n], dtype=torch.int32, device="cuda")
+    ks, vs = fm.flash_msa_cache_append(cache, k[:, :, :s], v[:, :, :s], table, at(s), return_values=True)
+    for x, which in ((ks, "k"), (vs, "v")):
+        for h in range(hkv):
+            held = R.rows_of(cache, table[0], s, h, which)
+            assert torch.equal(x[0, h], held.to(torch.float32).to(dtype))
+            given = (k if which == "k" else v)[0, h, :s].double().unflatten(-1, (4, 32))
+            top = given.abs().amax(-1, keepdim=True)      # (half a step, and the rounding of the scale times the largest code)
+            assert ((held.unflatten(-1, (4, 32)) - given).abs() <= top / 14 * (1 + 2.0 ** -8) + top * 2.0 ** -8).all()
+    out = fm.flash_msa_prompt_func(q[:, :, :s], ks, vs, None, SCALE).view(1, s, hq, 128).double()
+    want, tol = R.prompt(q[:, :, :s], ks, vs, [[0, s]], SCALE)
+    assert ((out - want).abs() <= tol).all() and (want.abs() > tol).double().mean() > 0.9
+    for i in range(s, s + new):
+        fm.flash_msa_cache_append(cache, k[:, :, i:i + 1], v[:, :, i:i + 1], table, at(i + 1))
+        want, tol, _ = R.attend(q[:, :, i:i + 1], cache, table, [i + 1], SCALE)
+        out = fm.flash_msa_cache_func(q[:, :, i:i + 1], cache, table, at(i + 1), SCALE).view(1, 1, hq, 128).double()
+        assert ((out - want).abs() <= tol).all() and (want.abs() > tol).double().mean() > 0.9
 
 
 # ---------------------------------------------------------------------------------------------------------------------
@@ -214,6 +382,8 @@ def evict_and_check(fm, lengths, hkv, keep, recent, fill_weights, seed, width=No
         assert int(new_lengths[i]) == n
         for h in range(hkv):
             assert kept[i, h].tolist() == want[i, h] + [-1] * (keep - n)
+            if n == 0:
+                continue
             at, j = torch.tensor(want[i, h], device="cuda"), torch.arange(n, device="cuda")
             for which in "kv":
                 assert torch.equal(R.rows_of(cache, to[i], n, h, which), R.rows_of(old, table[i], length, h, which)[at])
@@ -270,3 +440,14 @@ def test_evict_takes_tokens_of_pages_that_do_not_exist_last(late, length, width,
             rows = R.rows_of(cache, to[0], keep, h, which)
             assert torch.equal(rows, R.rows_of(old, table[0], length, h, which)[at] * there.view(-1, 1).double())
         assert torch.equal(w[to[0].long()[j // 128], h, j % 128], old_w[table[0].long()[at // 128], h, at % 128] * there)
+
+
+def ties(w, g):
+    return torch.round(w * 4) / 4
+
+
+@pytest.mark.parametrize("fill", [lambda w, g: w, ties, some_nan(0.5), some_nan(0.01)])
+@pytest.mark.parametrize("lengths,hkv,keep,recent", [([20000], 1, 4000, 100), ([1100, 3, 0], 2, 512, 64), ([24676, 24677], 1, 300, 100), ([33000], 1, 32000, 0)])
+def test_evict_under_a_table_beyond_32k_tokens(fm, lengths, hkv, keep, recent, fill):  # noqa: F811
+    """The form for long tables with sequences whose weights fit its shared memory, just so and just not."""
+    evict_and_check(fm, lengths, hkv, keep, recent, fill, seed=42, width=300)
