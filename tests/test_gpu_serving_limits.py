@@ -138,6 +138,51 @@ def test_query_layouts_in_every_form(fm, form, weights):  # noqa: F811
 
 
 @pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("scale", [-0.05, 0.0, 1e-30, 3.0])
+def test_scales_and_sinks_in_every_form(fm, form, scale):  # noqa: F811
+    """Scales of either sign and none; sinks that take everything, or nothing."""
+    hq, hkv, n, lengths = FORMS[form]
+    cache, table, ls, g = pool(fm, lengths, hkv, seed=84)
+    q = torch.randn(len(lengths), hq, n, 128, generator=g, device="cuda").to(torch.bfloat16)
+    for sinks in (None, torch.tensor([-math.inf, -1e30, 1e4, 0.0] * hq, device="cuda")[:hq].contiguous()):
+        out = fm.flash_msa_cache_func(q, cache, table, ls, scale, sinks=sinks)
+        want, tol, _ = R.attend(-q if scale < 0 else q, cache, table, lengths, abs(scale), sinks)
+        assert ((out.view(want.shape).double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+def test_tables_and_pools_that_are_parts_of_others(fm, form):  # noqa: F811
+    """A table of some columns of a wider one, a row that all sequences share, a pool behind other records, keys that heads share by stride 0."""
+    hq, hkv, n, lengths = FORMS[form]
+    cache, table, ls, g = pool(fm, lengths, hkv, seed=85)
+    b, width = table.shape
+    q = torch.randn(b, hq, n, 128, generator=g, device="cuda").to(torch.bfloat16)
+    want = check_attend(fm, cache, table, ls, lengths, q)
+    wide = torch.full((b, width + 5), -1, dtype=torch.int32, device="cuda")
+    wide[:, 3:3 + width] = table
+    part = torch.cat([torch.full_like(cache[:3], 0xFF), cache])[3:]
+    assert torch.equal(fm.flash_msa_cache_func(q, part, wide[:, 3:3 + width], ls, SCALE), want)
+    one = max(range(b), key=lambda i: lengths[i])
+    shared, same = table[one:one + 1].expand(b, width), torch.full_like(ls, lengths[one])
+    check_attend(fm, cache, shared, same, [lengths[one]] * b, q)
+    x = torch.randn(b, 1, 1, 128, generator=g, device="cuda").to(torch.bfloat16)
+    for kv in (x.expand(b, hkv, 2, 128), x[:1].expand(b, hkv, 2, 128)):
+        w = torch.rand(part.shape[0], hkv, 128, generator=g, device="cuda")
+        a, c, w2 = part.clone(), cache.clone(), w.clone()
+        got = fm.flash_msa_cache_append(a, kv, kv, wide[:, 3:3 + width], ls, weights=w, return_values=True)
+        exp = fm.flash_msa_cache_append(c, kv.contiguous(), kv.contiguous(), table, ls, weights=w2, return_values=True)
+        assert torch.equal(a, c) and torch.equal(w, w2) and all(torch.equal(y, z) for y, z in zip(got, exp))
+    to = torch.full((b, 4), -1, dtype=torch.int32, device="cuda")
+    # (the spare page: for the longest sequence, the others are empty)
+    to[:, 1] = torch.where(torch.arange(b, device="cuda") == one, b * width, -1)
+    few = torch.where(torch.arange(b, device="cuda") == one, ls, 0).to(torch.int32)
+    w = torch.rand(cache.shape[0], hkv, 128, generator=g, device="cuda")
+    kept = fm.flash_msa_cache_evict(cache.clone(), w.clone(), wide[:, 3:3 + width], few, to[:, 1:3], 100, 5)[1]
+    ref = R.evict(w, table, few.tolist(), 100, 5)
+    assert all(kept[one, h].tolist() == (ref[one, h] + [-1] * 100)[:100] for h in range(hkv))
+
+
+@pytest.mark.parametrize("form", list(FORMS))
 def test_values_that_are_not_finite_in_every_form(fm, form):  # noqa: F811
     """The last token, which only the last query of its sequence sees, and one that all see: other sequences and heads stay what they are bit for
     bit, and other rows but for their rounding; of V only the group of channels that holds the value shows it, K shows it in all of a row, and so
