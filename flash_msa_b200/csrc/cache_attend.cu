@@ -17,8 +17,9 @@
 //           others): q - 8 by one more fma per pair.
 //   * scales are per token and group, so they are applied to sums (K) and to probabilities (V), not to values.
 // Queries are scaled by a power of two per row to [2^13, 2^14), so that fp16 holds bf16 ones exactly.  Probabilities times V scales are
-// rounded to fp16, relative to the running maximum of (logit + log2 scale): neither large nor tiny values of V leave fp16's range, and the
-// rounding (2^-12) stays below that of the result in either type.
+// rounded to fp16, relative to the running maximum of (logit + log2 scale): neither large nor tiny values of V leave fp16's range. That
+// rounding (2^-11) is an eighth of a bf16 result's own and as large as an fp16 result's.  (A group of channels 2^-r below its token's largest has its
+// products at 2^(6-r): normal numbers down to r = 20.)
 //
 // B=32 Hq=32 Hkv=8, lengths to 8192 (158 MB): 38.4 us and 4.5 us for what was cut, 3.7 TB/s; without its products the first kernel takes
 // 32 us (6 us of them before the first page and behind the last), whatever the depth of the ring.  A tile of 16 tokens takes 300

@@ -6,10 +6,10 @@
 // First kernel, a block per (sequence, KV head): the weight of rank keep - recent among the weights as ordered whole numbers by up to three
 // histograms of 2048 bins in shared memory, then the list of kept tokens in order.  Up to kHeld * 512 tokens the numbers stay in registers, bins
 // divide the range that is still open, the search ends with the bin whose keys are just those still needed, and the list comes from one
-// scan of (larger, equal) counts.  (32 sequences of up to 8192 tokens, 8 heads: 13.7 us, most of it waiting: lengths, table, weights, and the
+// scan of (larger, equal) counts.  (32 sequences of up to 8192 tokens, 8 heads: 13.8 us, most of it waiting: lengths, table, weights, and the
 // block's barriers; bins of the keys' upper bits 14.9, bit by bit with one count over the block each 22.7.)  Of longer sequences kKeysHeld numbers
 // are held in shared memory and more come from L2 again, by radix selection (11 + 11 + 10 bits); every warp counts and writes a run of tokens.
-// Second kernel, a block per page that is written: 144 + 4 bytes per token, 44.5 us there: at the memory rate (6.2 TB/s of what passes HBM).
+// Second kernel, a block per page that is written: 144 + 4 bytes per token, 45 us there: at the memory rate (6.2 TB/s of what passes HBM).
 #include "cache4.cuh"
 #include "host_common.h"
 #include "sm100.cuh"
@@ -23,7 +23,7 @@ struct EvictParams {
     const int32_t* to;          // [seqs][to_stride]
     int32_t* new_lengths;       // [seqs]
     int32_t* kept;              // [seqs][heads][keep]
-    int32_t to_stride, to_width, keep, recent, held;
+    int32_t to_stride, keep, recent, held;
 };
 
 constexpr int kSelectThreads = 1024, kBins = 2048, kKeysHeld = 24576, kHeldThreads = 512, kHeld = 64;
@@ -355,7 +355,6 @@ extern "C" int fmsa_cache_evict(const fmsa_cache_evict_args* args, void* stream)
     P.weights = weights;
     P.to = new_table;
     P.to_stride = static_cast<int32_t>(new_table_stride);
-    P.to_width = new_width;
     P.new_lengths = new_lengths;
     P.kept = kept;
     P.keep = keep;
