@@ -5,7 +5,8 @@ The cache is a pool of pages of 128 tokens (the block of the training path), a u
 owns (`cache_empty`), with a block table int32 [sequences, pages of a sequence] and lengths int32 [sequences] in device memory: no call
 waits for the device, and all of them can be captured in a CUDA graph (after a first call outside of one).  What those tensors hold the
 kernels check: a sequence whose length is beyond its row of the table counts as empty in every call, pages that do not exist are not
-touched and attention passes over their tokens, and either raises, at a later call or in `check_pending_status()`; a length below zero is zero.  Keys and values are symmetric 4-bit codes with a bf16 scale per token and group of 32
+touched and attention passes over their tokens, boundaries in device memory that do not rise leave rows undefined; each of these raises, at a later
+call or in `check_pending_status()`.  A length below zero is zero.  Keys and values are symmetric 4-bit codes with a bf16 scale per token and group of 32
 channels, 144 bytes per token and head instead of 512."""
 from __future__ import annotations
 
